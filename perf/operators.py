@@ -1,0 +1,460 @@
+"""Cases, plain forms and work of the block operators: rotary positions with several axes, the gated
+feed-forward block with its gradients, and the AdamW step over many tensors.
+
+``own`` False computes the operators in their plain form (elementary torch operations in 32 bits, 64 where the
+comments say so); ``own`` True makes the calls a user makes of ``nerf_amd.operators`` and ``nerf_amd.optim``.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+E4M3 = torch.float8_e4m3fn
+BLOCK = 256                      # elements that share one scale of an 8-bit state
+BETA1, BETA2, EPS, LR, DECAY, MAX_NORM, STEPS = 0.9, 0.999, 1e-8, 3e-4, 0.01, 1.0, 1000
+
+
+# ------------------------------------------------------------------------------------------------ cases --
+def listed():
+    return [
+        # one new token of a served model: every layer makes this call once, so its latency is what counts
+        dict(name="rotary one token", op="rotary", batch=1, tokens=1, heads_q=32, heads_k=8, dim=128,
+             sections="16,24,24", dtype="bfloat16", positions="index", ladder="shared", pairs="split",
+             inverse=False, layout="tokens"),
+        # features of the sample points of 2048 rays x 64 samples, at their x, y, z in the scene
+        dict(name="rotary ray samples", op="rotary", batch=1, tokens=131072, heads_q=8, heads_k=0, dim=32,
+             sections="5,5,5", dtype="float32", positions="point", ladder="octaves", pairs="interleaved",
+             inverse=False, layout="tokens"),
+        # part of each head turned, three sequences, an odd number of tokens
+        dict(name="rotary odd lengths", op="rotary", batch=3, tokens=1237, heads_q=10, heads_k=2, dim=80,
+             sections="8,12,12", dtype="float16", positions="index", ladder="axis", pairs="split",
+             inverse=False, layout="tokens"),
+        # gradients of queries and keys of two clips (time, height, width), heads before tokens
+        dict(name="rotary clip gradients", op="rotary", batch=2, tokens=16384, heads_q=24, heads_k=24, dim=128,
+             sections="16,24,24", dtype="bfloat16", positions="index", ladder="shared", pairs="split",
+             inverse=True, layout="heads"),
+        # one token through a block: the weights' bytes are the cost
+        dict(name="block one token", op="block", run="forward", rows=1, width=2048, hidden=5120, out=2048,
+             dtype="bfloat16", activation="silu"),
+        # a training step of a 256-wide block over the samples of 2048 rays x 64
+        dict(name="block ray samples", op="block", run="step", rows=131072, width=256, hidden=512, out=256,
+             dtype="bfloat16", activation="relu"),
+        # odd sizes all over: rows of neither 16 bytes nor whole tiles
+        dict(name="block odd sizes", op="block", run="step", rows=1531, width=1000, hidden=2730, out=1001,
+             dtype="float16", activation="gelu"),
+        # the framework's own type: 32 bits all through
+        dict(name="block 32 bits", op="block", run="step", rows=4096, width=1024, hidden=2816, out=1024,
+             dtype="float32", activation="silu"),
+        # a wide block over a long batch
+        dict(name="block wide", op="block", run="step", rows=8192, width=4096, hidden=10240, out=4096,
+             dtype="bfloat16", activation="silu"),
+        # the two networks that the trainer steps: 44 tensors, from 1 to 81,664 values, clipped to norm 1
+        dict(name="adamw two networks", op="adamw", tensors="networks", layers=2, width=256, dtype="float32",
+             bits=32, clip=True),
+        # a stack of 512-wide blocks with its moments in 8 bits
+        dict(name="adamw 8 bits", op="adamw", tensors="blocks", layers=40, width=512, dtype="float32", bits=8,
+             clip=True),
+        # a large model of 16-bit weights, 32-bit masters and 32-bit moments
+        dict(name="adamw 16-bit weights", op="adamw", tensors="blocks", layers=12, width=2000, dtype="bfloat16",
+             bits=32, clip=False),
+    ]
+
+
+def _spread(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(("rotary", "block", "adamw"))
+    if op == "rotary":
+        dim = rng.choice((32, 48, 64, 80, 96, 128, 160, 192, 256))
+        axes = rng.randint(1, 4)
+        pairs = dim // 2 if rng.random() < 0.6 else rng.randint(axes, dim // 2)
+        cuts = sorted(rng.sample(range(1, pairs), axes - 1))
+        sections = [b - a for a, b in zip([0] + cuts, cuts + [pairs])]
+        heads_q = _spread(rng, 1, 48)
+        heads_k = rng.choice((0, heads_q, max(1, heads_q // 4)))
+        batch = rng.randint(1, 4)
+        most = 200_000_000 // (batch * (heads_q + heads_k) * dim)
+        point = rng.random() < 0.4
+        return dict(op=op, batch=batch, tokens=_spread(rng, 1, min(65536, most)), heads_q=heads_q, heads_k=heads_k,
+                    dim=dim, sections=",".join(map(str, sections)), dtype=rng.choice(sorted(DTYPES)),
+                    positions="point" if point else "index",
+                    # octaves as a positional encoding has them: 2^k pi stays below 2^10 pi
+                    ladder="octaves" if point and max(sections) <= 10 else rng.choice(("axis", "shared")),
+                    pairs=rng.choice(("split", "interleaved")), inverse=rng.random() < 0.5,
+                    layout=rng.choice(("tokens", "heads")))
+    if op == "block":
+        width = _spread(rng, 64, 4096)
+        hidden = int(width * rng.uniform(1.0, 4.0))
+        if rng.random() < 0.5:
+            width, hidden = -(-width // 64) * 64, -(-hidden // 64) * 64
+        out = width if rng.random() < 0.8 else _spread(rng, 3, 4096)
+        dtype = rng.choice(sorted(DTYPES))
+        most = 2 * 10 ** 11 // (hidden * (width + out))
+        return dict(op=op, run=rng.choice(("forward", "step")), rows=_spread(rng, 1, max(2, min(131072, most))),
+                    width=width, hidden=hidden, out=out, dtype=dtype,
+                    activation=rng.choice(("silu", "gelu", "relu")))
+    width = _spread(rng, 8, 2048)
+    most = max(1, min(64, 300_000_000 // (12 * width * width)))
+    return dict(op=op, tensors="blocks", layers=rng.randint(1, most), width=width,
+                dtype=rng.choice(sorted(DTYPES)), bits=rng.choice((32, 8)), clip=rng.random() < 0.5)
+
+
+# ----------------------------------------------------------------------------------------------- inputs --
+def _package():
+    path = os.path.join(os.getcwd(), "nerf-dbr_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from nerf_amd import operators, optim
+
+    return operators, optim
+
+
+def _sections(case):
+    return [int(v) for v in case["sections"].split(",")]
+
+
+def _frequencies(case):
+    """The pairs' frequencies, axis after axis (host doubles)."""
+    sections, got = _sections(case), []
+    for s in sections:
+        for j in range(s):
+            if case["ladder"] == "octaves":
+                got.append(2.0 ** j * math.pi)
+            elif case["ladder"] == "axis":
+                got.append(10000.0 ** (-j / s))
+            else:
+                got.append(10000.0 ** (-len(got) / sum(sections)))
+    return got
+
+
+def _shapes(case):
+    """[(shape, whether it decays)] of the tensors that an optimizer steps."""
+    got = []
+    if case["tensors"] == "networks":       # encodings of 63 and 27 values, a skip into layer 4, two heads
+        w = case["width"]
+        for _ in range(case["layers"]):
+            for o, i in [(w, 63)] + [(w, w)] * 3 + [(w, w + 63)] + [(w, w)] * 3 + [(1, w), (w // 2, w + 27), (3, w // 2)]:
+                got += [((o, i), True), ((o,), True)]
+        return got
+    w = case["width"]
+    for _ in range(case["layers"]):         # an attention's four products, a block, two norms, biases
+        got += [((3 * w, w), True), ((w, w), True), ((4 * w, w), True), ((w, 4 * w), True)]
+        got += [((w,), False), ((w,), False), ((3 * w,), False), ((w + 1,), False)]
+    return got
+
+
+def _flat(case):
+    """(offsets, total): where each tensor starts in a store whose tensors begin at whole blocks."""
+    offsets, total = [], 0
+    for shape, _ in _shapes(case):
+        offsets.append(total)
+        total += -(-math.prod(shape) // BLOCK) * BLOCK
+    return offsets, total
+
+
+def _views(case, store):
+    offsets, _ = _flat(case)
+    return [store[o:o + math.prod(s)].view(s) for o, (s, _) in zip(offsets, _shapes(case))]
+
+
+def _block_views(case, store):
+    offsets, _ = _flat(case)
+    return [store[o // BLOCK:o // BLOCK - (-math.prod(s) // BLOCK)] for o, (s, _) in zip(offsets, _shapes(case))]
+
+
+def _quantised(x):
+    """(e4m3 codes, scales) of a store: each block of 256 shares absmax / 448."""
+    x = x.view(-1, BLOCK)
+    scale = x.abs().amax(1) / 448.0
+    code = torch.where(scale[:, None] > 0, x / scale[:, None], torch.zeros_like(x)).to(E4M3)
+    return code.reshape(-1), scale
+
+
+def _root_quantised(x):
+    """The same for roots: one that is not zero keeps at least the smallest code, 2^-9."""
+    code, scale = _quantised(x)
+    least = (x > 0) & (code.float() == 0) & (scale[:, None] > 0).expand(-1, BLOCK).reshape(-1)
+    return torch.where(least, torch.full_like(x, 2.0 ** -9), code.float()).to(E4M3), scale
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(int(seed))
+
+    def normal(*shape, dtype=torch.float32, scale=1.0):
+        return (torch.randn(*shape, device="cuda", generator=gen, dtype=torch.float32) * scale).to(dtype)
+
+    s = {"case": case}
+    if case["op"] == "rotary":
+        dtype, b, n, d = DTYPES[case["dtype"]], case["batch"], case["tokens"], case["dim"]
+        axes = len(_sections(case))
+        s["x"] = []
+        for heads in (case["heads_q"], case["heads_k"]):
+            if heads and case["layout"] == "heads":
+                s["x"].append(normal(b, heads, n, d, dtype=dtype).transpose(1, 2))
+            elif heads:
+                s["x"].append(normal(b, n, heads, d, dtype=dtype))
+        if case["positions"] == "point":    # scene coordinates of samples between near and far
+            s["positions"] = torch.rand(b, n, axes, device="cuda", generator=gen) * 8.0 - 4.0
+        else:                               # (time, height, width): a first axis that counts far, then grids
+            far = torch.randint(0, 1_000_000, (b, 1, 1), device="cuda", generator=gen)
+            count = torch.arange(n, device="cuda").view(1, n, 1)
+            s["positions"] = torch.cat([far + count // 64 if a == 0 else (far % 7 + count // (8 ** a) % 64)
+                                        for a in range(axes)], 2)
+        # the ladder as the plain form reads it; a user of the framework names it or gives it as a list
+        s["axis"] = torch.tensor([a for a, k in enumerate(_sections(case)) for _ in range(k)], device="cuda")
+        s["frequency"] = torch.tensor(_frequencies(case), device="cuda", dtype=torch.float64)
+    elif case["op"] == "block":
+        dtype, n, d, f, o = DTYPES[case["dtype"]], case["rows"], case["width"], case["hidden"], case["out"]
+        s["x"] = normal(n, d, dtype=dtype)
+        s["gate"] = normal(f, d, dtype=dtype, scale=d ** -0.5)
+        s["up"] = normal(f, d, dtype=dtype, scale=d ** -0.5)
+        s["down"] = normal(o, f, dtype=dtype, scale=f ** -0.5)
+        if case["run"] == "step":
+            s["dy"] = normal(n, o, dtype=dtype)
+    else:
+        dtype = DTYPES[case["dtype"]]
+        _, total = _flat(case)
+        inside = torch.zeros(total, device="cuda")
+        decay = torch.zeros(total, device="cuda")
+        for v, w, (_, decays) in zip(_views(case, inside), _views(case, decay), _shapes(case)):
+            v.fill_(1.0)
+            if decays:
+                w.fill_(DECAY)
+        s["decay"] = decay
+        master = normal(total, scale=0.05).mul_(inside)
+        s["params"] = master.to(dtype)
+        s["master"] = master if dtype != torch.float32 else None
+        s["grads"] = normal(total, scale=1e-3).mul_(inside).to(dtype)
+        m, root = normal(total, scale=3e-4).mul_(inside), normal(total, scale=1e-3).abs_().mul_(inside)
+        s["steps"] = STEPS
+        if case["bits"] == 8:
+            s["m"], s["m_scale"] = _quantised(m)
+            s["v"], s["v_scale"] = _root_quantised(root)
+        else:
+            s["m"], s["v"] = m, root.square_()
+        if own:                             # the optimizer that a user's program keeps, on these very stores
+            _, optim = _package()
+            state = dict(steps=STEPS, exp_avg=_views(case, s["m"]), exp_avg_sq=_views(case, s["v"]))
+            if case["bits"] == 8:
+                state.update(exp_avg_scale=_block_views(case, s["m_scale"]),
+                             exp_avg_sq_scale=_block_views(case, s["v_scale"]))
+            if s["master"] is not None:
+                state["masters"] = _views(case, s["master"])
+            s["grad_list"] = _views(case, s["grads"])
+            s["optimizer"] = optim.AdamW(_views(case, s["params"]), lr=LR, betas=(BETA1, BETA2), eps=EPS,
+                                         weight_decay=[DECAY if w else 0.0 for _, w in _shapes(case)],
+                                         state_bits=case["bits"], max_norm=MAX_NORM if case["clip"] else None,
+                                         state=state)
+    return s
+
+
+# ----------------------------------------------------------------------------------------- plain forms --
+def _rotary_plain(s):
+    case = s["case"]
+    # angles in 64 bits: far positions times a frequency lose their fraction in 32
+    angle = s["positions"].double().index_select(-1, s["axis"]) * s["frequency"]
+    cos, sin = angle.cos().float().unsqueeze(2), angle.sin().float().unsqueeze(2)
+    sin = -sin if case["inverse"] else sin
+    r = cos.shape[-1]
+    outs = []
+    for x in s["x"]:
+        f = x.float()
+        u, v = (f[..., 0:2 * r:2], f[..., 1:2 * r:2]) if case["pairs"] == "interleaved" else (f[..., :r], f[..., r:2 * r])
+        p, q = u * cos - v * sin, u * sin + v * cos
+        turned = torch.stack((p, q), -1).flatten(-2) if case["pairs"] == "interleaved" else torch.cat((p, q), -1)
+        outs.append(torch.cat((turned, f[..., 2 * r:]), -1).to(x.dtype))
+    return outs
+
+
+def _activation_plain(g, kind):
+    """(act(g), act'(g))."""
+    if kind == "relu":
+        on = (g > 0).to(g.dtype)
+        return g * on, on
+    if kind == "silu":
+        e = 1.0 / (1.0 + torch.exp(-g))
+        return g * e, e * (1.0 + g * (1.0 - e))
+    c = 0.5 * (1.0 + torch.erf(g * math.sqrt(0.5)))
+    return g * c, c + g * torch.exp(-0.5 * g * g) * (1.0 / math.sqrt(2.0 * math.pi))
+
+
+def _block_plain(s):
+    case, dtype = s["case"], s["x"].dtype
+    x, gate, up, down = (s[k].float() for k in ("x", "gate", "up", "down"))
+    g, u = x @ gate.t(), x @ up.t()
+    a, da = _activation_plain(g, case["activation"])
+    h = a * u
+    outs = {"y": (h @ down.t()).to(dtype)}
+    if case["run"] == "step":
+        dy = s["dy"].float()
+        dh = dy @ down
+        dg, du = dh * u * da, dh * a
+        outs["dx"] = (dg @ gate + du @ up).to(dtype)
+        outs["dgate"], outs["dup"], outs["ddown"] = (dg.t() @ x).to(dtype), (du.t() @ x).to(dtype), (dy.t() @ h).to(dtype)
+    return outs
+
+
+def _adamw_plain(s):
+    case = s["case"]
+    s["steps"] += 1
+    g = s["grads"].float()
+    norm = s["grads"].double().square().sum().sqrt()        # a long sum: 64 bits
+    if case["clip"]:
+        g = g * (MAX_NORM / (norm + 1e-6)).clamp(max=1.0).float()
+    eight = case["bits"] == 8
+    if eight:
+        m = (s["m"].float().view(-1, BLOCK) * s["m_scale"][:, None]).view(-1)
+        v = (s["v"].float().view(-1, BLOCK) * s["v_scale"][:, None]).view(-1).square()
+    else:
+        m, v = s["m"], s["v"]
+    m = m + (g - m) * (1.0 - BETA1)
+    v = v * BETA2 + g * g * (1.0 - BETA2)
+    p = s["params"] if s["master"] is None else s["master"]
+    rate = LR / (1.0 - BETA1 ** s["steps"])
+    p = p * (1.0 - LR * s["decay"]) - rate * m / (v.sqrt() / math.sqrt(1.0 - BETA2 ** s["steps"]) + EPS)
+    if s["master"] is None:
+        s["params"].copy_(p)
+    else:
+        s["master"].copy_(p)
+        s["params"].copy_(p.to(s["params"].dtype))
+    if eight:
+        code, scale = _quantised(m)
+        s["m"].copy_(code), s["m_scale"].copy_(scale)
+        code, scale = _root_quantised(v.sqrt())
+        s["v"].copy_(code), s["v_scale"].copy_(scale)
+    else:
+        s["m"].copy_(m), s["v"].copy_(v)
+    return _adamw_outputs(s, norm.float() if case["clip"] else None)
+
+
+def _adamw_outputs(s, norm):
+    return {k: v for k, v in (("params", s["params"]), ("master", s["master"]), ("m", s["m"]), ("v", s["v"]),
+                              ("m_scale", s.get("m_scale")), ("v_scale", s.get("v_scale")), ("norm", norm))
+            if v is not None}
+
+
+def run(state):
+    case = state["case"]
+    if not own:
+        return {"rotary": _rotary_plain, "block": _block_plain, "adamw": _adamw_plain}[case["op"]](state)
+    operators, _ = _package()
+    if case["op"] == "rotary":
+        ladder = {"octaves": dict(frequencies=_frequencies(case))}.get(case["ladder"], dict(ladder=case["ladder"]))
+        return operators.rotary_axes(state["x"], state["positions"], _sections(case), pairs=case["pairs"],
+                                     inverse=case["inverse"], **ladder)
+    if case["op"] == "block":
+        weights = (state["gate"], state["up"], state["down"])
+        outs = {"y": operators.gated_block(state["x"], *weights, activation=case["activation"])}
+        if case["run"] == "step":
+            outs["dx"], outs["dgate"], outs["dup"], outs["ddown"] = operators.gated_block_backward(
+                state["dy"], state["x"], *weights, activation=case["activation"])
+        return outs
+    norm = state["optimizer"].step(state["grad_list"])
+    return _adamw_outputs(state, norm)
+
+
+# -------------------------------------------------------------------------------------- work and exact --
+def work(case):
+    if case["op"] == "rotary":
+        size = 4 if case["dtype"] == "float32" else 2
+        pairs, axes = sum(_sections(case)), len(_sections(case))
+        tokens = case["batch"] * case["tokens"]
+        values = tokens * (case["heads_q"] + case["heads_k"]) * case["dim"]
+        position = 4 if case["positions"] == "point" else 8
+        return {"bytes": 2 * values * size + tokens * axes * position,
+                "flops": 6 * tokens * (case["heads_q"] + case["heads_k"]) * pairs}
+    if case["op"] == "block":
+        size = 4 if case["dtype"] == "float32" else 2
+        n, d, f, o = case["rows"], case["width"], case["hidden"], case["out"]
+        one = 2 * n * f * (2 * d + o)
+        if case["run"] == "forward":
+            return {"bytes": size * (n * d + n * o + f * (2 * d + o)), "flops": one}
+        return {"bytes": size * (2 * n * d + 2 * n * o + 2 * f * (2 * d + o)), "flops": 3 * one}
+    n = sum(math.prod(s) for s, _ in _shapes(case))
+    size = 4 if case["dtype"] == "float32" else 2
+    per = size + 8 + (0 if size == 4 else size) + (16 if case["bits"] == 32 else 4 + 16 / BLOCK)
+    return {"bytes": n * per, "flops": 20 * n}
+
+
+def exact(case, seed):
+    """The definitions in 64 bits, on the inputs of prepare()."""
+    s = prepare(case, seed)
+    wide = torch.float64
+    if case["op"] == "rotary":
+        turn = torch.stack([s["positions"][..., a].to(wide) * f
+                            for a, f in zip([a for a, k in enumerate(_sections(case)) for _ in range(k)],
+                                            _frequencies(case))], -1)
+        turn = torch.polar(torch.ones_like(turn), -turn if case["inverse"] else turn)
+        r, outs = turn.shape[-1], []
+        for x in s["x"]:
+            y = x.to(wide)
+            for h in range(x.shape[2]):
+                row = y[:, :, h]
+                first, second = (slice(0, 2 * r, 2), slice(1, 2 * r, 2)) if case["pairs"] == "interleaved" else \
+                    (slice(0, r), slice(r, 2 * r))
+                z = torch.complex(row[..., first].contiguous(), row[..., second].contiguous()) * turn
+                row[..., first], row[..., second] = z.real, z.imag
+            outs.append(y)
+        return outs
+    if case["op"] == "block":
+        x, gate, up, down = (s[k].to(wide) for k in ("x", "gate", "up", "down"))
+        g, u = torch.mm(x, gate.T.contiguous()), torch.mm(x, up.T.contiguous())
+        if case["activation"] == "relu":
+            slope, a = torch.where(g > 0, 1.0, 0.0).to(wide), torch.clamp(g, min=0.0)
+        elif case["activation"] == "silu":
+            slope = torch.sigmoid(g)
+            a, slope = g * slope, slope + g * slope * (1.0 - slope)
+        else:
+            slope = 0.5 * torch.erfc(-g / math.sqrt(2.0))
+            a, slope = g * slope, slope + g * torch.exp(-g * g / 2.0) / math.sqrt(2.0 * math.pi)
+        outs = {"y": torch.mm(a * u, down.T.contiguous())}
+        if case["run"] == "step":
+            dy = s["dy"].to(wide)
+            outs["ddown"] = torch.mm(dy.T.contiguous(), a * u)
+            dh = torch.mm(dy, down)
+            du = dh * a
+            dg = dh.mul_(u).mul_(slope)
+            outs["dx"] = torch.mm(dg, gate).add_(torch.mm(du, up))
+            outs["dgate"], outs["dup"] = torch.mm(dg.T.contiguous(), x), torch.mm(du.T.contiguous(), x)
+        return outs
+    grads = [v.to(wide) for v in _views(case, s["grads"])]
+    norm = sum(float(torch.sum(g * g)) for g in grads) ** 0.5
+    factor = min(1.0, MAX_NORM / (norm + 1e-6)) if case["clip"] else 1.0
+    t, eight = STEPS + 1, case["bits"] == 8
+    source = s["params"] if s["master"] is None else s["master"]
+    outs = {k: torch.zeros(source.numel(), device="cuda", dtype=wide) for k in ("params", "m", "v")}
+    if eight:
+        outs["m_scale"], outs["v_scale"] = (torch.zeros(source.numel() // BLOCK, device="cuda", dtype=wide) for _ in "mv")
+    offsets, _ = _flat(case)
+    for o, g, (shape, decays) in zip(offsets, grads, _shapes(case)):
+        n = math.prod(shape)
+        # whole blocks: what lies behind a tensor's end is zero
+        span, blocks = slice(o, o - (-n // BLOCK) * BLOCK), slice(o // BLOCK, o // BLOCK - (-n // BLOCK))
+        g = torch.nn.functional.pad(g.reshape(-1) * factor, (0, span.stop - span.start - n))
+        m, v, p = s["m"][span].to(wide), s["v"][span].to(wide), source[span].to(wide)
+        if eight:
+            m = m * s["m_scale"][blocks].to(wide).repeat_interleave(BLOCK)
+            v = (v * s["v_scale"][blocks].to(wide).repeat_interleave(BLOCK)) ** 2
+        m, v = BETA1 * m + (1 - BETA1) * g, BETA2 * v + (1 - BETA2) * g * g
+        step = (m / (1 - BETA1 ** t)) / (torch.sqrt(v / (1 - BETA2 ** t)) + EPS)
+        outs["params"][span] = p - LR * ((DECAY if decays else 0.0) * p + step)
+        if eight:
+            for key, w in (("m", m), ("v", torch.sqrt(v))):
+                scale = w.view(-1, BLOCK).abs().max(1).values / 448
+                code = (w.view(-1, BLOCK) / scale.clamp(min=1e-300)[:, None]).float().to(E4M3).to(wide).reshape(-1)
+                outs[key][span] = torch.where((w > 0) & (code == 0), 2.0 ** -9, code) if key == "v" else code
+                outs[key + "_scale"][blocks] = scale
+        else:
+            outs["m"][span], outs["v"][span] = m, v
+    if s["master"] is not None:
+        outs["master"] = outs["params"]
+    if case["clip"]:
+        outs["norm"] = torch.tensor(norm, dtype=wide)
+    return outs
