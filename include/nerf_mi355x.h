@@ -374,6 +374,134 @@ int nerf_trainer_stage_ms(nerf_trainer* tr, float* ms_out /* [NERF_TRAIN_N_STAGE
  * unpadded shapes), for roofline reporting. */
 double nerf_trainer_gemm_flops(const nerf_trainer* tr);
 
+/* ---------------------------------------------------------------------------------------
+ * Block operators (no reference counterpart: the reference's networks are ReLU chains on sin /
+ * cos encodings, trained by Adam).  They run on the device that is current when they are called
+ * and queue their work on `stream`; nothing is kept between calls, so calls on different streams
+ * do not disturb each other as long as their outputs and workspaces differ, and every call can be
+ * captured into a graph.
+ * ------------------------------------------------------------------------------------- */
+enum nerf_dtype { NERF_F32 = 0, NERF_BFLOAT16 = 1, NERF_FLOAT16 = 2, NERF_INT32 = 3, NERF_INT64 = 4 };
+
+/* Rotary positions with several axes, beside nerf_positional_encoding: pair i of a head belongs to
+ * axis a(i) (sections[0] pairs to axis 0, the next sections[1] to axis 1, ...) and is turned by
+ * theta = position[a(i)] * f_i:  (u, v) -> (u cos - v sin, u sin + v cos); values behind the last
+ * pair pass through.  inverse turns by -theta, which is also the gradient of the forward turn.
+ *   frequencies  host [sum of sections] doubles f_i, or NULL: base^(-j / sections[a]) for pair j
+ *                of axis a, or with shared_ladder base^(-i / sum of sections);
+ *   interleaved  0: pair i is (x[i], x[i + pairs]); 1: pair i is (x[2i], x[2i + 1]);
+ *   positions    device, [n_batch][n_tokens][n_axes] by element strides (0 repeats); NERF_F32,
+ *                NERF_INT32 or NERF_INT64; the angle and its reduction are fp64;
+ *   x, out       device [n_batch][n_tokens][heads][head_dim] by element strides, head_dim
+ *                contiguous; one or two tensors (queries and keys) turn by the same angles;
+ *                out may be x. */
+#define NERF_ROTARY_MAX_AXES 4
+#define NERF_ROTARY_MAX_PAIRS 256
+typedef struct nerf_rotary_tensor {
+  const void* x;
+  void* out;
+  int heads;
+  int64_t x_stride[3], out_stride[3]; /* batch, token, head; elements */
+} nerf_rotary_tensor;
+typedef struct nerf_rotary_desc {
+  int dtype;                             /* NERF_F32, NERF_BFLOAT16 or NERF_FLOAT16 */
+  int head_dim;
+  int n_axes;
+  int sections[NERF_ROTARY_MAX_AXES];
+  int shared_ladder, interleaved, inverse;
+  double base;
+  const double* frequencies;
+  const void* positions;
+  int position_dtype;
+  int64_t position_stride[3];            /* batch, token, axis; elements */
+  int n_batch;
+  int64_t n_tokens;
+  int n_tensors;
+  nerf_rotary_tensor tensor[2];
+} nerf_rotary_desc;
+int nerf_rotary_axes(const nerf_rotary_desc* desc, void* stream);
+
+/* The gated feed-forward block, beside nerf_query and the training step:
+ *   g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T
+ * for x [rows][width], Wg and Wu [hidden][width], Wd [out][hidden], y [rows][out], row-major with
+ * row strides ld_* in elements, all of one dtype; sums in fp32 or wider, h rounded once to dtype
+ * for 16-bit types.  The backward call recomputes g and u from x (nothing is stored by the forward)
+ * and writes dx [rows][width] (row stride ld_dx) and the weights' gradients, contiguous; any of the
+ * four may be NULL.  Neither output may overlap an input.
+ * workspace: device memory of at least nerf_gated_block_workspace(desc, backward) bytes, 256-byte
+ * aligned, the call's own until its work is done (0 bytes: may be NULL). */
+enum nerf_activation { NERF_SILU = 0, NERF_GELU = 1 /* x Phi(x) */, NERF_RELU = 2 };
+typedef struct nerf_block_desc {
+  int dtype;
+  int activation;
+  int64_t rows;
+  int width, hidden, out;
+  const void *x, *w_gate, *w_up, *w_down;
+  int64_t ld_x, ld_gate, ld_up, ld_down;
+} nerf_block_desc;
+size_t nerf_gated_block_workspace(const nerf_block_desc* desc, int backward);
+int nerf_gated_block_forward(const nerf_block_desc* desc, void* y, int64_t ld_y, void* workspace,
+                             size_t workspace_bytes, void* stream);
+int nerf_gated_block_backward(const nerf_block_desc* desc, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx,
+                              void* dw_gate, void* dw_up, void* dw_down, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* One AdamW step over many tensors at once (decoupled weight decay), beside nerf_trainer_update:
+ *   g = grad * min(1, max_norm / (|grads| + 1e-6))                   (max_norm > 0)
+ *   m = m + (1 - beta1)(g - m), v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * param is the fp32 weight; with model != NULL it is the master of a 16-bit weight, which is
+ * written as the rounded new value.  grad is NERF_F32, NERF_BFLOAT16 or NERF_FLOAT16.
+ * state_bits 32: exp_avg and exp_avg_sq are fp32 [numel].  state_bits 8: they are e4m3 codes
+ * [numel] of m and of sqrt(v), each block of NERF_ADAMW_BLOCK values (counted from the tensor's
+ * start, the last one short) times its fp32 scale = absmax / 448 in *_scale; a sqrt(v) > 0 keeps at
+ * least the smallest code.  The step itself uses the unrounded new m and v.
+ * control (device, zeroed once by the caller, one per optimizer): the step count t, which the call
+ * advances on the device so that a captured call counts its replays; the gradient norm (max_norm
+ * > 0 or NERF_ADAMW_SKIP_NONFINITE) and the steps skipped.  flags: NERF_ADAMW_SKIP_NONFINITE leaves
+ * everything as it is when the norm is not finite (counted in control); NERF_ADAMW_WRITE_GRADS
+ * stores the clipped gradients.  lr_device (device fp32, or NULL) replaces lr.
+ * workspace: nerf_adamw_workspace(n_tensors, tensors, ...) bytes of device memory, 8-byte aligned. */
+#define NERF_ADAMW_BLOCK 256
+#define NERF_ADAMW_SKIP_NONFINITE 1
+#define NERF_ADAMW_WRITE_GRADS 2
+typedef struct nerf_adamw_control {
+  int32_t steps;
+  uint32_t ticket; /* internal, zero between calls */
+  int32_t skipped;
+  float norm;
+  float factor;    /* what the gradients were multiplied by */
+  int32_t reserved[3];
+} nerf_adamw_control;
+typedef struct nerf_adamw_tensor {
+  float* param;
+  void* model;       /* 16-bit weight, or NULL */
+  void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;    /* state_bits 8 */
+  float* exp_avg_sq_scale;
+  int64_t numel;
+  double weight_decay;
+  int32_t model_dtype, grad_dtype;
+} nerf_adamw_tensor;
+typedef struct nerf_adamw_config {
+  double lr, beta1, beta2, eps, max_norm;
+  const float* lr_device;
+  int32_t state_bits;
+  int32_t flags;
+} nerf_adamw_config;
+size_t nerf_adamw_workspace(int n_tensors, const nerf_adamw_tensor* tensors);
+int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_adamw_tensor* tensors,
+                    nerf_adamw_control* control, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The trainer's optimizer: NERF_OPT_ADAM (the reference's, default) or NERF_OPT_ADAMW on the
+ * trainer's settings (decoupled weight decay on every tensor), with its moments in 32 or 8 bits.
+ * Moments keep their values over the change (rounded when they become 8-bit); nerf_trainer_read and
+ * nerf_trainer_write see them as fp32 either way. */
+enum nerf_optimizer { NERF_OPT_ADAM = 0, NERF_OPT_ADAMW = 1 };
+int nerf_trainer_set_optimizer(nerf_trainer* tr, int optimizer, int state_bits);
+
 #ifdef __cplusplus
 }
 #endif

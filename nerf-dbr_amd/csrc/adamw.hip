@@ -1,0 +1,375 @@
+// One AdamW step over many tensors at once (nerf_adamw_step).
+//   g = grad * min(1, max_norm / (|grads| + 1e-6))
+//   m = m + (1 - b1)(g - m),  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// Bound by bytes: 28 per fp32 value with 32-bit moments, 16 + 16 / 256 with 8-bit ones.  The tensors'
+// addresses travel in the kernel arguments (48 tensors a launch), so nothing is uploaded, nothing is
+// kept between calls and a captured call replays as it was made.
+#include <cmath>
+#include <cstring>
+
+#include "nerf_internal.h"
+
+namespace nerf {
+namespace {
+
+constexpr int kTensors = 48;   // per launch: 48 x 72 bytes of the 4 KiB of kernel arguments
+struct AdamTensor {
+  float* p;
+  void* model;
+  void* g;
+  void* m;
+  void* v;
+  float* ms;
+  float* vs;
+  long n;
+  float decay;      // 1 - lr * weight_decay with the host's lr; with lr_device the kernel forms it
+  float wd;
+};
+struct AdamArgs {
+  AdamTensor t[kTensors];
+  unsigned first[kTensors];   // the tensor's first chunk in this launch
+  int n_tensors, iters, flags, last;
+  unsigned char wide[kTensors];   // every address allows vector access
+  nerf_adamw_control* ctl;
+  const float* lr_dev;
+  float lr, b1, b2, eps;
+  double b1d, b2d;
+  int clip;
+};
+static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+constexpr int kStep = 1024;    // values a workgroup takes per iteration: 256 threads x 4
+
+// The tensor that a chunk belongs to: the last one whose first chunk is not behind it.
+__device__ __forceinline__ int find(const AdamArgs& a, unsigned chunk) {
+  int lo = 0, hi = a.n_tensors - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.first[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T>
+struct alignas(sizeof(T) * 4) Quad {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, long i, long n, bool wide, float out[4]) {
+  if (wide && i + 4 <= n) {
+    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(p + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = float(q.v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = i + k < n ? float(p[i + k]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, long i, long n, bool wide, const float in[4]) {
+  if (wide && i + 4 <= n) {
+    Quad<T> q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q.v[k] = T(in[k]);
+    *reinterpret_cast<Quad<T>*>(p + i) = q;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = T(in[k]);
+  }
+}
+// four e4m3 codes (OCP, the hardware's conversion) as one word
+__device__ __forceinline__ void load_codes(const unsigned char* p, long i, long n, bool wide, float out[4]) {
+  unsigned w = 0;
+  if (wide && i + 4 <= n) w = *reinterpret_cast<const unsigned*>(p + i);
+  else
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) w |= unsigned(p[i + k]) << (8 * k);
+  out[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+  out[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+  out[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+  out[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+}
+__device__ __forceinline__ void store_codes(unsigned char* p, long i, long n, bool wide, unsigned w) {
+  if (wide && i + 4 <= n) *reinterpret_cast<unsigned*>(p + i) = w;
+  else
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = (unsigned char)(w >> (8 * k));
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ double pow_steps(double b, int t) {   // b^t, t > 0, by squaring
+  double r = 1.0;
+  for (; t; t >>= 1, b *= b)
+    if (t & 1) r *= b;
+  return r;
+}
+
+// True in the one workgroup of the launch that comes last; everything the others wrote before is
+// visible to it.  The ticket is zero again afterwards.
+__device__ __forceinline__ bool last_group(nerf_adamw_control* ctl) {
+  __shared__ bool is_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned t = __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = t == gridDim.x - 1;
+    if (is_last) __hip_atomic_store(&ctl->ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return is_last;
+}
+
+// The gradients' squares summed in fp64, one partial per workgroup at a fixed place; the last
+// workgroup of the last launch adds the partials in order, so the norm does not depend on timing.
+template <typename G>
+__global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part, long done, float max_norm) {
+  __shared__ double red[4];
+  const int k = find(a, blockIdx.x);
+  const AdamTensor& t = a.t[k];
+  long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
+  double s = 0.0;
+  for (int it = 0; it < a.iters && i < t.n; ++it, i += kStep) {
+    float g[4];
+    load4(static_cast<const G*>(t.g), i, t.n, a.wide[k], g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += double(g[j]) * double(g[j]);
+  }
+  auto sum = [&](double x) {   // of the workgroup, in thread 0
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_down(x, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+  };
+  s = sum(s);
+  if (threadIdx.x == 0) __hip_atomic_store(part + done + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_group(a.ctl) || !a.last) return;
+  __threadfence();
+  double all = 0.0;
+#pragma unroll 8
+  for (long j = threadIdx.x; j < done + gridDim.x; j += 256) all += part[j];
+  all = sum(all);
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(all), f = max_norm > 0.0f ? double(max_norm) / (norm + 1e-6) : 1.0;
+    a.ctl->norm = float(norm);
+    a.ctl->factor = f > 1.0 ? 1.0f : float(f);   // NaN stays NaN
+  }
+}
+
+template <typename G, typename M, int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamArgs a) {
+  const int k = find(a, blockIdx.x);
+  const AdamTensor& t = a.t[k];
+  const bool wide = a.wide[k];
+  const int step = a.ctl->steps + 1;
+  const float factor = a.clip ? a.ctl->factor : 1.0f;
+  const bool skip = (a.flags & NERF_ADAMW_SKIP_NONFINITE) && !__builtin_isfinite(a.ctl->norm);
+  if (!skip) {
+    const float lr = a.lr_dev ? *a.lr_dev : a.lr;
+    const float decay = a.lr_dev ? 1.0f - lr * t.wd : t.decay;
+    const float rate = float(double(lr) / (1.0 - pow_steps(a.b1d, step)));
+    const float root = float(sqrt(1.0 - pow_steps(a.b2d, step)));
+    const float b1c = float(1.0 - a.b1d), b2c = float(1.0 - a.b2d);
+    long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
+    for (int it = 0; it < a.iters; ++it, i += kStep) {
+      if (BITS == 32 && i >= t.n) break;
+      if (BITS == 8 && i - (threadIdx.x & 63) * 4 >= t.n) break;   // uniform in a wave: its block is behind the end
+      float g[4], p[4], m[4], v[4], r[4];
+      load4(static_cast<const G*>(t.g), i, t.n, wide, g);
+      load4(t.p, i, t.n, wide, p);
+      const long block = i >> 8;    // the wave's 256 values are one block
+      if (BITS == 32) {
+        load4(static_cast<const float*>(t.m), i, t.n, wide, m);
+        load4(static_cast<const float*>(t.v), i, t.n, wide, v);
+      } else {
+        load_codes(static_cast<const unsigned char*>(t.m), i, t.n, wide, m);
+        load_codes(static_cast<const unsigned char*>(t.v), i, t.n, wide, v);
+        const float ms = t.ms[block], vs = t.vs[block];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[j] *= ms;
+          v[j] *= vs;
+          v[j] *= v[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[j] *= factor;
+        m[j] += (g[j] - m[j]) * b1c;
+        v[j] = v[j] * a.b2 + g[j] * g[j] * b2c;
+        r[j] = sqrtf(v[j]);
+        p[j] = p[j] * decay - rate * m[j] / (r[j] / root + a.eps);
+      }
+      if (a.flags & NERF_ADAMW_WRITE_GRADS) store4(static_cast<G*>(t.g), i, t.n, wide, g);
+      store4(t.p, i, t.n, wide, p);
+      if (sizeof(M) == 2) store4(static_cast<M*>(t.model), i, t.n, wide, p);
+      if (BITS == 32) {
+        store4(static_cast<float*>(t.m), i, t.n, wide, m);
+        store4(static_cast<float*>(t.v), i, t.n, wide, v);
+      } else {
+        // values behind the tensor's end were loaded as zeros: they do not raise the block's maximum
+        const float top = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+        const float rtop = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+        const float ms = top / 448.0f, vs = rtop / 448.0f;
+        unsigned mw = 0, vw = 0;
+        if (ms > 0.0f) {
+          mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] / ms, m[1] / ms, mw, false);
+          mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] / ms, m[3] / ms, mw, true);
+        }
+        if (vs > 0.0f) {
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[0] / vs, r[1] / vs, vw, false);
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[2] / vs, r[3] / vs, vw, true);
+          // a root that is not zero keeps the smallest code: m / (0 + eps) of a value whose v was
+          // rounded away would be a step of any size
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (r[j] > 0.0f && ((vw >> (8 * j)) & 0xffu) == 0) vw |= 1u << (8 * j);
+        }
+        store_codes(static_cast<unsigned char*>(t.m), i, t.n, wide, mw);
+        store_codes(static_cast<unsigned char*>(t.v), i, t.n, wide, vw);
+        if ((threadIdx.x & 63) == 0) t.ms[block] = ms, t.vs[block] = vs;
+      }
+    }
+  }
+  if (!last_group(a.ctl) || !a.last || threadIdx.x) return;   // every workgroup has read steps
+  if (skip) a.ctl->skipped += 1;
+  else a.ctl->steps = step;
+}
+
+// Chunks of a call: as many as fill the machine with one iteration each, at most 8 iterations (32 KiB
+// of fp32 per array) so that a workgroup's fixed cost (tensor search, bias corrections) is spread.
+int iterations(int n, const nerf_adamw_tensor* t) {
+  long steps = 0;
+  for (int i = 0; i < n; ++i) steps += (t[i].numel + kStep - 1) / kStep;
+  const long per = steps / (8L * 256);
+  return int(per < 1 ? 1 : per > 8 ? 8 : per);
+}
+long chunks(const nerf_adamw_tensor& t, int iters) { return (t.numel + long(iters) * kStep - 1) / (long(iters) * kStep); }
+
+template <typename G, typename M>
+void launch_step(const AdamArgs& a, int bits, unsigned grid, hipStream_t s) {
+  if (bits == 32) hipLaunchKernelGGL((adamw_kernel<G, M, 32>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((adamw_kernel<G, M, 8>), dim3(grid), dim3(256), 0, s, a);
+}
+template <typename G>
+void launch_step(const AdamArgs& a, int model, int bits, unsigned grid, hipStream_t s) {
+  if (model == NERF_BFLOAT16) launch_step<G, __bf16>(a, bits, grid, s);
+  else if (model == NERF_FLOAT16) launch_step<G, _Float16>(a, bits, grid, s);
+  else launch_step<G, float>(a, bits, grid, s);
+}
+
+int check(const nerf_adamw_config* c, int n, const nerf_adamw_tensor* t) {
+  if (!c || (n > 0 && !t) || n < 0) return set_error(NERF_E_INVALID, "nerf_adamw_step: null argument");
+  if (!(c->lr >= 0.0) || !(c->beta1 >= 0.0 && c->beta1 < 1.0) || !(c->beta2 >= 0.0 && c->beta2 < 1.0) || !(c->eps >= 0.0))
+    return set_error(NERF_E_INVALID, "nerf_adamw_step: lr %g, betas %g %g, eps %g", c->lr, c->beta1, c->beta2, c->eps);
+  if (c->state_bits != 32 && c->state_bits != 8) return set_error(NERF_E_INVALID, "nerf_adamw_step: state_bits %d (32 or 8)", c->state_bits);
+  if (c->flags & ~(NERF_ADAMW_SKIP_NONFINITE | NERF_ADAMW_WRITE_GRADS)) return set_error(NERF_E_INVALID, "nerf_adamw_step: flags %d", c->flags);
+  bool any = false;
+  for (int i = 0; i < n; ++i) {
+    const nerf_adamw_tensor& x = t[i];
+    any = any || x.numel > 0;
+    if (x.numel < 0 || x.numel > (1L << 40)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has %ld values", i, long(x.numel));
+    if (x.numel == 0) continue;
+    if (!x.param || !x.grad || !x.exp_avg || !x.exp_avg_sq || (c->state_bits == 8 && (!x.exp_avg_scale || !x.exp_avg_sq_scale)))
+      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has a null store", i);
+    if (x.grad_dtype != NERF_F32 && x.grad_dtype != NERF_BFLOAT16 && x.grad_dtype != NERF_FLOAT16)
+      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has gradient dtype %d", i, x.grad_dtype);
+    if (x.model && x.model_dtype != NERF_BFLOAT16 && x.model_dtype != NERF_FLOAT16)
+      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has model dtype %d", i, x.model_dtype);
+    if (!(x.weight_decay >= 0.0)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has weight decay %g", i, x.weight_decay);
+    uintptr_t four = uintptr_t(x.param) | uintptr_t(x.exp_avg_scale) | uintptr_t(x.exp_avg_sq_scale);
+    uintptr_t two = uintptr_t(x.model);
+    (x.grad_dtype == NERF_F32 ? four : two) |= uintptr_t(x.grad);
+    if (c->state_bits == 32) four |= uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq);
+    if ((four & 3) || (two & 1)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d is not aligned to its type", i);
+  }
+  if (!any) return set_error(NERF_E_INVALID, "nerf_adamw_step: no values to step");
+  return NERF_OK;
+}
+
+}  // namespace
+}  // namespace nerf
+
+using namespace nerf;
+
+extern "C" {
+
+size_t nerf_adamw_workspace(int n_tensors, const nerf_adamw_tensor* tensors) {
+  if (n_tensors <= 0 || !tensors) return 0;
+  const int iters = iterations(n_tensors, tensors);
+  long n = 0;
+  for (int i = 0; i < n_tensors; ++i) n += chunks(tensors[i], iters);
+  return sizeof(double) * size_t(n);
+}
+
+int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_adamw_tensor* tensors,
+                    nerf_adamw_control* control, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(config, n_tensors, tensors);
+  if (rc != NERF_OK) return rc;
+  if (!control) return set_error(NERF_E_INVALID, "nerf_adamw_step: null control");
+  const bool clip = config->max_norm > 0.0, norm = clip || (config->flags & NERF_ADAMW_SKIP_NONFINITE);
+  if (norm && (workspace_bytes < nerf_adamw_workspace(n_tensors, tensors) ||
+               (workspace_bytes && (!workspace || (uintptr_t(workspace) & 7)))))
+    return set_error(NERF_E_INVALID, "nerf_adamw_step: workspace of %zu bytes, %zu needed (8-byte aligned)", workspace_bytes,
+                     nerf_adamw_workspace(n_tensors, tensors));
+  const hipStream_t s = (hipStream_t)stream;
+  const int iters = iterations(n_tensors, tensors);
+  // launches of up to kTensors tensors of the same types, in order; pass 0 sums squares, pass 1 steps
+  for (int pass = norm ? 0 : 1; pass < 2; ++pass) {
+    AdamArgs a;
+    std::memset(&a, 0, sizeof a);
+    long done = 0;
+    int grad = -1, model = -1;
+    unsigned grid = 0;
+    auto flush = [&](int last) -> int {
+      if (a.n_tensors == 0) return NERF_OK;
+      a.last = last;
+      if (pass == 0) {
+        const float mx = float(config->max_norm);
+        double* part = static_cast<double*>(workspace);
+        if (grad == NERF_F32) hipLaunchKernelGGL((norm_kernel<float>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
+        else if (grad == NERF_BFLOAT16) hipLaunchKernelGGL((norm_kernel<__bf16>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
+        else hipLaunchKernelGGL((norm_kernel<_Float16>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
+      } else {
+        if (grad == NERF_F32) launch_step<float>(a, model, config->state_bits, grid, s);
+        else if (grad == NERF_BFLOAT16) launch_step<__bf16>(a, model, config->state_bits, grid, s);
+        else launch_step<_Float16>(a, model, config->state_bits, grid, s);
+      }
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return set_error(NERF_E_HIP, "nerf_adamw_step: %s", hipGetErrorString(e));
+      done += grid;
+      a.n_tensors = 0, grid = 0;
+      return NERF_OK;
+    };
+    a.iters = iters, a.flags = config->flags, a.ctl = control, a.lr_dev = config->lr_device, a.clip = clip;
+    a.lr = float(config->lr), a.b1 = float(config->beta1), a.b2 = float(config->beta2), a.eps = float(config->eps);
+    a.b1d = config->beta1, a.b2d = config->beta2;
+    for (int i = 0; i < n_tensors; ++i) {
+      const nerf_adamw_tensor& x = tensors[i];
+      if (x.numel == 0) continue;
+      const int md = x.model ? x.model_dtype : NERF_F32;
+      const long c = chunks(x, iters);
+      if (c > 0x40000000L) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d is too large", i);
+      if (a.n_tensors == kTensors || x.grad_dtype != grad || md != model || grid + c > 0x7fffffffL)
+        if ((rc = flush(0)) != NERF_OK) return rc;
+      grad = x.grad_dtype, model = md;
+      const int k = a.n_tensors++;
+      a.t[k] = AdamTensor{x.param, x.model, x.grad, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, long(x.numel),
+                          float(1.0 - config->lr * x.weight_decay), float(x.weight_decay)};
+      a.first[k] = grid;
+      const uintptr_t gsize = x.grad_dtype == NERF_F32 ? 15 : 7;
+      a.wide[k] = !(uintptr_t(x.param) & 15) && !(uintptr_t(x.grad) & gsize) && !(uintptr_t(x.model) & 7) &&
+                  !((uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq)) & (config->state_bits == 32 ? 15 : 3));
+      grid += unsigned(c);
+    }
+    if ((rc = flush(1)) != NERF_OK) return rc;
+  }
+  return NERF_OK;
+}
+
+}  // extern "C"

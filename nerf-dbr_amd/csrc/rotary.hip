@@ -1,0 +1,225 @@
+// Rotary positions with several axes (nerf_rotary_axes): every pair (u, v) of a head is turned by
+// theta = position[axis of the pair] * frequency of the pair,
+//   (u, v) -> (u cos - v sin, u sin + v cos),
+// the same angles for every head of a token.  The cost is the bytes of x and out; the angles are
+// computed once per (token, pair) by the thread that then runs over the heads, so they need no table
+// in memory and no second launch.
+#include <cmath>
+
+#include "nerf_internal.h"
+
+namespace nerf {
+namespace {
+
+struct RotaryTensor {
+  const void* x;
+  void* out;
+  long xs[3], os[3];   // batch, token, head
+  int heads;
+  int copy_tail;       // out is not x: the values behind the last pair are copied
+};
+struct RotaryArgs {
+  RotaryTensor t[2];
+  const void* pos;
+  long ps[3];
+  long n_tokens, items;            // items: (batch, token, group of V values of a head)
+  int n_tensors, dim, pairs, groups, rot_groups, pos_dtype, interleaved;
+  float sign;                      // -1 turns back
+  unsigned char axis[NERF_ROTARY_MAX_PAIRS];
+  double freq[NERF_ROTARY_MAX_PAIRS];
+};
+static_assert(sizeof(RotaryArgs) <= 4096, "kernel arguments");
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+__device__ __forceinline__ double position(const RotaryArgs& a, long at) {
+  if (a.pos_dtype == NERF_F32) return double(static_cast<const float*>(a.pos)[at]);
+  if (a.pos_dtype == NERF_INT32) return double(static_cast<const int*>(a.pos)[at]);
+  return double(static_cast<const long*>(a.pos)[at]);
+}
+
+// cos and sin of an fp64 angle to fp32 accuracy for |angle| < 2^52: the multiple of pi/2 comes off in
+// fp64 (two-part pi/2, each step one fma: the remainder is good to ~1e-16 + |angle| 2^-106), then the
+// Taylor polynomials on [-pi/4, pi/4] in fp32 (next terms x^11/11! = 1.8e-9 and x^12/12! = 1.2e-10).
+// An fp32 angle would lose the fraction of a far position: position 10^6 has 2^-4 between neighbours.
+__device__ __forceinline__ void turn(double angle, float& c, float& s) {
+  const double q = rint(angle * 0.63661977236758134308);
+  double r = fma(-q, 1.57079632679489655800, angle);
+  r = fma(-q, 6.12323399573676603587e-17, r);
+  const float x = float(r), z = __fmul_rn(x, x);
+  const float ps = fmaf(fmaf(fmaf(2.7557319e-6f, z, -1.9841270e-4f), z, 8.3333333e-3f), z, -1.6666667e-1f);
+  const float sn = fmaf(__fmul_rn(x, z), ps, x);
+  const float pc = fmaf(fmaf(fmaf(fmaf(-2.7557319e-7f, z, 2.4801587e-5f), z, -1.3888889e-3f), z, 4.1666667e-2f), z, -0.5f);
+  const float cs = fmaf(z, pc, 1.0f);
+  const int k = int(q - 4.0 * floor(q * 0.25));   // q mod 4
+  const float a = (k & 1) ? cs : sn, b = (k & 1) ? sn : cs;
+  s = (k & 2) ? -a : a;
+  c = ((k + 1) & 2) ? -b : b;
+}
+
+// A thread owns V pairs of one token in split form (two vectors of V values per head) and V / 2 pairs
+// in interleaved form (one vector), or V values behind the last pair, and runs over the heads
+// [blockIdx.y * per, + per) of both tensors.
+template <typename T, int V, bool INTER>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int per) {
+  const long item = long(blockIdx.x) * 256 + threadIdx.x;
+  if (item >= a.items) return;
+  const long row = item / a.groups;
+  const int g = int(item - row * a.groups);
+  const long b = row / a.n_tokens, n = row - b * a.n_tokens;
+  const bool tail = g >= a.rot_groups;
+  constexpr int P = INTER ? (V > 1 ? V / 2 : 1) : V;   // pairs a thread turns
+  float c[P], s[P];
+  if (!tail) {
+    const long at = b * a.ps[0] + n * a.ps[1];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int p = g * P + i;
+      c[i] = 1.0f, s[i] = 0.0f;
+      if (p < a.pairs) {
+        turn(position(a, at + a.axis[p] * a.ps[2]) * a.freq[p], c[i], s[i]);
+        s[i] *= a.sign;
+      }
+    }
+  }
+  int h = blockIdx.y * per;
+  const int last = h + per;
+  for (int k = 0, first = 0; k < a.n_tensors; first += a.t[k].heads, ++k) {
+    const RotaryTensor& t = a.t[k];
+    const T* x = static_cast<const T*>(t.x) + b * t.xs[0] + n * t.xs[1];
+    T* o = static_cast<T*>(t.out) + b * t.os[0] + n * t.os[1];
+    const int end = min(last, first + t.heads);
+    for (; h < end; ++h) {
+      const T* xh = x + (h - first) * t.xs[2];
+      T* oh = o + (h - first) * t.os[2];
+      if (tail) {
+        if (!t.copy_tail) continue;
+        const int e = 2 * a.pairs + (g - a.rot_groups) * V;
+        *reinterpret_cast<Vec<T, V>*>(oh + e) = *reinterpret_cast<const Vec<T, V>*>(xh + e);
+      } else if (INTER && V > 1) {
+        const int e = g * V;
+        Vec<T, V> w = *reinterpret_cast<const Vec<T, V>*>(xh + e);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          const float u = float(w.v[2 * i]), v = float(w.v[2 * i + 1]);
+          w.v[2 * i] = T(u * c[i] - v * s[i]);
+          w.v[2 * i + 1] = T(u * s[i] + v * c[i]);
+        }
+        *reinterpret_cast<Vec<T, V>*>(oh + e) = w;
+      } else {
+        const int e = INTER ? 2 * g : g * V, f = INTER ? 2 * g + 1 : a.pairs + g * V;
+        Vec<T, V> p = *reinterpret_cast<const Vec<T, V>*>(xh + e), q = *reinterpret_cast<const Vec<T, V>*>(xh + f);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float u = float(p.v[i]), v = float(q.v[i]);
+          p.v[i] = T(u * c[i] - v * s[i]);
+          q.v[i] = T(u * s[i] + v * c[i]);
+        }
+        *reinterpret_cast<Vec<T, V>*>(oh + e) = p;
+        *reinterpret_cast<Vec<T, V>*>(oh + f) = q;
+      }
+    }
+  }
+}
+
+template <typename T, int V>
+hipError_t launch(const RotaryArgs& a, int heads, hipStream_t s) {
+  // heads per thread: all of them where the (token, group) threads alone fill the machine, so that the
+  // angles are computed once; else spread over blockIdx.y
+  const long blocks = (a.items + 255) / 256;
+  const long want = 4L * current_device_cus();
+  const int spread = int(blocks >= want ? 1 : (want + blocks - 1) / blocks < heads ? (want + blocks - 1) / blocks : heads);
+  const int per = (heads + spread - 1) / spread;
+  const dim3 grid{unsigned(blocks), unsigned((heads + per - 1) / per)};
+  if (a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, V, true>), grid, dim3(256), 0, s, a, per);
+  else hipLaunchKernelGGL((rotary_kernel<T, V, false>), grid, dim3(256), 0, s, a, per);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_v(const RotaryArgs& a, int v, int heads, hipStream_t s) {
+  constexpr int kMost = 16 / sizeof(T);
+  if (v == kMost) return launch<T, kMost>(a, heads, s);
+  if (v == 2) return launch<T, 2>(a, heads, s);
+  return launch<T, 1>(a, heads, s);
+}
+
+}  // namespace
+}  // namespace nerf
+
+using namespace nerf;
+
+extern "C" int nerf_rotary_axes(const nerf_rotary_desc* d, void* stream) {
+  if (!d) return set_error(NERF_E_INVALID, "nerf_rotary_axes: null descriptor");
+  if (d->dtype != NERF_F32 && d->dtype != NERF_BFLOAT16 && d->dtype != NERF_FLOAT16)
+    return set_error(NERF_E_INVALID, "nerf_rotary_axes: dtype %d", d->dtype);
+  if (d->position_dtype != NERF_F32 && d->position_dtype != NERF_INT32 && d->position_dtype != NERF_INT64)
+    return set_error(NERF_E_INVALID, "nerf_rotary_axes: position dtype %d", d->position_dtype);
+  if (d->n_axes < 1 || d->n_axes > NERF_ROTARY_MAX_AXES)
+    return set_error(NERF_E_INVALID, "nerf_rotary_axes: %d axes (1..%d)", d->n_axes, NERF_ROTARY_MAX_AXES);
+  if (d->n_tensors < 1 || d->n_tensors > 2) return set_error(NERF_E_INVALID, "nerf_rotary_axes: %d tensors (1 or 2)", d->n_tensors);
+  if (d->n_batch < 0 || d->n_tokens < 0 || d->head_dim < 1)
+    return set_error(NERF_E_INVALID, "nerf_rotary_axes: batch %d, tokens %ld, head_dim %d", d->n_batch, long(d->n_tokens), d->head_dim);
+  RotaryArgs a{};
+  for (int k = 0; k < d->n_axes; ++k) {
+    const int n = d->sections[k];
+    if (n < 0 || a.pairs + n > NERF_ROTARY_MAX_PAIRS || 2 * (a.pairs + n) > d->head_dim)
+      return set_error(NERF_E_INVALID, "nerf_rotary_axes: sections need 2 * (pairs) <= head_dim %d and <= %d pairs", d->head_dim,
+                       NERF_ROTARY_MAX_PAIRS);
+    for (int j = 0; j < n; ++j) a.axis[a.pairs++] = (unsigned char)k;
+  }
+  if (!d->frequencies && !(d->base > 0.0 && std::isfinite(d->base)))
+    return set_error(NERF_E_INVALID, "nerf_rotary_axes: base must be positive");
+  for (int i = 0, k = 0, j = 0; i < a.pairs; ++i, ++j) {
+    while (a.axis[i] != k) ++k, j = 0;
+    a.freq[i] = d->frequencies ? d->frequencies[i]
+                               : std::pow(d->base, d->shared_ladder ? -double(i) / a.pairs : -double(j) / d->sections[k]);
+    if (!std::isfinite(a.freq[i])) return set_error(NERF_E_INVALID, "nerf_rotary_axes: frequency %d is not finite", i);
+  }
+  const size_t size = d->dtype == NERF_F32 ? 4 : 2;
+  int heads = 0;
+  uintptr_t align = 16;    // what every address divides by: bases and strides
+  for (int k = 0; k < d->n_tensors; ++k) {
+    const nerf_rotary_tensor& t = d->tensor[k];
+    if (t.heads < 0) return set_error(NERF_E_INVALID, "nerf_rotary_axes: %d heads", t.heads);
+    if (t.heads > (1 << 20)) return set_error(NERF_E_INVALID, "nerf_rotary_axes: %d heads", t.heads);
+    a.t[k].x = t.x, a.t[k].out = t.out, a.t[k].heads = t.heads, a.t[k].copy_tail = t.x != t.out;
+    uintptr_t bits = uintptr_t(t.x) | uintptr_t(t.out);
+    for (int i = 0; i < 3; ++i) {
+      a.t[k].xs[i] = t.x_stride[i], a.t[k].os[i] = t.out_stride[i];
+      bits |= uintptr_t(t.x_stride[i] * int64_t(size)) | uintptr_t(t.out_stride[i] * int64_t(size));
+    }
+    while (bits & (align - 1)) align >>= 1;
+    heads += t.heads;
+  }
+  if (d->n_batch == 0 || d->n_tokens == 0 || heads == 0) return NERF_OK;
+  for (int k = 0; k < d->n_tensors; ++k)
+    if (d->tensor[k].heads && (!d->tensor[k].x || !d->tensor[k].out)) return set_error(NERF_E_INVALID, "nerf_rotary_axes: null tensor %d", k);
+  if (!d->positions) return set_error(NERF_E_INVALID, "nerf_rotary_axes: null positions");
+  if (align < size) return set_error(NERF_E_INVALID, "nerf_rotary_axes: a tensor is not aligned to its type");
+  for (int i = 0; i < 3; ++i) a.ps[i] = d->position_stride[i];
+  a.pos = d->positions, a.pos_dtype = d->position_dtype;
+  a.n_tensors = d->n_tensors, a.dim = d->head_dim, a.interleaved = d->interleaved != 0;
+  a.sign = d->inverse ? -1.0f : 1.0f;
+  a.n_tokens = d->n_tokens;
+  // values per access: 16 bytes where addresses, halves and tail allow it, else 2 values, else 1
+  const int tail = d->head_dim - 2 * a.pairs;
+  auto fits = [&](int v) {
+    return align >= v * size && tail % v == 0 && (a.interleaved ? (2 * a.pairs) % v == 0 : a.pairs % v == 0);
+  };
+  const int v = fits(int(16 / size)) ? int(16 / size) : fits(2) ? 2 : 1;
+  a.rot_groups = a.interleaved && v > 1 ? 2 * a.pairs / v : a.pairs / v;
+  a.groups = a.rot_groups + tail / v;
+  const double items = double(d->n_batch) * double(d->n_tokens) * a.groups;
+  if (items > 5.0e11) return set_error(NERF_E_INVALID, "nerf_rotary_axes: too many tokens");
+  a.items = long(d->n_batch) * a.n_tokens * a.groups;
+  const hipStream_t s = (hipStream_t)stream;
+  const hipError_t e = d->dtype == NERF_F32        ? launch_v<float>(a, v, heads, s)
+                       : d->dtype == NERF_BFLOAT16 ? launch_v<__bf16>(a, v, heads, s)
+                                                   : launch_v<_Float16>(a, v, heads, s);
+  if (e != hipSuccess) return set_error(NERF_E_HIP, "nerf_rotary_axes: %s", hipGetErrorString(e));
+  return NERF_OK;
+}

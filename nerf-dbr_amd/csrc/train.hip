@@ -1308,6 +1308,15 @@ struct nerf_trainer {
   // the rays): fork after the rays and samples, join before the loss and the update
   hipStream_t side = nullptr;
   hipEvent_t fork = nullptr, join = nullptr;
+  // nerf_trainer_set_optimizer: AdamW's step count on the device, its norm partials and, with 8-bit
+  // moments, the codes [2][kNetFloats] and scales [2][kMomentBlocks] that stand in for m and v
+  int optimizer = NERF_OPT_ADAM;
+  int state_bits = 32;
+  nerf_adamw_control* control = nullptr;
+  void* norm_ws = nullptr;
+  size_t norm_ws_bytes = 0;
+  unsigned char* codes[2] = {};
+  float* scales[2] = {};
 };
 
 namespace {
@@ -1627,7 +1636,55 @@ int net_pass(nerf_trainer* tr, int net, const float* rays_o, const float* rays_d
   return NERF_OK;
 }
 
+size_t param_offset(int i) { return size_t(tensor_desc(i).off); }
+size_t param_count(int i) { return size_t(tensor_desc(i).rows) * size_t(tensor_desc(i).cols); }
+
+// 8-bit moments: each tensor's blocks of NERF_ADAMW_BLOCK values follow the previous tensor's.
+size_t moment_block(int i) {
+  size_t b = 0;
+  for (int k = 0; k < i; ++k) b += (param_count(k) + NERF_ADAMW_BLOCK - 1) / NERF_ADAMW_BLOCK;
+  return b;
+}
+
+// Both nets' 44 tensors as nerf_adamw_step takes them.
+void adamw_tensors(const nerf_trainer* tr, nerf_adamw_tensor* out) {
+  const size_t blocks = moment_block(NERF_N_PARAMS);
+  for (int net = 0; net < 2; ++net)
+    for (int i = 0; i < NERF_N_PARAMS; ++i) {
+      const size_t at = net * size_t(kNetFloats) + param_offset(i), b = net * blocks + moment_block(i);
+      nerf_adamw_tensor& t = *out++;
+      t = nerf_adamw_tensor{};
+      t.param = tr->params + at;
+      t.grad = tr->grads + at;
+      const bool eight = tr->state_bits == 8;
+      t.exp_avg = eight ? (void*)(tr->codes[0] + at) : (void*)(tr->m + at);
+      t.exp_avg_sq = eight ? (void*)(tr->codes[1] + at) : (void*)(tr->v + at);
+      t.exp_avg_scale = eight ? tr->scales[0] + b : nullptr;
+      t.exp_avg_sq_scale = eight ? tr->scales[1] + b : nullptr;
+      t.numel = int64_t(param_count(i));
+      t.weight_decay = tr->cfg.weight_decay;
+      t.grad_dtype = NERF_F32;
+    }
+}
+
+int adamw_update(nerf_trainer* tr, hipStream_t s) {
+  nerf_adamw_tensor t[2 * NERF_N_PARAMS];
+  adamw_tensors(tr, t);
+  nerf_adamw_config c{};
+  c.lr = tr->lr, c.beta1 = tr->cfg.beta1, c.beta2 = tr->cfg.beta2, c.eps = tr->cfg.eps;
+  c.max_norm = tr->cfg.grad_clip > 0.0 ? tr->cfg.grad_clip : 0.0;
+  c.state_bits = tr->state_bits;
+  c.flags = c.max_norm > 0.0 ? NERF_ADAMW_WRITE_GRADS : 0;   // param.grad after the step: the clipped gradient
+  const int rc = nerf_adamw_step(&c, 2 * NERF_N_PARAMS, t, tr->control, tr->norm_ws, tr->norm_ws_bytes, s);
+  if (rc != NERF_OK) return rc;
+  HIP_TRY(pack_operands(tr, s));
+  tr->steps += 1;
+  tr->lr = tr->lr * tr->cfg.lr_gamma;   // ExponentialLR.step: lr * gamma
+  return NERF_OK;
+}
+
 int update_impl(nerf_trainer* tr, hipStream_t s) {
+  if (tr->optimizer == NERF_OPT_ADAMW) return adamw_update(tr, s);
   double* sq = (double*)(tr->scal + 4);
   const long n = 2 * kNetFloats;
   const bool clip = tr->cfg.grad_clip > 0.0;
@@ -1659,9 +1716,6 @@ int update_impl(nerf_trainer* tr, hipStream_t s) {
   tr->lr = tr->lr * tr->cfg.lr_gamma;   // ExponentialLR.step: lr * gamma
   return NERF_OK;
 }
-
-size_t param_offset(int i) { return size_t(tensor_desc(i).off); }
-size_t param_count(int i) { return size_t(tensor_desc(i).rows) * size_t(tensor_desc(i).cols); }
 
 }  // namespace
 
@@ -1751,6 +1805,12 @@ void nerf_trainer_destroy(nerf_trainer* tr) {
   for (float* p : {tr->params, tr->own_grads, tr->m, tr->v, tr->gemmw, tr->ztab, tr->scal, tr->ws, tr->part})
     if (p) (void)hipFree(p);
   if (tr->bad) (void)hipFree(tr->bad);
+  if (tr->control) (void)hipFree(tr->control);
+  if (tr->norm_ws) (void)hipFree(tr->norm_ws);
+  for (int k = 0; k < 2; ++k) {
+    if (tr->codes[k]) (void)hipFree(tr->codes[k]);
+    if (tr->scales[k]) (void)hipFree(tr->scales[k]);
+  }
   if (tr->x3) (void)hipFree(tr->x3);
   if (tr->bx3) (void)hipFree(tr->bx3);
   for (auto& e : tr->ev)
@@ -1764,6 +1824,70 @@ void nerf_trainer_destroy(nerf_trainer* tr) {
 }  // extern "C"
 
 namespace {
+
+// The e4m3 value of a code (OCP: 1 sign, 4 exponent (bias 7), 3 mantissa bits; 0x7f and 0xff are NaN).
+float e4m3_value(unsigned char c) {
+  const int e = (c >> 3) & 15, f = c & 7;
+  const float v = (c & 127) == 127 ? NAN : e ? std::ldexp(float(8 + f), e - 10) : std::ldexp(float(f), -9);
+  return c & 128 ? -v : v;
+}
+
+// Moment k (0: m, 1: v) of one net as fp32 host values, and back; the device is idle.
+int read_moments(nerf_trainer* tr, int k, int net, float* host) {
+  if (tr->state_bits == 32) {
+    HIP_TRY(hipMemcpy(host, (k ? tr->v : tr->m) + net * kNetFloats, sizeof(float) * kNetFloats, hipMemcpyDeviceToHost));
+    return NERF_OK;
+  }
+  const size_t blocks = moment_block(NERF_N_PARAMS);
+  std::vector<unsigned char> codes(kNetFloats);
+  std::vector<float> scales(blocks);
+  HIP_TRY(hipMemcpy(codes.data(), tr->codes[k] + net * kNetFloats, kNetFloats, hipMemcpyDeviceToHost));
+  HIP_TRY(hipMemcpy(scales.data(), tr->scales[k] + net * blocks, blocks * sizeof(float), hipMemcpyDeviceToHost));
+  for (int i = 0; i < NERF_N_PARAMS; ++i)
+    for (size_t e = 0; e < param_count(i); ++e) {
+      const size_t at = param_offset(i) + e;
+      const float x = e4m3_value(codes[at]) * scales[moment_block(i) + e / NERF_ADAMW_BLOCK];
+      host[at] = k ? x * x : x;
+    }
+  return NERF_OK;
+}
+int write_moments(nerf_trainer* tr, int k, int net, const float* host) {
+  if (tr->state_bits == 32) {
+    HIP_TRY(hipMemcpy((k ? tr->v : tr->m) + net * kNetFloats, host, sizeof(float) * kNetFloats, hipMemcpyHostToDevice));
+    return NERF_OK;
+  }
+  const size_t blocks = moment_block(NERF_N_PARAMS);
+  std::vector<unsigned char> codes(kNetFloats, 0);
+  std::vector<float> scales(blocks, 0.0f);
+  for (int i = 0; i < NERF_N_PARAMS; ++i)
+    for (size_t e = 0; e < param_count(i); e += NERF_ADAMW_BLOCK) {
+      const size_t end = std::min(param_count(i), e + NERF_ADAMW_BLOCK), at = param_offset(i);
+      float x[NERF_ADAMW_BLOCK], top = 0.0f;
+      for (size_t j = e; j < end; ++j) {
+        x[j - e] = k ? std::sqrt(host[at + j]) : host[at + j];
+        top = std::max(top, std::fabs(x[j - e]));
+      }
+      const float scale = top / 448.0f;
+      scales[moment_block(i) + e / NERF_ADAMW_BLOCK] = scale;
+      if (!(scale > 0.0f)) continue;
+      for (size_t j = e; j < end; ++j) {
+        const float q = std::min(448.0f, std::max(-448.0f, x[j - e] / scale));
+        nerf_f32_to_e4m3(&q, 1, &codes[at + j]);
+        if (k && x[j - e] > 0.0f && codes[at + j] == 0) codes[at + j] = 1;
+      }
+    }
+  HIP_TRY(hipMemcpy(tr->codes[k] + net * kNetFloats, codes.data(), kNetFloats, hipMemcpyHostToDevice));
+  HIP_TRY(hipMemcpy(tr->scales[k] + net * blocks, scales.data(), blocks * sizeof(float), hipMemcpyHostToDevice));
+  return NERF_OK;
+}
+// AdamW's device step count follows the trainer's; the device is idle.
+int sync_control(nerf_trainer* tr) {
+  if (!tr->control) return NERF_OK;
+  nerf_adamw_control c{};
+  c.steps = int32_t(tr->steps);
+  HIP_TRY(hipMemcpy(tr->control, &c, sizeof c, hipMemcpyHostToDevice));
+  return NERF_OK;
+}
 
 // A call on a different stream than the previous call's waits for that call's work.
 int order_after_last(nerf_trainer* tr, hipStream_t s) {
@@ -1889,6 +2013,51 @@ int nerf_trainer_update(nerf_trainer* tr, void* stream) {
   return record_done(tr, s);
 }
 
+int nerf_trainer_set_optimizer(nerf_trainer* tr, int optimizer, int state_bits) {
+  if (!tr) return set_error(NERF_E_INVALID, "null trainer");
+  if (optimizer != NERF_OPT_ADAM && optimizer != NERF_OPT_ADAMW)
+    return set_error(NERF_E_INVALID, "nerf_trainer_set_optimizer: optimizer %d", optimizer);
+  if (state_bits != 32 && (state_bits != 8 || optimizer != NERF_OPT_ADAMW))
+    return set_error(NERF_E_INVALID, "nerf_trainer_set_optimizer: %d-bit moments (32, or 8 with NERF_OPT_ADAMW)", state_bits);
+  DeviceGuardT dg(tr->device);
+  HIP_TRY(hipDeviceSynchronize());
+  const size_t n = 2 * size_t(kNetFloats), blocks = 2 * moment_block(NERF_N_PARAMS);
+  if (optimizer == NERF_OPT_ADAMW && !tr->control) {
+    nerf_adamw_tensor t[2 * NERF_N_PARAMS];
+    adamw_tensors(tr, t);
+    tr->norm_ws_bytes = nerf_adamw_workspace(2 * NERF_N_PARAMS, t);
+    if (!tr->norm_ws) HIP_TRY(hipMalloc(&tr->norm_ws, tr->norm_ws_bytes));
+    HIP_TRY(hipMalloc((void**)&tr->control, sizeof(nerf_adamw_control)));
+  }
+  if (state_bits == 8)
+    for (int k = 0; k < 2; ++k) {
+      if (!tr->codes[k]) HIP_TRY(hipMalloc((void**)&tr->codes[k], n));
+      if (!tr->scales[k]) HIP_TRY(hipMalloc((void**)&tr->scales[k], blocks * sizeof(float)));
+    }
+  if (state_bits != tr->state_bits) {   // the moments keep their values
+    std::vector<float> host[2];
+    for (int k = 0; k < 2; ++k) {
+      host[k].resize(n);
+      for (int net = 0; net < 2; ++net) {
+        const int rc = read_moments(tr, k, net, host[k].data() + net * kNetFloats);
+        if (rc != NERF_OK) return rc;
+      }
+    }
+    const int before = tr->state_bits;
+    tr->state_bits = state_bits;
+    for (int k = 0; k < 2; ++k)
+      for (int net = 0; net < 2; ++net) {
+        const int rc = write_moments(tr, k, net, host[k].data() + net * kNetFloats);
+        if (rc != NERF_OK) {
+          tr->state_bits = before;
+          return rc;
+        }
+      }
+  }
+  tr->optimizer = optimizer;
+  return sync_control(tr);
+}
+
 int nerf_trainer_read(nerf_trainer* tr, int what, int net, float* const* host_out, int n_params) {
   if (!tr || !host_out) return set_error(NERF_E_INVALID, "nerf_trainer_read: null argument");
   if (net != NERF_NET_COARSE && net != NERF_NET_FINE) return set_error(NERF_E_INVALID, "bad net %d", net);
@@ -1902,7 +2071,12 @@ int nerf_trainer_read(nerf_trainer* tr, int what, int net, float* const* host_ou
   HIP_TRY(hipMemcpy(&bad, tr->bad, sizeof(int), hipMemcpyDeviceToHost));
   if (bad) return set_error(NERF_E_INVALID, "a train_step's select held an index outside the image");
   std::vector<float> host(kNetFloats);
-  HIP_TRY(hipMemcpy(host.data(), src + net * kNetFloats, sizeof(float) * kNetFloats, hipMemcpyDeviceToHost));
+  if (what == NERF_TR_EXP_AVG || what == NERF_TR_EXP_AVG_SQ) {
+    const int rc = read_moments(tr, what == NERF_TR_EXP_AVG_SQ, net, host.data());
+    if (rc != NERF_OK) return rc;
+  } else {
+    HIP_TRY(hipMemcpy(host.data(), src + net * kNetFloats, sizeof(float) * kNetFloats, hipMemcpyDeviceToHost));
+  }
   for (int i = 0; i < NERF_N_PARAMS; ++i) {
     if (!host_out[i]) return set_error(NERF_E_INVALID, "nerf_trainer_read: null buffer %d", i);
     std::memcpy(host_out[i], host.data() + param_offset(i), sizeof(float) * param_count(i));
@@ -1939,6 +2113,7 @@ int nerf_trainer_write(nerf_trainer* tr, int what, int net, const float* const* 
   }
   DeviceGuardT dg(tr->device);
   HIP_TRY(hipDeviceSynchronize());
+  if (what == NERF_TR_EXP_AVG || what == NERF_TR_EXP_AVG_SQ) return write_moments(tr, what == NERF_TR_EXP_AVG_SQ, net, host.data());
   HIP_TRY(hipMemcpy(dst + net * kNetFloats, host.data(), sizeof(float) * kNetFloats, hipMemcpyHostToDevice));
   if (what == NERF_TR_PARAMS) {   // the kernels' operand copies of the weights
     HIP_TRY(pack_operands(tr, 0));
@@ -1952,7 +2127,10 @@ int nerf_trainer_set_schedule(nerf_trainer* tr, long steps, double lr) {
   if (steps < 0 || !(lr >= 0.0)) return set_error(NERF_E_INVALID, "nerf_trainer_set_schedule: steps %ld, lr %g", steps, lr);
   tr->steps = steps;
   tr->lr = lr;
-  return NERF_OK;
+  if (!tr->control) return NERF_OK;
+  DeviceGuardT dg(tr->device);
+  HIP_TRY(hipDeviceSynchronize());
+  return sync_control(tr);
 }
 
 int nerf_trainer_set_precision(nerf_trainer* tr, int precision) {

@@ -39,7 +39,12 @@ def main(argv=None) -> int:
     ap.add_argument("--precisions", default="fp32,f16x3,bf16")
     ap.add_argument("--hierarchical", type=int, default=0, help="also run bf16 with N importance samples")
     ap.add_argument("--output_dir", default="outputs")
+    ap.add_argument("--optimizer", default="adam", choices=("adam", "adamw"), help="the training step's optimizer")
+    ap.add_argument("--optimizer_state_bits", type=int, default=32, choices=(32, 8),
+                    help="bits of the optimizer's moments (8: with --optimizer adamw)")
     args = ap.parse_args(argv)
+    if args.optimizer_state_bits == 8 and args.optimizer != "adamw":
+        ap.error("--optimizer_state_bits 8 goes with --optimizer adamw")
 
     from nerf_amd import weights as W
     from nerf_amd.benchmark.benchmark_suite import UnifiedBenchmarkSuite
@@ -57,7 +62,10 @@ def main(argv=None) -> int:
         datasets = load_synthetic_data(args.data_dir, "cpu")
         if "train" not in datasets:
             raise ValueError(f"Training dataset not found in {args.data_dir}")
-        trainer = MI355XTrainer(dict(MAIN_CONFIG))
+        config = dict(MAIN_CONFIG)
+        if args.optimizer != "adam":
+            config.update(optimizer=args.optimizer, optimizer_state_bits=args.optimizer_state_bits)
+        trainer = MI355XTrainer(config)
         trainer.train(datasets["train"], datasets.get("val"), args.epochs)
         trainer.save_checkpoint(args.checkpoint)
         print(f"\nTraining completed! Model saved to: {args.checkpoint}")

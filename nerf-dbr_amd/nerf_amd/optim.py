@@ -1,0 +1,248 @@
+"""AdamW over many tensors at once on the MI355X, moments in 32 or 8 bits (``nerf_adamw_step``).
+
+Stands beside the trainer's Adam (``nerf_trainer_update``); ``MI355XTrainer`` runs the same kernels
+with ``config["optimizer"] = "adamw"``.  The formula is torch.optim.AdamW's
+(decoupled weight decay), with torch.nn.utils.clip_grad_norm_'s factor when ``max_norm`` is given.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Union
+
+import numpy as np
+
+from . import runtime as rt
+
+BLOCK = rt.NERF_ADAMW_BLOCK
+
+
+def blocks(numel: int) -> int:
+    """Scales of an 8-bit moment of numel values."""
+    return -(-int(numel) // BLOCK)
+
+
+class AdamW:
+    """AdamW on device tensors: ``step(grads)`` updates every parameter in one or two kernel launches per 48 tensors.
+
+    params: contiguous float32, bfloat16 or float16 tensors on one device, none twice.  A 16-bit
+    parameter has a float32 master here: the step updates the master and writes its rounded value.
+    weight_decay: one number, or one per parameter.  state_bits: 32 (float32 moments) or 8 (e4m3 codes of
+    m and of sqrt(v), one float32 scale per 256 values).  max_norm: clip all gradients by their norm.
+    skip_nonfinite: leave everything unchanged when the norm is inf or NaN (``skipped`` counts).
+    state: moments to adopt without a copy, as ``state_dict`` gives them (``steps``, ``exp_avg``,
+    ``exp_avg_sq``, with 8 bits ``exp_avg_scale`` and ``exp_avg_sq_scale``, ``masters``).
+
+    The step count lives on the device, so a captured step counts its replays; lr may be a float32
+    device tensor, which a replay reads anew."""
+
+    def __init__(self, params: Sequence, lr: Union[float, object] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay=1e-2, state_bits: int = 32, max_norm: Optional[float] = None,
+                 skip_nonfinite: bool = False, write_grads: bool = False, state: Optional[dict] = None):
+        import torch
+
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits {state_bits}: 32 or 8")
+        self._model = {torch.bfloat16: rt.NERF_BFLOAT16, torch.float16: rt.NERF_FLOAT16}
+        self._grad = {torch.float32: rt.NERF_F32, **self._model}
+        device = self.params[0].device
+        for i, p in enumerate(self.params):
+            if p.dtype not in self._grad:
+                raise ValueError(f"parameter {i} is {p.dtype}: float32, bfloat16 or float16")
+            if not p.is_contiguous():
+                raise ValueError(f"parameter {i} is not contiguous")
+            if p.device != device:
+                raise ValueError(f"parameter {i} is on {p.device}, not on {device}")
+        if not sum(p.numel() for p in self.params):
+            raise ValueError("no values in the parameters")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters share memory (one is given twice?)")
+        decay = [float(weight_decay)] * len(self.params) if np.ndim(weight_decay) == 0 else [float(w) for w in weight_decay]
+        if len(decay) != len(self.params):
+            raise ValueError(f"{len(self.params)} weight decays needed, got {len(decay)}")
+        if min(decay) < 0.0 or not all(map(np.isfinite, decay)):
+            raise ValueError("weight decays must be finite and not negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+            raise ValueError(f"betas {betas}, eps {eps}")
+        if max_norm is not None and not max_norm > 0.0:
+            raise ValueError(f"max_norm {max_norm}: positive, or None")
+        self.device, self.state_bits, self.max_norm = device, state_bits, max_norm
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), float(eps), decay
+        self._norm = max_norm is not None or skip_nonfinite
+        self._lr(lr)
+        if device.type != "cuda":
+            raise ValueError(f"device tensors are needed, got {device}")
+        state = dict(state or {})
+        moment = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+
+        def store(key, dtype, sizes):
+            given = state.pop(key, None)
+            if given is None:
+                return [torch.zeros(n, dtype=dtype, device=device) for n in sizes]
+            given = list(given)
+            if len(given) != len(sizes):
+                raise ValueError(f"state {key!r}: {len(sizes)} tensors needed, got {len(given)}")
+            for i, (t, n) in enumerate(zip(given, sizes)):
+                if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
+                    raise ValueError(f"state {key!r}[{i}] must be {n} contiguous values of {dtype} on {device}")
+            return given
+
+        numels = [p.numel() for p in self.params]
+        self.exp_avg = store("exp_avg", moment, numels)
+        self.exp_avg_sq = store("exp_avg_sq", moment, numels)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if state_bits == 8:
+            self.exp_avg_scale = store("exp_avg_scale", torch.float32, [blocks(n) for n in numels])
+            self.exp_avg_sq_scale = store("exp_avg_sq_scale", torch.float32, [blocks(n) for n in numels])
+        masters = state.pop("masters", None)
+        if masters is not None and len(masters) != len(self.params):
+            raise ValueError(f"state 'masters': {len(self.params)} entries needed")
+        self.masters = []
+        for i, p in enumerate(self.params):
+            m = masters[i] if masters is not None else None
+            if p.dtype == torch.float32:
+                m = None
+            elif m is None:
+                m = p.detach().float()
+            elif m.dtype != torch.float32 or m.numel() != p.numel() or not m.is_contiguous() or m.device != device:
+                raise ValueError(f"state 'masters'[{i}] must be {p.numel()} contiguous float32 values on {device}")
+            self.masters.append(m)
+        steps = int(state.pop("steps", 0))
+        if state:
+            raise ValueError(f"unknown state {sorted(state)}")
+        self._control = torch.zeros(ctypes.sizeof(rt.AdamWControl) // 4, dtype=torch.int32, device=device)
+        self._control[0] = steps
+        self.grad_norm = self._control.view(torch.float32)[3]
+
+        n = len(self.params)
+        self._table = (rt.AdamWTensor * n)()
+        self._columns = np.frombuffer(self._table, dtype=np.dtype(rt.AdamWTensor))
+        self._numels = np.array(numels, np.int64)
+        for i, p in enumerate(self.params):
+            t, m = self._table[i], self.masters[i]
+            t.param = (p if m is None else m).data_ptr()
+            t.model = 0 if m is None else p.data_ptr()
+            t.model_dtype = 0 if m is None else self._model[p.dtype]
+            t.exp_avg, t.exp_avg_sq = self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr()
+            if state_bits == 8:
+                t.exp_avg_scale, t.exp_avg_sq_scale = self.exp_avg_scale[i].data_ptr(), self.exp_avg_sq_scale[i].data_ptr()
+            t.numel, t.weight_decay = p.numel(), decay[i]
+        self._shapes = [p.shape for p in self.params]
+        c = rt.AdamWConfig()
+        c.beta1, c.beta2, c.eps = float(betas[0]), float(betas[1]), float(eps)
+        c.max_norm = 0.0 if max_norm is None else float(max_norm)
+        c.state_bits = state_bits
+        c.flags = (rt.NERF_ADAMW_SKIP_NONFINITE if skip_nonfinite else 0) | (rt.NERF_ADAMW_WRITE_GRADS if write_grads else 0)
+        self._config = c
+        self._workspace_bytes = rt.load_library().nerf_adamw_workspace(n, self._table) if self._norm else 0
+
+    def _lr(self, lr):
+        """(host value, device tensor or None) of a learning rate."""
+        import torch
+
+        if isinstance(lr, torch.Tensor):
+            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
+                raise ValueError(f"a learning rate on the device is one float32 value on {self.device}")
+            return 0.0, lr
+        lr = float(lr)
+        if not (lr >= 0.0 and np.isfinite(lr)):
+            raise ValueError(f"learning rate {lr}")
+        return lr, None
+
+    def step(self, grads: Optional[Sequence] = None, lr=None, stream=None):
+        """One step on grads (one per parameter; None entries are left out; default: the parameters'
+        ``.grad``), float32 or the 16-bit types, contiguous, of the parameters' shapes.  lr replaces the
+        optimizer's for this step.  Returns the gradients' norm (a device scalar that the next step
+        overwrites) if one is computed, else None."""
+        import torch
+
+        from .operators import _On
+
+        grads = [p.grad for p in self.params] if grads is None else grads
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(self.params)} gradients needed, got {len(grads)}")
+        host, on_device = self._lr(self.lr if lr is None else lr)
+        codes, device, shapes = self._grad, self.device, self._shapes
+        ptr, kind, numel = [], [], self._numels
+        for i, g in enumerate(grads):
+            if g is None:
+                ptr.append(0)
+                kind.append(0)
+                continue
+            k = codes.get(g.dtype)
+            if k is None or g.shape != shapes[i] or not g.is_contiguous() or g.device != device:
+                raise ValueError(f"gradient {i} {tuple(g.shape)} {g.dtype} on {g.device} must be contiguous, "
+                                 f"{tuple(shapes[i])} and on {device}")
+            ptr.append(g.data_ptr())
+            kind.append(k)
+        col = self._columns
+        col["grad"] = ptr
+        col["grad_dtype"] = kind
+        none = [i for i, g in enumerate(grads) if g is None]
+        col["numel"] = numel
+        if none:
+            col["numel"][none] = 0
+            if not col["numel"].any():
+                raise ValueError("no gradients")
+        c = self._config
+        c.lr = host
+        c.lr_device = None if on_device is None else on_device.data_ptr()
+        lib = rt.load_library()
+        with _On(torch, device, stream) as on:
+            n = self._workspace_bytes
+            if none and n:    # fewer values can be cut into more, smaller pieces
+                n = max(n, lib.nerf_adamw_workspace(len(ptr), self._table))
+            ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+            rt._check(lib.nerf_adamw_step(ctypes.byref(c), len(ptr), self._table, self._control.data_ptr(),
+                                          None if ws is None else ws.data_ptr(), n, on.stream))
+        return self.grad_norm if self._norm else None
+
+    @property
+    def steps(self) -> int:
+        """Steps taken (synchronises)."""
+        return int(self._control[0].item())
+
+    @property
+    def skipped(self) -> int:
+        """Steps left out because their norm was not finite (synchronises)."""
+        return int(self._control[2].item())
+
+    def moments(self, i: int):
+        """(m, v) of parameter i as float32 tensors of its shape."""
+        m, v = self.exp_avg[i].float(), self.exp_avg_sq[i].float()
+        if self.state_bits == 8:
+            n = m.numel()
+            m = m * self.exp_avg_scale[i].repeat_interleave(BLOCK)[:n]
+            v = (v * self.exp_avg_sq_scale[i].repeat_interleave(BLOCK)[:n]).square()
+        return m.reshape(self._shapes[i]), v.reshape(self._shapes[i])
+
+    def state_dict(self) -> dict:
+        """The optimizer's state: the tensors themselves, in the form ``state=`` takes."""
+        d = {"steps": self.steps, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "masters": self.masters}
+        if self.state_bits == 8:
+            d.update(exp_avg_scale=self.exp_avg_scale, exp_avg_sq_scale=self.exp_avg_sq_scale)
+        return d
+
+    def load_state_dict(self, state: dict) -> None:
+        """Copy a state_dict's values into this optimizer's own stores (same state_bits)."""
+        mine = self.state_dict()
+        if set(state) != set(mine):
+            raise ValueError(f"state holds {sorted(state)}, not {sorted(mine)}")
+        for key, own in mine.items():
+            if key == "steps":
+                continue
+            if len(state[key]) != len(own):
+                raise ValueError(f"state {key!r}: {len(own)} tensors needed, got {len(state[key])}")
+            for i, (a, b) in enumerate(zip(own, state[key])):
+                if (a is None) != (b is None) or (a is not None and (a.numel() != b.numel() or a.dtype != b.dtype)):
+                    raise ValueError(f"state {key!r}[{i}] does not fit")
+        for key, own in mine.items():
+            if key != "steps":
+                for a, b in zip(own, state[key]):
+                    if a is not None:
+                        a.copy_(b.reshape(a.shape))
+        self._control.zero_()
+        self._control[0] = int(state["steps"])

@@ -97,6 +97,13 @@ SIGNATURES = {
     "nerf_trainer_set_profiling": (_c.c_int, [_P, _c.c_int]),
     "nerf_trainer_stage_ms": (_c.c_int, [_P, _FP]),
     "nerf_trainer_gemm_flops": (_c.c_double, [_P]),
+    "nerf_rotary_axes": (_c.c_int, [_P, _P]),
+    "nerf_gated_block_workspace": (_c.c_size_t, [_P, _c.c_int]),
+    "nerf_gated_block_forward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_size_t, _P]),
+    "nerf_gated_block_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P, _c.c_size_t, _P]),
+    "nerf_adamw_workspace": (_c.c_size_t, [_c.c_int, _P]),
+    "nerf_adamw_step": (_c.c_int, [_P, _c.c_int, _P, _P, _P, _c.c_size_t, _P]),
+    "nerf_trainer_set_optimizer": (_c.c_int, [_P, _c.c_int, _c.c_int]),
 }
 
 
@@ -105,6 +112,56 @@ class TrainConfig(_c.Structure):
     _fields_ = [("lr", _c.c_double), ("beta1", _c.c_double), ("beta2", _c.c_double), ("eps", _c.c_double),
                 ("weight_decay", _c.c_double), ("lr_gamma", _c.c_double), ("grad_clip", _c.c_double),
                 ("n_coarse", _c.c_int), ("n_fine", _c.c_int), ("near_", _c.c_float), ("far_", _c.c_float)]
+
+
+NERF_F32, NERF_BFLOAT16, NERF_FLOAT16, NERF_INT32, NERF_INT64 = 0, 1, 2, 3, 4
+NERF_ROTARY_MAX_AXES, NERF_ROTARY_MAX_PAIRS = 4, 256
+NERF_SILU, NERF_GELU, NERF_RELU = 0, 1, 2
+NERF_ADAMW_BLOCK = 256
+NERF_ADAMW_SKIP_NONFINITE, NERF_ADAMW_WRITE_GRADS = 1, 2
+NERF_OPT_ADAM, NERF_OPT_ADAMW = 0, 1
+
+
+class RotaryTensor(_c.Structure):
+    """nerf_rotary_tensor (include/nerf_mi355x.h)."""
+    _fields_ = [("x", _P), ("out", _P), ("heads", _c.c_int), ("x_stride", _c.c_int64 * 3),
+                ("out_stride", _c.c_int64 * 3)]
+
+
+class RotaryDesc(_c.Structure):
+    """nerf_rotary_desc."""
+    _fields_ = [("dtype", _c.c_int), ("head_dim", _c.c_int), ("n_axes", _c.c_int),
+                ("sections", _c.c_int * NERF_ROTARY_MAX_AXES), ("shared_ladder", _c.c_int), ("interleaved", _c.c_int),
+                ("inverse", _c.c_int), ("base", _c.c_double), ("frequencies", _c.POINTER(_c.c_double)),
+                ("positions", _P), ("position_dtype", _c.c_int), ("position_stride", _c.c_int64 * 3),
+                ("n_batch", _c.c_int), ("n_tokens", _c.c_int64), ("n_tensors", _c.c_int), ("tensor", RotaryTensor * 2)]
+
+
+class BlockDesc(_c.Structure):
+    """nerf_block_desc."""
+    _fields_ = [("dtype", _c.c_int), ("activation", _c.c_int), ("rows", _c.c_int64), ("width", _c.c_int),
+                ("hidden", _c.c_int), ("out", _c.c_int), ("x", _P), ("w_gate", _P), ("w_up", _P), ("w_down", _P),
+                ("ld_x", _c.c_int64), ("ld_gate", _c.c_int64), ("ld_up", _c.c_int64), ("ld_down", _c.c_int64)]
+
+
+class AdamWControl(_c.Structure):
+    """nerf_adamw_control."""
+    _fields_ = [("steps", _c.c_int32), ("ticket", _c.c_uint32), ("skipped", _c.c_int32), ("norm", _c.c_float),
+                ("factor", _c.c_float), ("reserved", _c.c_int32 * 3)]
+
+
+class AdamWTensor(_c.Structure):
+    """nerf_adamw_tensor (addresses as integers)."""
+    _fields_ = [("param", _c.c_uint64), ("model", _c.c_uint64), ("grad", _c.c_uint64), ("exp_avg", _c.c_uint64),
+                ("exp_avg_sq", _c.c_uint64), ("exp_avg_scale", _c.c_uint64), ("exp_avg_sq_scale", _c.c_uint64),
+                ("numel", _c.c_int64), ("weight_decay", _c.c_double), ("model_dtype", _c.c_int32),
+                ("grad_dtype", _c.c_int32)]
+
+
+class AdamWConfig(_c.Structure):
+    """nerf_adamw_config."""
+    _fields_ = [("lr", _c.c_double), ("beta1", _c.c_double), ("beta2", _c.c_double), ("eps", _c.c_double),
+                ("max_norm", _c.c_double), ("lr_device", _P), ("state_bits", _c.c_int32), ("flags", _c.c_int32)]
 
 
 NERF_TRAIN_NO_UPDATE = 1

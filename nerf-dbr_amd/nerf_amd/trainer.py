@@ -125,8 +125,11 @@ class MI355XTrainer:
         # "bf16x3": split bf16, faster, gradients as close to the float64 step as fp32's;
         # include/nerf_mi355x.h)
         self.precision = "fp32"
+        # "adam" (the reference's) or "adamw", whose moments may be kept in 8 bits
+        self.optimizer, self.optimizer_state_bits = "adam", 32
         try:
             self.set_precision(str(c.get("precision", "fp32")))
+            self.set_optimizer(str(c.get("optimizer", "adam")), int(c.get("optimizer_state_bits", 32)))
         except ValueError:
             self.close()
             raise
@@ -288,6 +291,19 @@ class MI355XTrainer:
         rt._check(self.lib.nerf_trainer_set_precision(self._h, rt.PRECISIONS[precision]))
         self.precision = precision
 
+    def set_optimizer(self, optimizer: str, state_bits: int = 32) -> None:
+        """"adam" (trainer.py:57) or "adamw" (decoupled weight decay, moments in 32 or 8 bits;
+        nerf_trainer_set_optimizer in include/nerf_mi355x.h)."""
+        if optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer {optimizer!r}: 'adam' or 'adamw'")
+        if state_bits != 32 and (state_bits != 8 or optimizer != "adamw"):
+            raise ValueError(f"optimizer_state_bits {state_bits}: 32, or 8 with 'adamw'")
+        if (optimizer, state_bits) == (self.optimizer, self.optimizer_state_bits):
+            return
+        kind = rt.NERF_OPT_ADAMW if optimizer == "adamw" else rt.NERF_OPT_ADAM
+        rt._check(self.lib.nerf_trainer_set_optimizer(self._h, kind, state_bits))
+        self.optimizer, self.optimizer_state_bits = optimizer, state_bits
+
     def set_profiling(self, enable: bool) -> None:
         rt._check(self.lib.nerf_trainer_set_profiling(self._h, 1 if enable else 0))
 
@@ -375,7 +391,7 @@ class MI355XTrainer:
         print("Training completed!")
 
     def _torch_optimizer(self):
-        """torch.optim.Adam + ExponentialLR over CPU stand-ins of the 44 parameters (coarse then
+        """torch.optim.Adam (or AdamW) + ExponentialLR over CPU stand-ins of the 44 parameters (coarse then
         fine, state-dict order: NeRFTrainer's `list(coarse.parameters()) + list(fine...)`,
         trainer.py:54-64) holding this trainer's state, for state_dict() in torch's format."""
         import torch
@@ -383,7 +399,8 @@ class MI355XTrainer:
         c = self.config
         params = [torch.nn.Parameter(torch.from_numpy(v.copy()))
                   for sd in self.state_dicts() for v in sd.values()]
-        opt = torch.optim.Adam(params, lr=float(c["lr"]), weight_decay=float(c["weight_decay"]))
+        kind = torch.optim.AdamW if self.optimizer == "adamw" else torch.optim.Adam
+        opt = kind(params, lr=float(c["lr"]), weight_decay=float(c["weight_decay"]))
         sched = torch.optim.lr_scheduler.ExponentialLR(opt, gamma=self._cfg.lr_gamma)
         steps = self.steps
         if steps > 0:

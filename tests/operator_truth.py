@@ -1,0 +1,122 @@
+"""The block operators' formulas in 64 bits on the CPU, with bounds on what rounding may do to them.
+
+``half(t)``: the relative error of one rounding to t.  A sum of K products formed in fp32 in any order is
+within (K + 2) 2^-24 of its absolute sum (each product and each addition rounds once).  Products of fp32
+operands may be formed from two 16-bit halves each (22 bits or more of every operand: 2^-22 per operand,
+2^-22 for the product of the low halves): 2^-20 covers them.
+"""
+import math
+
+import torch
+
+BOUND_FN = 4e-7        # exp, erfc and the arithmetic around them in fp32, relative to the result's scale
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """Half a step of the type's subnormal numbers."""
+    return {torch.float16: 2.0 ** -25}.get(dtype, 0.0)
+
+
+def rotary(x, positions, sections, frequencies, interleaved, inverse):
+    """x [..., tokens, heads, dim] with positions [..., tokens, axes]: (turned in 64 bits, error bound)."""
+    f = x.double()
+    axis = torch.tensor([a for a, k in enumerate(sections) for _ in range(k)], dtype=torch.long)
+    angle = positions.double()[..., axis] * torch.tensor(frequencies, dtype=torch.float64)
+    angle = (-angle if inverse else angle).unsqueeze(-2)
+    r = len(axis)
+    first, second = (slice(0, 2 * r, 2), slice(1, 2 * r, 2)) if interleaved else (slice(0, r), slice(r, 2 * r))
+    u, v = f[..., first], f[..., second]
+    out, size = f.clone(), torch.zeros_like(f)
+    out[..., first] = u * angle.cos() - v * angle.sin()
+    out[..., second] = u * angle.sin() + v * angle.cos()
+    size[..., first] = size[..., second] = u.abs() + v.abs()
+    # sine and cosine to 1.5e-7, two products and a sum in fp32: 2^-24 each; then the type's rounding
+    return out, 4e-7 * size + half(x.dtype) * out.abs() * 1.001 + tiny(x.dtype)
+
+
+def ladder(sections, base=10000.0, shared=False):
+    got = []
+    for s in sections:
+        got += [base ** (-(len(got) + j) / sum(sections) if shared else -j / s) for j in range(s)]
+    return got
+
+
+def act(g, kind):
+    """(act, act', bound of |act''|; None: a step at 0)."""
+    if kind == "relu":
+        return g.clamp(min=0), (g > 0).double(), None
+    if kind == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s)), 0.5
+    c = 0.5 * torch.erfc(-g / math.sqrt(2.0))
+    return g * c, c + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi), 0.8
+
+
+def block(x, wg, wu, wd, kind, dy=None):
+    """{name: (value in 64 bits, error bound)} for y and, with dy, dx, dw_gate, dw_up, dw_down."""
+    t = x.dtype
+    low = half(t) if t != torch.float32 else 0.0       # intermediates rounded to a 16-bit type
+    floor = tiny(t)
+    split = 2.0 ** -20 if t == torch.float32 else 0.0
+    x, wg, wu, wd = (v.double() for v in (x, wg, wu, wd))
+
+    def gamma(k):
+        return (k + 2) * 2.0 ** -24 + split
+
+    def product(a, da, b, db):
+        """a b (a [m, k], b [k, n]) with errors da, db of the operands: value and bound before rounding."""
+        k = a.shape[1]
+        return a @ b, da @ b.abs() + a.abs() @ db + da @ db + gamma(k) * (a.abs() + da) @ (b.abs() + db)
+
+    zero = torch.zeros_like
+    g, eg = product(x, zero(x), wg.t(), zero(wg.t()))
+    u, eu = product(x, zero(x), wu.t(), zero(wu.t()))
+    a, s, curve = act(g, kind)
+    ea = 1.13 * eg + BOUND_FN * a.abs() + 2.0 ** -24 * BOUND_FN
+    h = a * u
+    eh = ea * u.abs() + a.abs() * eu + ea * eu
+    eh = eh + (h.abs() + eh) * (2.0 ** -23 + low) + floor
+    y, ey = product(h, eh, wd.t(), zero(wd.t()))
+    last = lambda v, e: (v, e + half(t) * (v.abs() + e) + tiny(t) + 1e-30)  # noqa: E731
+    got = {"y": last(y, ey)}
+    if dy is None:
+        return got
+    dy = dy.double()
+    d, ed = product(dy, zero(dy), wd, zero(wd))
+    es = (g.abs() <= eg).double() if curve is None else curve * eg + BOUND_FN
+    du = d * a
+    edu = ed * a.abs() + d.abs() * ea + ed * ea
+    edu = edu + (du.abs() + edu) * (2.0 ** -23 + low) + floor
+    dg = d * u * s
+    edg = (d.abs() + ed) * (u.abs() + eu) * (s.abs() + es) - d.abs() * u.abs() * s.abs()
+    edg = edg + (dg.abs() + edg) * (2.0 ** -22 + low) + floor
+    p, ep = product(dg, edg, wg, zero(wg))
+    q, eq = product(du, edu, wu, zero(wu))
+    # one accumulator over both products
+    got["dx"] = last(p + q, ep + eq + gamma(2 * wg.shape[0]) * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()))
+    got["dw_gate"] = last(*product(dg.t(), edg.t(), x, zero(x)))
+    got["dw_up"] = last(*product(du.t(), edu.t(), x, zero(x)))
+    got["dw_down"] = last(*product(dy.t(), zero(dy.t()), h, eh))
+    return got
+
+
+def adamw(p, g, m, v, t, lr, b1, b2, eps, decay, factor=1.0):
+    """(p, m, v) after step t in 64 bits."""
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    g = g * factor
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    return p - lr * (decay * p + (m / (1 - b1 ** t)) / ((v / (1 - b2 ** t)).sqrt() + eps)), m, v
+
+
+def within(got, want, bound, what):
+    got, want, bound = got.detach().double().cpu(), want.detach().cpu(), bound.detach().cpu()
+    assert got.shape == want.shape, what
+    off = (got - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside; worst {float(off[bad].max()):.3g} where "
+                           f"{float(bound[bad][off[bad].argmax()]):.3g} is allowed, at {bad.nonzero()[0].tolist()}")
