@@ -170,7 +170,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs a) {
   const float factor = a.clip ? a.ctl->factor : 1.0f;
   const bool skip = (a.flags & NERF_ADAMW_SKIP_NONFINITE) && !__builtin_isfinite(a.ctl->norm);
   if (!skip) {
-    const float lr = a.lr_dev ? *a.lr_dev : a.lr;
+    float lr = a.lr;
+    // (a global load: a plain one would be merged with the argument's into one through a flat address)
+    if (a.lr_dev) lr = *(const __attribute__((address_space(1))) float*)a.lr_dev;
     const float decay = a.lr_dev ? 1.0f - lr * t.wd : t.decay;
     const float rate = float(double(lr) / (1.0 - pow_steps(a.b1d, step)));
     const float root = float(sqrt(1.0 - pow_steps(a.b2d, step)));

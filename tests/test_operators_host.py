@@ -218,6 +218,22 @@ def test_block_c_refuses_outputs_and_workspaces():
     assert f(ref, None, 5, None, 0, None) == 0
 
 
+def test_block_workspaces_of_all_types_and_sizes():
+    lib, d = rt.load_library(), _block_desc()
+    for dtype in (rt.NERF_F32, rt.NERF_BFLOAT16, rt.NERF_FLOAT16):
+        for rows in (0, 1, 16, 17, 300, 1 << 20):
+            for width, hidden, out in ((1, 1, 1), (64, 128, 64), (1000, 2730, 1001), (4096, 10240, 4096)):
+                d.dtype, d.rows, d.width, d.hidden, d.out = dtype, rows, width, hidden, out
+                d.ld_x = d.ld_gate = d.ld_up = width
+                d.ld_down = hidden
+                for back in (0, 1):
+                    need = lib.nerf_gated_block_workspace(ctypes.byref(d), back)
+                    assert rows == 0 or need > 0 or not back
+                    # h, dg and du of every row, padded copies and partials: bounded by the operands' own sizes
+                    values = rows * (3 * hidden + width + out + 64) + 8 * (hidden + 64) * (width + out + 64)
+                    assert need <= 16 * values + (256 << 20)
+
+
 # -------------------------------------------------------------------------------------------- adamw --
 @pytest.mark.parametrize("k, words", [
     (dict(params=[]), "no parameters"),
