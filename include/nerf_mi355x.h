@@ -467,11 +467,12 @@ int nerf_gated_block_backward(const nerf_block_desc* desc, const void* dy, int64
 #define NERF_ADAMW_WRITE_GRADS 2
 typedef struct nerf_adamw_control {
   int32_t steps;
-  uint32_t ticket; /* internal, zero between calls */
+  int32_t apply;     /* 0: the last call left everything as it was */
   int32_t skipped;
   float norm;
-  float factor;    /* what the gradients were multiplied by */
-  int32_t reserved[3];
+  float factor;      /* what the gradients were multiplied by */
+  float rate, root;  /* 1 / (1 - beta1^t), sqrt(1 - beta2^t) of the last step */
+  int32_t reserved;
 } nerf_adamw_control;
 typedef struct nerf_adamw_tensor {
   float* param;

@@ -29,13 +29,11 @@ struct AdamTensor {
 struct AdamArgs {
   AdamTensor t[kTensors];
   unsigned first[kTensors];   // the tensor's first chunk in this launch
-  int n_tensors, iters, flags, last;
+  int n_tensors, iters, flags;
   unsigned char wide[kTensors];   // every address allows vector access
-  nerf_adamw_control* ctl;
+  const nerf_adamw_control* ctl;
   const float* lr_dev;
-  float lr, b1, b2, eps;
-  double b1d, b2d;
-  int clip;
+  float lr, b1c, b2, b2c, eps;   // b1c = 1 - beta1, b2c = 1 - beta2
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 constexpr int kStep = 1024;    // values a workgroup takes per iteration: 256 threads x 4
@@ -109,24 +107,9 @@ __device__ __forceinline__ double pow_steps(double b, int t) {   // b^t, t > 0, 
   return r;
 }
 
-// True in the one workgroup of the launch that comes last; everything the others wrote before is
-// visible to it.  The ticket is zero again afterwards.
-__device__ __forceinline__ bool last_group(nerf_adamw_control* ctl) {
-  __shared__ bool is_last;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const unsigned t = __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    is_last = t == gridDim.x - 1;
-    if (is_last) __hip_atomic_store(&ctl->ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  return is_last;
-}
-
-// The gradients' squares summed in fp64, one partial per workgroup at a fixed place; the last
-// workgroup of the last launch adds the partials in order, so the norm does not depend on timing.
+// The gradients' squares summed in fp64, one partial per workgroup at a fixed place.
 template <typename G>
-__global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part, long done, float max_norm) {
+__global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part) {
   __shared__ double red[4];
   const int k = find(a, blockIdx.x);
   const AdamTensor& t = a.t[k];
@@ -138,27 +121,42 @@ __global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part, lon
 #pragma unroll
     for (int j = 0; j < 4; ++j) s += double(g[j]) * double(g[j]);
   }
-  auto sum = [&](double x) {   // of the workgroup, in thread 0
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_down(x, o, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-  };
-  s = sum(s);
-  if (threadIdx.x == 0) __hip_atomic_store(part + done + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!last_group(a.ctl) || !a.last) return;
-  __threadfence();
-  double all = 0.0;
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_down(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// One workgroup: the norm from the partials, added in order (it does not depend on timing), the step
+// count and the step's scalars for adamw_kernel.  A launch of its own: a count of finished workgroups in
+// the kernels before (one atomic each on one address, ~0.1 us apiece) cost 3.5 ms where there were 35,000.
+__global__ __launch_bounds__(1024) void prepare_kernel(nerf_adamw_control* c, const double* part, long n, float max_norm, double b1,
+                                                       double b2, int skip_nonfinite) {
+  __shared__ double red[16];
+  double s = 0.0;
 #pragma unroll 8
-  for (long j = threadIdx.x; j < done + gridDim.x; j += 256) all += part[j];
-  all = sum(all);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(all), f = max_norm > 0.0f ? double(max_norm) / (norm + 1e-6) : 1.0;
-    a.ctl->norm = float(norm);
-    a.ctl->factor = f > 1.0 ? 1.0f : float(f);   // NaN stays NaN
+  for (long j = threadIdx.x; j < n; j += 1024) s += part[j];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_down(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.0;
+  for (int w = 0; w < 16; ++w) s += red[w];
+  const double norm = sqrt(s), f = max_norm > 0.0f ? double(max_norm) / (norm + 1e-6) : 1.0;
+  if (n) c->norm = float(norm);
+  c->factor = f > 1.0 ? 1.0f : float(f);   // NaN stays NaN
+  const bool skip = skip_nonfinite && !__builtin_isfinite(float(norm));
+  c->apply = skip ? 0 : 1;
+  if (skip) {
+    c->skipped += 1;
+    return;
   }
+  const int step = c->steps + 1;
+  c->steps = step;
+  c->rate = float(1.0 / (1.0 - pow_steps(b1, step)));
+  c->root = float(sqrt(1.0 - pow_steps(b2, step)));
 }
 
 template <typename G, typename M, int BITS>
@@ -166,81 +164,72 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs a) {
   const int k = find(a, blockIdx.x);
   const AdamTensor& t = a.t[k];
   const bool wide = a.wide[k];
-  const int step = a.ctl->steps + 1;
-  const float factor = a.clip ? a.ctl->factor : 1.0f;
-  const bool skip = (a.flags & NERF_ADAMW_SKIP_NONFINITE) && !__builtin_isfinite(a.ctl->norm);
-  if (!skip) {
-    float lr = a.lr;
-    // (a global load: a plain one would be merged with the argument's into one through a flat address)
-    if (a.lr_dev) lr = *(const __attribute__((address_space(1))) float*)a.lr_dev;
-    const float decay = a.lr_dev ? 1.0f - lr * t.wd : t.decay;
-    const float rate = float(double(lr) / (1.0 - pow_steps(a.b1d, step)));
-    const float root = float(sqrt(1.0 - pow_steps(a.b2d, step)));
-    const float b1c = float(1.0 - a.b1d), b2c = float(1.0 - a.b2d);
-    long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
-    for (int it = 0; it < a.iters; ++it, i += kStep) {
-      if (BITS == 32 && i >= t.n) break;
-      if (BITS == 8 && i - (threadIdx.x & 63) * 4 >= t.n) break;   // uniform in a wave: its block is behind the end
-      float g[4], p[4], m[4], v[4], r[4];
-      load4(static_cast<const G*>(t.g), i, t.n, wide, g);
-      load4(t.p, i, t.n, wide, p);
-      const long block = i >> 8;    // the wave's 256 values are one block
-      if (BITS == 32) {
-        load4(static_cast<const float*>(t.m), i, t.n, wide, m);
-        load4(static_cast<const float*>(t.v), i, t.n, wide, v);
-      } else {
-        load_codes(static_cast<const unsigned char*>(t.m), i, t.n, wide, m);
-        load_codes(static_cast<const unsigned char*>(t.v), i, t.n, wide, v);
-        const float ms = t.ms[block], vs = t.vs[block];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          m[j] *= ms;
-          v[j] *= vs;
-          v[j] *= v[j];
-        }
-      }
+  if (!a.ctl->apply) return;
+  const float factor = a.ctl->factor, root = a.ctl->root;
+  float lr = a.lr;
+  // (a global load: a plain one would be merged with the argument's into one through a flat address)
+  if (a.lr_dev) lr = *(const __attribute__((address_space(1))) float*)a.lr_dev;
+  const float decay = a.lr_dev ? 1.0f - lr * t.wd : t.decay, rate = lr * a.ctl->rate;
+  long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
+  for (int it = 0; it < a.iters; ++it, i += kStep) {
+    if (BITS == 32 && i >= t.n) break;
+    if (BITS == 8 && i - (threadIdx.x & 63) * 4 >= t.n) break;   // uniform in a wave: its block is behind the end
+    float g[4], p[4], m[4], v[4], r[4];
+    load4(static_cast<const G*>(t.g), i, t.n, wide, g);
+    load4(t.p, i, t.n, wide, p);
+    const long block = i >> 8;    // the wave's 256 values are one block
+    if (BITS == 32) {
+      load4(static_cast<const float*>(t.m), i, t.n, wide, m);
+      load4(static_cast<const float*>(t.v), i, t.n, wide, v);
+    } else {
+      load_codes(static_cast<const unsigned char*>(t.m), i, t.n, wide, m);
+      load_codes(static_cast<const unsigned char*>(t.v), i, t.n, wide, v);
+      const float ms = t.ms[block], vs = t.vs[block];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        g[j] *= factor;
-        m[j] += (g[j] - m[j]) * b1c;
-        v[j] = v[j] * a.b2 + g[j] * g[j] * b2c;
-        r[j] = sqrtf(v[j]);
-        p[j] = p[j] * decay - rate * m[j] / (r[j] / root + a.eps);
-      }
-      if (a.flags & NERF_ADAMW_WRITE_GRADS) store4(static_cast<G*>(t.g), i, t.n, wide, g);
-      store4(t.p, i, t.n, wide, p);
-      if (sizeof(M) == 2) store4(static_cast<M*>(t.model), i, t.n, wide, p);
-      if (BITS == 32) {
-        store4(static_cast<float*>(t.m), i, t.n, wide, m);
-        store4(static_cast<float*>(t.v), i, t.n, wide, v);
-      } else {
-        // values behind the tensor's end were loaded as zeros: they do not raise the block's maximum
-        const float top = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
-        const float rtop = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
-        const float ms = top / 448.0f, vs = rtop / 448.0f;
-        unsigned mw = 0, vw = 0;
-        if (ms > 0.0f) {
-          mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] / ms, m[1] / ms, mw, false);
-          mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] / ms, m[3] / ms, mw, true);
-        }
-        if (vs > 0.0f) {
-          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[0] / vs, r[1] / vs, vw, false);
-          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[2] / vs, r[3] / vs, vw, true);
-          // a root that is not zero keeps the smallest code: m / (0 + eps) of a value whose v was
-          // rounded away would be a step of any size
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (r[j] > 0.0f && ((vw >> (8 * j)) & 0xffu) == 0) vw |= 1u << (8 * j);
-        }
-        store_codes(static_cast<unsigned char*>(t.m), i, t.n, wide, mw);
-        store_codes(static_cast<unsigned char*>(t.v), i, t.n, wide, vw);
-        if ((threadIdx.x & 63) == 0) t.ms[block] = ms, t.vs[block] = vs;
+        m[j] *= ms;
+        v[j] *= vs;
+        v[j] *= v[j];
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      g[j] *= factor;
+      m[j] += (g[j] - m[j]) * a.b1c;
+      v[j] = v[j] * a.b2 + g[j] * g[j] * a.b2c;
+      r[j] = sqrtf(v[j]);
+      p[j] = p[j] * decay - rate * m[j] / (r[j] / root + a.eps);
+    }
+    if (a.flags & NERF_ADAMW_WRITE_GRADS) store4(static_cast<G*>(t.g), i, t.n, wide, g);
+    store4(t.p, i, t.n, wide, p);
+    if (sizeof(M) == 2) store4(static_cast<M*>(t.model), i, t.n, wide, p);
+    if (BITS == 32) {
+      store4(static_cast<float*>(t.m), i, t.n, wide, m);
+      store4(static_cast<float*>(t.v), i, t.n, wide, v);
+    } else {
+      // values behind the tensor's end were loaded as zeros: they do not raise the block's maximum
+      const float top = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+      const float rtop = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+      const float ms = top / 448.0f, vs = rtop / 448.0f;
+      unsigned mw = 0, vw = 0;
+      if (ms > 0.0f) {
+        mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] / ms, m[1] / ms, mw, false);
+        mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] / ms, m[3] / ms, mw, true);
+      }
+      if (vs > 0.0f) {
+        vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[0] / vs, r[1] / vs, vw, false);
+        vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[2] / vs, r[3] / vs, vw, true);
+        // a root that is not zero keeps the smallest code: m / (0 + eps) of a value whose v was
+        // rounded away would be a step of any size
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r[j] > 0.0f && ((vw >> (8 * j)) & 0xffu) == 0) vw |= 1u << (8 * j);
+      }
+      store_codes(static_cast<unsigned char*>(t.m), i, t.n, wide, mw);
+      store_codes(static_cast<unsigned char*>(t.v), i, t.n, wide, vw);
+      if ((threadIdx.x & 63) == 0) t.ms[block] = ms, t.vs[block] = vs;
+    }
   }
-  if (!last_group(a.ctl) || !a.last || threadIdx.x) return;   // every workgroup has read steps
-  if (skip) a.ctl->skipped += 1;
-  else a.ctl->steps = step;
 }
 
 // Chunks of a call: as many as fill the machine with one iteration each, at most 8 iterations (32 KiB
@@ -321,36 +310,44 @@ int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_a
                      nerf_adamw_workspace(n_tensors, tensors));
   const hipStream_t s = (hipStream_t)stream;
   const int iters = iterations(n_tensors, tensors);
+  double* part = static_cast<double*>(workspace);
   // launches of up to kTensors tensors of the same types, in order; pass 0 sums squares, pass 1 steps
   for (int pass = norm ? 0 : 1; pass < 2; ++pass) {
     AdamArgs a;
     std::memset(&a, 0, sizeof a);
-    long done = 0;
     int grad = -1, model = -1;
     unsigned grid = 0;
-    auto flush = [&](int last) -> int {
+    long done = 0;      // partials of the launches before
+    auto launched = [&]() -> int {
+      const hipError_t e = hipGetLastError();
+      return e == hipSuccess ? NERF_OK : set_error(NERF_E_HIP, "nerf_adamw_step: %s", hipGetErrorString(e));
+    };
+    auto flush = [&]() -> int {
       if (a.n_tensors == 0) return NERF_OK;
-      a.last = last;
       if (pass == 0) {
-        const float mx = float(config->max_norm);
-        double* part = static_cast<double*>(workspace);
-        if (grad == NERF_F32) hipLaunchKernelGGL((norm_kernel<float>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
-        else if (grad == NERF_BFLOAT16) hipLaunchKernelGGL((norm_kernel<__bf16>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
-        else hipLaunchKernelGGL((norm_kernel<_Float16>), dim3(grid), dim3(256), 0, s, a, part, done, mx);
+        if (grad == NERF_F32) hipLaunchKernelGGL((norm_kernel<float>), dim3(grid), dim3(256), 0, s, a, part + done);
+        else if (grad == NERF_BFLOAT16) hipLaunchKernelGGL((norm_kernel<__bf16>), dim3(grid), dim3(256), 0, s, a, part + done);
+        else hipLaunchKernelGGL((norm_kernel<_Float16>), dim3(grid), dim3(256), 0, s, a, part + done);
       } else {
         if (grad == NERF_F32) launch_step<float>(a, model, config->state_bits, grid, s);
         else if (grad == NERF_BFLOAT16) launch_step<__bf16>(a, model, config->state_bits, grid, s);
         else launch_step<_Float16>(a, model, config->state_bits, grid, s);
       }
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return set_error(NERF_E_HIP, "nerf_adamw_step: %s", hipGetErrorString(e));
       done += grid;
       a.n_tensors = 0, grid = 0;
-      return NERF_OK;
+      return launched();
     };
-    a.iters = iters, a.flags = config->flags, a.ctl = control, a.lr_dev = config->lr_device, a.clip = clip;
-    a.lr = float(config->lr), a.b1 = float(config->beta1), a.b2 = float(config->beta2), a.eps = float(config->eps);
-    a.b1d = config->beta1, a.b2d = config->beta2;
+    if (pass == 1) {
+      long n = 0;
+      if (norm)
+        for (int i = 0; i < n_tensors; ++i) n += chunks(tensors[i], iters);
+      hipLaunchKernelGGL(prepare_kernel, dim3(1), dim3(1024), 0, s, control, (const double*)part, n, float(clip ? config->max_norm : 0.0),
+                         config->beta1, config->beta2, config->flags & NERF_ADAMW_SKIP_NONFINITE);
+      if ((rc = launched()) != NERF_OK) return rc;
+    }
+    a.iters = iters, a.flags = config->flags, a.ctl = control, a.lr_dev = config->lr_device;
+    a.lr = float(config->lr), a.b1c = float(1.0 - config->beta1), a.b2 = float(config->beta2), a.b2c = float(1.0 - config->beta2);
+    a.eps = float(config->eps);
     for (int i = 0; i < n_tensors; ++i) {
       const nerf_adamw_tensor& x = tensors[i];
       if (x.numel == 0) continue;
@@ -358,7 +355,7 @@ int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_a
       const long c = chunks(x, iters);
       if (c > 0x40000000L) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d is too large", i);
       if (a.n_tensors == kTensors || x.grad_dtype != grad || md != model || grid + c > 0x7fffffffL)
-        if ((rc = flush(0)) != NERF_OK) return rc;
+        if ((rc = flush()) != NERF_OK) return rc;
       grad = x.grad_dtype, model = md;
       const int k = a.n_tensors++;
       a.t[k] = AdamTensor{x.param, x.model, x.grad, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, long(x.numel),
@@ -369,7 +366,7 @@ int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_a
                   !((uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq)) & (config->state_bits == 32 ? 15 : 3));
       grid += unsigned(c);
     }
-    if ((rc = flush(1)) != NERF_OK) return rc;
+    if ((rc = flush()) != NERF_OK) return rc;
   }
   return NERF_OK;
 }

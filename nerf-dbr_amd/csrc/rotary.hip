@@ -60,9 +60,10 @@ __device__ __forceinline__ void turn(double angle, float& c, float& s) {
   c = ((k + 1) & 2) ? -b : b;
 }
 
-// A thread owns V pairs of one token in split form (two vectors of V values per head) and V / 2 pairs
-// in interleaved form (one vector), or V values behind the last pair, and runs over the heads
-// [blockIdx.y * per, + per) of both tensors.
+// A thread owns V pairs of one token in split form (two vectors of V values per head) or V values behind
+// the last pair; in interleaved form one vector of V values, pairs and values behind them alike (a tail
+// that is no whole vector then costs no narrower access: 131072 x 8 heads x 32 values, 15 pairs, fp32).
+// It runs over the heads [blockIdx.y * per, + per) of both tensors.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int per) {
   const long item = long(blockIdx.x) * 256 + threadIdx.x;
@@ -104,6 +105,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int per) {
         Vec<T, V> w = *reinterpret_cast<const Vec<T, V>*>(xh + e);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
+          if (g * P + i >= a.pairs) continue;      // as they are, whatever they hold
           const float u = float(w.v[2 * i]), v = float(w.v[2 * i + 1]);
           w.v[2 * i] = T(u * c[i] - v * s[i]);
           w.v[2 * i + 1] = T(u * s[i] + v * c[i]);
@@ -208,11 +210,11 @@ extern "C" int nerf_rotary_axes(const nerf_rotary_desc* d, void* stream) {
   // values per access: 16 bytes where addresses, halves and tail allow it, else 2 values, else 1
   const int tail = d->head_dim - 2 * a.pairs;
   auto fits = [&](int v) {
-    return align >= v * size && tail % v == 0 && (a.interleaved ? (2 * a.pairs) % v == 0 : a.pairs % v == 0);
+    return align >= v * size && (a.interleaved ? d->head_dim % v == 0 : tail % v == 0 && a.pairs % v == 0);
   };
   const int v = fits(int(16 / size)) ? int(16 / size) : fits(2) ? 2 : 1;
-  a.rot_groups = a.interleaved && v > 1 ? 2 * a.pairs / v : a.pairs / v;
-  a.groups = a.rot_groups + tail / v;
+  a.rot_groups = a.interleaved && v > 1 ? d->head_dim / v : a.pairs / v;
+  a.groups = a.interleaved && v > 1 ? a.rot_groups : a.rot_groups + tail / v;
   const double items = double(d->n_batch) * double(d->n_tokens) * a.groups;
   if (items > 5.0e11) return set_error(NERF_E_INVALID, "nerf_rotary_axes: too many tokens");
   a.items = long(d->n_batch) * a.n_tokens * a.groups;

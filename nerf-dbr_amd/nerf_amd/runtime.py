@@ -146,8 +146,8 @@ class BlockDesc(_c.Structure):
 
 class AdamWControl(_c.Structure):
     """nerf_adamw_control."""
-    _fields_ = [("steps", _c.c_int32), ("ticket", _c.c_uint32), ("skipped", _c.c_int32), ("norm", _c.c_float),
-                ("factor", _c.c_float), ("reserved", _c.c_int32 * 3)]
+    _fields_ = [("steps", _c.c_int32), ("apply", _c.c_int32), ("skipped", _c.c_int32), ("norm", _c.c_float),
+                ("factor", _c.c_float), ("rate", _c.c_float), ("root", _c.c_float), ("reserved", _c.c_int32)]
 
 
 class AdamWTensor(_c.Structure):
