@@ -28,98 +28,35 @@ __device__ __forceinline__ void activate(int kind, float g, float& a, float& d) 
   }
 }
 
-// An operand: element (i, k) at p[i * si + k * sk], i the row or column of the product, k summed over.
-struct Operand {
-  const void* p;
-  long si, sk;
-};
-
-constexpr int kT = 64, kK = 16;
-
-// One 64 x 64 tile of sum over k of A(i, k) B(j, k) into acc, 4 x 4 values a thread; staged in LDS as fp32.
-template <typename T>
-__device__ __forceinline__ void tile_product(const Operand& a, const Operand& b, long i0, long j0, long m, long n, long k,
-                                             float (*as)[kT + 1], float (*bs)[kT + 1], float acc[4][4]) {
-  const int t = threadIdx.x, ti = t >> 4, tj = t & 15;
-  const T* ap = static_cast<const T*>(a.p);
-  const T* bp = static_cast<const T*>(b.p);
-  for (long k0 = 0; k0 < k; k0 += kK) {
-    __syncthreads();
-    for (int e = t; e < kT * kK; e += 256) {
-      // neighbouring threads along the operand's contiguous direction
-      const int ai = a.sk == 1 ? e / kK : e % kT, ak = a.sk == 1 ? e % kK : e / kT;
-      const int bi = b.sk == 1 ? e / kK : e % kT, bk = b.sk == 1 ? e % kK : e / kT;
-      as[ak][ai] = i0 + ai < m && k0 + ak < k ? float(ap[(i0 + ai) * a.si + (k0 + ak) * a.sk]) : 0.0f;
-      bs[bk][bi] = j0 + bi < n && k0 + bk < k ? float(bp[(j0 + bi) * b.si + (k0 + bk) * b.sk]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kK; ++q)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(as[q][ti + 16 * r], bs[q][tj + 16 * c], acc[r][c]);
-  }
-}
-
-// C (m x n, row stride ldc) = A1 B1 (+ A2 B2)
-template <typename T>
-__global__ __launch_bounds__(256) void product_kernel(Operand a1, Operand b1, Operand a2, Operand b2, long m, long n, long k, T* c,
-                                                      long ldc) {
-  __shared__ float as[kK][kT + 1], bs[kK][kT + 1];
-  const long across = (n + kT - 1) / kT, i0 = blockIdx.x / across * kT, j0 = blockIdx.x % across * kT;
-  float acc[4][4] = {};
-  tile_product<T>(a1, b1, i0, j0, m, n, k, as, bs, acc);
-  if (a2.p) tile_product<T>(a2, b2, i0, j0, m, n, k, as, bs, acc);
-  for (int r = 0; r < 4; ++r)
-    for (int q = 0; q < 4; ++q) {
-      const long i = i0 + (threadIdx.x >> 4) + 16 * r, j = j0 + (threadIdx.x & 15) + 16 * q;
-      if (i < m && j < n) c[i * ldc + j] = T(acc[r][q]);
-    }
-}
-
-// h = act(x Wg^T) (x Wu^T); with dy also dg and du
-template <typename T, bool BACK>
-__global__ __launch_bounds__(256) void gate_kernel(Operand x, Operand wg, Operand wu, Operand dy, Operand wd, long rows, long hidden,
-                                                   long width, long out, int kind, T* h, T* dg, T* du) {
-  __shared__ float as[kK][kT + 1], bs[kK][kT + 1];
-  const long across = (hidden + kT - 1) / kT, i0 = blockIdx.x / across * kT, j0 = blockIdx.x % across * kT;
-  float g[4][4] = {}, u[4][4] = {}, d[4][4] = {};
-  tile_product<T>(x, wg, i0, j0, rows, hidden, width, as, bs, g);
-  tile_product<T>(x, wu, i0, j0, rows, hidden, width, as, bs, u);
-  if (BACK) tile_product<T>(dy, wd, i0, j0, rows, hidden, out, as, bs, d);
-  for (int r = 0; r < 4; ++r)
-    for (int q = 0; q < 4; ++q) {
-      const long i = i0 + (threadIdx.x >> 4) + 16 * r, j = j0 + (threadIdx.x & 15) + 16 * q;
-      if (i >= rows || j >= hidden) continue;
-      float a, s;
-      activate(kind, g[r][q], a, s);
-      h[i * hidden + j] = T(a * u[r][q]);
-      if (BACK) {
-        dg[i * hidden + j] = T(d[r][q] * u[r][q] * s);
-        du[i * hidden + j] = T(d[r][q] * a);
-      }
-    }
-}
-
 // ------------------------------------------------------------------ 16-bit types on the matrix cores --
 // The 256 x 256 tile of 8 waves carries long products; the 128 x 128 tile of 4 waves (two workgroups a CU)
 // fills the machine where there are few tiles.
 typedef Tile<2, 4, 8, 4> Large;
 typedef Tile<2, 2, 4, 4> Small;
 
+// 32-bit operands run on the f16 matrix cores as two halves each, x 2^e = hi + lo with e from the largest
+// value of the operand's row (or column, where the sum runs over rows), so that hi lies in [2^-14, 2^15] and
+// lo's rounding is 2^-25 of 2^15: x b ~ hi bh + hi bl + lo bh, 22 bits of every operand at a third of the
+// 16-bit rate.  The f32 matrix instruction carries 24 bits at a sixteenth.  The tables hold the largest
+// values' bits, index by row or column.
+struct Scales {
+  const unsigned *x, *wg, *wu, *dy, *wd;
+};
+__device__ __forceinline__ int exponent(unsigned top) { return 141 - max(int(top >> 23), 1); }
+
 // h = act(x Wg^T) (x Wu^T): the J tile holds TJ / 2 rows of Wg and the same rows of Wu, so a lane owns the
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
-template <typename T, typename C>
-__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int kind, T* h, long ld_h, long rows,
-                                                                      long hidden, unsigned tiles_i, unsigned tiles_j) {
+template <typename T, typename C, typename O>
+__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
+                                                            long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
+  constexpr bool kScaled = sizeof(O) == 4;
   __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
   unsigned ti, tj;
   tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * (C::TJ / 2);
   f32x4_t acc[C::NJ][C::NI] = {};
-  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps, lds_addr(lds));
+  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   const long ib = i0 + (wave / C::WJ) * C::NI * 16 + (l & 15), jb = j0 + (wave % C::WJ) * (C::NJ / 2) * 16 + (l >> 4) * 4;
 #pragma unroll
@@ -131,9 +68,15 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
       f32x4_t o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float a, d;
-        activate(kind, acc[j][i][r], a, d);
-        o[r] = col + r < hidden ? a * acc[j + C::NJ / 2][i][r] : 0.0f;
+        float a, d, g = acc[j][i][r], u = acc[j + C::NJ / 2][i][r];
+        const bool in = col + r < hidden;
+        if (kScaled && in) {
+          const int e = exponent(sc.x[row]);
+          g = ldexpf(g, -e - exponent(sc.wg[col + r]));
+          u = ldexpf(u, -e - exponent(sc.wu[col + r]));
+        }
+        activate(kind, g, a, d);
+        o[r] = in ? a * u : 0.0f;
       }
       store_row4(h + row * ld_h, col, ld_h, true, o);
     }
@@ -141,18 +84,19 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
 // and h, dg and du of the tile from the three.
-template <typename T, typename C>
-__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy,
-                                                                           int kind, T* h, T* dg, T* du, long ld_h, long rows,
-                                                                           long hidden, unsigned tiles_i, unsigned tiles_j) {
+template <typename T, typename C, typename O>
+__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
+                                                                 int kind, O* h, O* dg, O* du, long ld_h, long rows, long hidden,
+                                                                 unsigned tiles_i, unsigned tiles_j, Scales sc) {
+  constexpr bool kScaled = sizeof(O) == 4;
   typedef Tile<C::WI, C::WJ, C::NI, C::NJ / 2> Half;
   __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
   unsigned ti, tj;
   tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * Half::TJ;
   f32x4_t acc[C::NJ][C::NI] = {}, dh[Half::NJ][C::NI] = {};
-  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps, lds_addr(lds));
-  accumulate<T, Half, true, false, 1>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy, lds_addr(lds));
+  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
+  accumulate<T, Half, true, false, 1>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy * segs, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   const long ib = i0 + (wave / C::WJ) * C::NI * 16 + (l & 15), jb = j0 + (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
 #pragma unroll
@@ -164,10 +108,15 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
       f32x4_t oh, og, ou;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float a, s;
-        activate(kind, acc[j][i][r], a, s);
-        const float u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
+        float a, s, g = acc[j][i][r], u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
         const bool in = col + r < hidden;
+        if (kScaled && in) {
+          const int e = exponent(sc.x[row]);
+          g = ldexpf(g, -e - exponent(sc.wg[col + r]));
+          u = ldexpf(u, -e - exponent(sc.wu[col + r]));
+          d = ldexpf(d, -exponent(sc.dy[row]) - exponent(sc.wd[col + r]));
+        }
+        activate(kind, g, a, s);
         oh[r] = in ? a * u : 0.0f;
         og[r] = in ? d * u * s : 0.0f;
         ou[r] = in ? d * a : 0.0f;
@@ -192,6 +141,7 @@ struct Problem {
   unsigned splits, tiles_i, tiles_j, first;   // first workgroup
   long part;         // first partial tile of this problem
   int wide;
+  const unsigned *top_i, *top_j;   // 32-bit operands' scales
 };
 struct Problems {
   Problem p[3];
@@ -203,7 +153,14 @@ __device__ __forceinline__ void store_tile(const Problem& p, unsigned ti, unsign
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   const long row = long(ti) * C::TI + ((wave / C::WJ) * C::NI + i) * 16 + (l & 15);
   const long col = long(tj) * C::TJ + ((wave % C::WJ) * C::NJ + j) * 16 + (l >> 4) * 4;
-  if (row < p.m && col < p.n) store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, v);
+  if (row >= p.m || col >= p.n) return;
+  if (sizeof(O) == 4) {
+    const int e = exponent(p.top_i[row]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < p.n) v[r] = ldexpf(v[r], -e - exponent(p.top_j[col + r]));
+  }
+  store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, v);
 }
 template <typename T, typename C, bool IK, bool JK, typename O>
 __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
@@ -257,6 +214,113 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long ld, long ro
   Out4<T>* to = reinterpret_cast<Out4<T>*>(dst + r * ld_dst + c);
   to[0] = o[0];
   to[1] = o[1];
+}
+
+// 32-bit matrices on their way to halves: the largest finite |value| of each row and / or column (bits in
+// zeroed tables; a maximum does not depend on the order of the atomics), then the halves by either.
+struct SplitJob {
+  const float* src;
+  long ld, rows, n, n8;
+  unsigned *row_top, *col_top;     // null: not wanted
+  _Float16 *row_hi, *col_hi;       // [rows][n8]; the lo half follows at + rows * n8
+  unsigned first;                  // first workgroup
+  unsigned across;                 // workgroups along a row
+  int wide;
+};
+struct SplitJobs {
+  SplitJob j[5];
+  int n;
+};
+constexpr int kSplitRows = 64, kSplitCols = 256;   // a workgroup's piece: 4 waves of 16 rows, 4 columns a lane
+
+__device__ __forceinline__ f32x4_t split_load(const SplitJob& p, long row, long col) {
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* at = p.src + row * p.ld + col;
+  if (p.wide && col + 4 <= p.n) return *reinterpret_cast<const f32x4_t*>(at);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (col + r < p.n) v[r] = at[r];
+  return v;
+}
+__device__ __forceinline__ const SplitJob& split_job(const SplitJobs& all) {
+  int k = 0;
+  while (k + 1 < all.n && blockIdx.x >= all.j[k + 1].first) ++k;
+  return all.j[k];
+}
+__global__ __launch_bounds__(256) void fill_kernel(unsigned* p, long n) {
+  const long i = long(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+__global__ __launch_bounds__(256) void split_scan_kernel(SplitJobs all) {
+  const SplitJob& p = split_job(all);
+  const unsigned b = blockIdx.x - p.first;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row0 = long(b / p.across) * kSplitRows + wave * 16, col = long(b % p.across) * kSplitCols + lane * 4;
+  __shared__ unsigned cols[4][kSplitCols];
+  unsigned top[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const long row = row0 + i;
+    unsigned mine = 0;
+    if (row < p.rows) {
+      const f32x4_t v = split_load(p, row, col);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned bits = __float_as_uint(v[r]) & 0x7fffffffu;
+        const unsigned f = bits < 0x7f800000u ? bits : 0u;    // infinities and NaN set no scale
+        top[r] = max(top[r], f);
+        mine = max(mine, f);
+      }
+    }
+    if (p.row_top) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) mine = max(mine, unsigned(__shfl_xor(int(mine), o, 64)));
+      if (lane == 0 && row < p.rows && mine) __hip_atomic_fetch_max(p.row_top + row, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (!p.col_top) return;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) cols[wave][lane * 4 + r] = top[r];
+  __syncthreads();
+  const int c = threadIdx.x;
+  const unsigned m = max(max(cols[0][c], cols[1][c]), max(cols[2][c], cols[3][c]));
+  const long at = long(b % p.across) * kSplitCols + c;
+  if (at < p.n && m) __hip_atomic_fetch_max(p.col_top + at, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void split_store(_Float16* hi, long lo, f32x4_t v, const int e[4]) {
+  Out4<_Float16> h, l;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float x = ldexpf(v[r], e[r]);
+    h.v[r] = _Float16(x);
+    const float d = x - float(h.v[r]);      // exact
+    l.v[r] = _Float16(d == d ? d : 0.0f);   // an infinity is all in hi
+  }
+  *reinterpret_cast<Out4<_Float16>*>(hi) = h;
+  *reinterpret_cast<Out4<_Float16>*>(hi + lo) = l;
+}
+__global__ __launch_bounds__(256) void split_kernel(SplitJobs all) {
+  const SplitJob& p = split_job(all);
+  const unsigned b = blockIdx.x - p.first;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row0 = long(b / p.across) * kSplitRows + wave * 16, col = long(b % p.across) * kSplitCols + lane * 4;
+  if (col >= p.n8) return;
+  int ec[4] = {0, 0, 0, 0};
+  if (p.col_hi)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < p.n) ec[r] = exponent(p.col_top[col + r]);
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const long row = row0 + i;
+    if (row >= p.rows) return;
+    const f32x4_t v = split_load(p, row, col);
+    if (p.row_hi) {
+      const int x = exponent(p.row_top[row]), e[4] = {x, x, x, x};
+      split_store(p.row_hi + row * p.n8 + col, p.rows * p.n8, v, e);
+    }
+    if (p.col_hi) split_store(p.col_hi + row * p.n8 + col, p.rows * p.n8, v, ec);
+  }
 }
 
 // --------------------------------------------------------------------------------------------- host --
@@ -394,6 +458,34 @@ dim3 gate_grid(long rows, long hidden, unsigned& ti, unsigned& tj) {
 }
 int steps_of(long k) { return int((k + 63) / 64); }
 
+template <typename T, typename O>
+void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, int segs, O* h, long hp, const Scales& sc) {
+  if (!r.go || !d.rows) return;
+  unsigned ti, tj;
+  const auto go = [&](auto tile) {
+    typedef decltype(tile) C;
+    const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
+    hipLaunchKernelGGL((gate_mma_kernel<T, C, O>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(d.width), segs, d.activation, h, hp,
+                       long(d.rows), long(d.hidden), ti, tj, sc);
+  };
+  if (use_large(d.rows, 2 * hp)) go(Large{});
+  else go(Small{});
+}
+template <typename T, typename O>
+void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, const Side& dy, const Side& wd, int segs, O* h, O* dg,
+                      O* du, long hp, const Scales& sc) {
+  if (!r.go || !d.rows) return;
+  unsigned ti, tj;
+  const auto go = [&](auto tile) {
+    typedef decltype(tile) C;
+    const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
+    hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(d.width), steps_of(d.out), segs,
+                       d.activation, h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
+  };
+  if (use_large(d.rows, 2 * hp)) go(Large{});
+  else go(Small{});
+}
+
 template <typename T>
 hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const long rows = d.rows, hidden = d.hidden, hp = align_up(hidden, 8);
@@ -401,15 +493,7 @@ hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const Pair w = weights<T>(r, d);
   const Matrix wd = r.matrix<T>(d.w_down, d.ld_down, d.out, hidden);
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  unsigned ti, tj;
-  if (r.go) {
-    if (use_large(rows, 2 * hidden))
-      hipLaunchKernelGGL((gate_mma_kernel<T, Large>), gate_grid<Large>(rows, hp, ti, tj), dim3(Large::NT), 0, r.s, rows_side(x), halves(w),
-                         steps_of(d.width), d.activation, h, hp, rows, hidden, ti, tj);
-    else
-      hipLaunchKernelGGL((gate_mma_kernel<T, Small>), gate_grid<Small>(rows, hp, ti, tj), dim3(Small::NT), 0, r.s, rows_side(x), halves(w),
-                         steps_of(d.width), d.activation, h, hp, rows, hidden, ti, tj);
-  }
+  launch_gate<T, T>(r, d, rows_side(x), halves(w), 1, h, hp, Scales{});
   Problems all{};
   all.n = 1;
   all.p[0] = problem<T>(rows_side(Matrix{h, hp, rows, hidden, hp}), rows_side(wd), rows, d.out, hidden, 1, y, ld_y);
@@ -428,17 +512,7 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* dg = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* du = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  unsigned ti, tj;
-  if (r.go && rows) {
-    if (use_large(rows, 2 * hidden))
-      hipLaunchKernelGGL((gate_back_mma_kernel<T, Large>), gate_grid<Large>(rows, hp, ti, tj), dim3(Large::NT), 0, r.s, rows_side(x),
-                         halves(w), rows_side(dy), columns_side(wd), steps_of(width), steps_of(out), d.activation, h, dg, du, hp, rows,
-                         hidden, ti, tj);
-    else
-      hipLaunchKernelGGL((gate_back_mma_kernel<T, Small>), gate_grid<Small>(rows, hp, ti, tj), dim3(Small::NT), 0, r.s, rows_side(x),
-                         halves(w), rows_side(dy), columns_side(wd), steps_of(width), steps_of(out), d.activation, h, dg, du, hp, rows,
-                         hidden, ti, tj);
-  }
+  launch_gate_back<T, T>(r, d, rows_side(x), halves(w), rows_side(dy), columns_side(wd), 1, h, dg, du, hp, Scales{});
   const Matrix mh{h, hp, rows, hidden, hp}, mg{dg, hp, rows, hidden, hp}, mu{du, hp, rows, hidden, hp};
   if ((dx || !r.go) && rows) {
     Side i = rows_side(mg), j = columns_side(w.g);
@@ -457,37 +531,145 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
   return hipGetLastError();
 }
 
-// ------------------------------------------------------------------------------- 32-bit, plain tiles --
-dim3 tiles(long m, long n) { return dim3(unsigned(((n + kT - 1) / kT) * ((m + kT - 1) / kT))); }
+// ------------------------------------------------------------------------------ 32-bit, in two halves --
+// A matrix's halves and its scales' table.
+struct Halves {
+  Matrix hi, lo;
+  const unsigned* top;
+};
+// Takes tables and halves for the jobs of one pass, and runs scan and split over them.
+struct Splitter {
+  Run& r;
+  SplitJobs all{};
+  unsigned* tops = nullptr;     // tables of this pass, zeroed together
+  long n_tops = 0;
+  explicit Splitter(Run& run) : r(run) {}
 
-template <typename T>
-hipError_t forward(const nerf_block_desc& d, T* y, long ld_y, void* ws, hipStream_t s) {
-  T* h = static_cast<T*>(ws);
-  const Operand x{d.x, d.ld_x, 1}, wg{d.w_gate, d.ld_gate, 1}, wu{d.w_up, d.ld_up, 1}, wd{d.w_down, d.ld_down, 1}, no{};
-  hipLaunchKernelGGL((gate_kernel<T, false>), tiles(d.rows, d.hidden), dim3(256), 0, s, x, wg, wu, no, no, long(d.rows), long(d.hidden),
-                     long(d.width), 0L, d.activation, h, (T*)nullptr, (T*)nullptr);
-  hipLaunchKernelGGL((product_kernel<T>), tiles(d.rows, d.out), dim3(256), 0, s, Operand{h, d.hidden, 1}, wd, no, no, long(d.rows),
-                     long(d.out), long(d.hidden), y, ld_y);
+  unsigned* table(unsigned* base, long n) {
+    unsigned* p = base ? base + n_tops : nullptr;
+    n_tops += align_up(n, 64);
+    return p;
+  }
+  // by: 1 rows, 2 columns, 3 both; the tables' addresses are given (joint scales share one)
+  SplitJob& add(const float* src, long ld, long rows, long n, unsigned* row_top, unsigned* col_top, int by) {
+    SplitJob& j = all.j[all.n++];
+    j.src = src, j.ld = ld, j.rows = rows, j.n = n, j.n8 = align_up(n, 8);
+    j.row_top = row_top, j.col_top = col_top;
+    if (by & 1) j.row_hi = static_cast<_Float16*>(r.a.take(size_t(rows) * j.n8 * 4));
+    if (by & 2) j.col_hi = static_cast<_Float16*>(r.a.take(size_t(rows) * j.n8 * 4));
+    j.wide = !(uintptr_t(src) & 15) && ld % 4 == 0;
+    return j;
+  }
+  void run() {
+    unsigned grid = 0;
+    for (int k = 0; k < all.n; ++k) {
+      SplitJob& j = all.j[k];
+      j.first = grid;
+      j.across = unsigned((j.n8 + kSplitCols - 1) / kSplitCols);
+      grid += j.across * unsigned((j.rows + kSplitRows - 1) / kSplitRows);
+    }
+    if (!r.go) return;
+    hipLaunchKernelGGL(fill_kernel, dim3(unsigned((n_tops + 255) / 256)), dim3(256), 0, r.s, tops, n_tops);
+    if (!grid) return;
+    hipLaunchKernelGGL(split_scan_kernel, dim3(grid), dim3(256), 0, r.s, all);
+    hipLaunchKernelGGL(split_kernel, dim3(grid), dim3(256), 0, r.s, all);
+  }
+};
+Halves by_rows(const SplitJob& j) { return {{j.row_hi, j.n8, j.rows, j.n, j.n8}, {j.row_hi + j.rows * j.n8, j.n8, j.rows, j.n, j.n8}, j.row_top}; }
+Halves by_columns(const SplitJob& j) { return {{j.col_hi, j.n8, j.rows, j.n, j.n8}, {j.col_hi + j.rows * j.n8, j.n8, j.rows, j.n, j.n8}, j.col_top}; }
+// hi hi + hi lo + lo hi, the small products first
+void set_segments(Side& i, Side& j, int at, const Halves& a, const Halves& b) {
+  const auto p = [](const Matrix& m) { return static_cast<const char*>(m.p); };
+  i.p[at] = p(a.hi), j.p[at] = p(b.lo);
+  i.p[at + 1] = p(a.lo), j.p[at + 1] = p(b.hi);
+  i.p[at + 2] = p(a.hi), j.p[at + 2] = p(b.hi);
+}
+Problem problem32(Side i, Side j, const Halves& a, const Halves& b, long m, long n, long k, float* out, long ld) {
+  set_segments(i, j, 0, a, b);
+  Problem p = problem<float>(i, j, m, n, k, 3, out, ld);
+  p.top_i = a.top, p.top_j = b.top;
+  return p;
+}
+
+hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r) {
+  const long rows = d.rows, width = d.width, hidden = d.hidden, out = d.out, hp = align_up(hidden, 8);
+  const long n_tops = 2 * align_up(rows, 64) + 2 * align_up(hidden, 64) + align_up(out, 64);
+  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(n_tops) * 4));
+  Splitter one(r);
+  one.tops = base;
+  unsigned *tx = one.table(base, rows), *tg = one.table(base, hidden), *tu = one.table(base, hidden), *td = one.table(base, out),
+           *th = one.table(base, rows);
+  const Halves x = by_rows(one.add((const float*)d.x, d.ld_x, rows, width, tx, nullptr, 1));
+  const Halves wg = by_rows(one.add((const float*)d.w_gate, d.ld_gate, hidden, width, tg, nullptr, 1));
+  const Halves wu = by_rows(one.add((const float*)d.w_up, d.ld_up, hidden, width, tu, nullptr, 1));
+  const Halves wd = by_rows(one.add((const float*)d.w_down, d.ld_down, out, hidden, td, nullptr, 1));
+  one.run();
+  float* h = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
+  Side i = rows_side(x.hi), j = halves(Pair{wg.hi, wu.hi});
+  set_segments(i, j, 0, x, wg);
+  launch_gate<_Float16, float>(r, d, i, j, 3, h, hp, Scales{tx, tg, tu, nullptr, nullptr});
+  Splitter two(r);
+  two.tops = th;       // zeroed twice: its table lies in the first pass's memory
+  two.n_tops = align_up(rows, 64);
+  const Halves hh = by_rows(two.add(h, hp, rows, hidden, th, nullptr, 1));
+  two.run();
+  Problems all{};
+  all.n = 1;
+  all.p[0] = problem32(rows_side(hh.hi), rows_side(wd.hi), hh, wd, rows, out, hidden, y, ld_y);
+  r.products<_Float16, true, true, float>(all);
   return hipGetLastError();
 }
 
-template <typename T>
-hipError_t backward(const nerf_block_desc& d, const void* dy, long ld_dy, T* dx, long ld_dx, T* dwg, T* dwu, T* dwd, void* ws,
-                    hipStream_t s) {
-  const long n = long(d.rows) * d.hidden;
-  T *h = static_cast<T*>(ws), *dg = h + n, *du = dg + n;
-  const long rows = d.rows, width = d.width, hidden = d.hidden, out = d.out;
-  const Operand x{d.x, d.ld_x, 1}, wg{d.w_gate, d.ld_gate, 1}, wu{d.w_up, d.ld_up, 1}, no{};
-  if (rows) hipLaunchKernelGGL((gate_kernel<T, true>), tiles(rows, hidden), dim3(256), 0, s, x, wg, wu, Operand{dy, ld_dy, 1},
-                     Operand{d.w_down, 1, d.ld_down}, rows, hidden, width, out, d.activation, h, dg, du);
-  auto product = [&](Operand a1, Operand b1, Operand a2, Operand b2, long m, long nn, long k, T* c, long ldc) {
-    if (c && m) hipLaunchKernelGGL((product_kernel<T>), tiles(m, nn), dim3(256), 0, s, a1, b1, a2, b2, m, nn, k, c, ldc);
-  };
-  product({dg, hidden, 1}, {d.w_gate, 1, d.ld_gate}, {du, hidden, 1}, {d.w_up, 1, d.ld_up}, rows, width, hidden, dx, ld_dx);
-  const Operand xt{d.x, 1, d.ld_x};
-  product({dg, 1, hidden}, xt, no, no, hidden, width, rows, dwg, width);
-  product({du, 1, hidden}, xt, no, no, hidden, width, rows, dwu, width);
-  product({dy, 1, ld_dy}, {h, 1, hidden}, no, no, out, hidden, rows, dwd, hidden);
+hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_dy, float* dx, long ld_dx, float* dwg, float* dwu,
+                           float* dwd, Run& r) {
+  const long rows = d.rows, width = d.width, hidden = d.hidden, out = d.out, hp = align_up(hidden, 8);
+  const long n1 = 2 * align_up(rows, 64) + 3 * align_up(hidden, 64) + 2 * align_up(width, 64) + align_up(out, 64);
+  const long n2 = align_up(rows, 64) + 3 * align_up(hidden, 64);
+  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(n1 + n2) * 4));
+  Splitter one(r);
+  one.tops = base;
+  unsigned *xr = one.table(base, rows), *xc = one.table(base, width), *gr = one.table(base, hidden), *ur = one.table(base, hidden),
+           *wc = one.table(base, width), *dc = one.table(base, hidden), *yr = one.table(base, rows), *yc = one.table(base, out);
+  const SplitJob jx = one.add((const float*)d.x, d.ld_x, rows, width, xr, xc, 3);
+  // dx adds the products of both weights: one table of their columns
+  const SplitJob jg = one.add((const float*)d.w_gate, d.ld_gate, hidden, width, gr, wc, 3);
+  const SplitJob ju = one.add((const float*)d.w_up, d.ld_up, hidden, width, ur, wc, 3);
+  const SplitJob jd = one.add((const float*)d.w_down, d.ld_down, out, hidden, nullptr, dc, 2);
+  const SplitJob jy = one.add(dy_p, ld_dy, rows, out, yr, yc, 3);
+  one.run();
+  float* h = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
+  float* dg = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
+  float* du = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
+  const Halves x = by_rows(jx), wg = by_rows(jg), wu = by_rows(ju), dy = by_rows(jy), wd = by_columns(jd);
+  Side i = rows_side(x.hi), j = halves(Pair{wg.hi, wu.hi}), iy = rows_side(dy.hi), jw = columns_side(wd.hi);
+  set_segments(i, j, 0, x, wg);
+  set_segments(iy, jw, 0, dy, wd);
+  launch_gate_back<_Float16, float>(r, d, i, j, iy, jw, 3, h, dg, du, hp, Scales{xr, gr, ur, yr, dc});
+  Splitter two(r);
+  two.tops = base ? base + n1 : nullptr;
+  unsigned *tr = two.table(two.tops, rows), *hc = two.table(two.tops, hidden), *gc = two.table(two.tops, hidden),
+           *uc = two.table(two.tops, hidden);
+  const SplitJob kh = two.add(h, hp, rows, hidden, nullptr, hc, 2);
+  const SplitJob kg = two.add(dg, hp, rows, hidden, tr, gc, 3);      // one table of both gradients' rows
+  const SplitJob ku = two.add(du, hp, rows, hidden, tr, uc, 3);
+  two.run();
+  if ((dx || !r.go) && rows) {
+    const Halves g = by_rows(kg), u = by_rows(ku), cg = by_columns(jg), cu = by_columns(ju);
+    Side a = rows_side(g.hi), b = columns_side(cg.hi);
+    set_segments(a, b, 0, g, cg);
+    set_segments(a, b, 3, u, cu);
+    Problems all{};
+    all.n = 1;
+    all.p[0] = problem<float>(a, b, rows, width, hidden, 6, dx, ld_dx);
+    all.p[0].top_i = tr, all.p[0].top_j = wc;
+    r.products<_Float16, true, false, float>(all);
+  }
+  const Halves cx = by_columns(jx), cg = by_columns(kg), cu = by_columns(ku), cy = by_columns(jy), ch = by_columns(kh);
+  Problems all{};
+  if (dwg || !r.go) all.p[all.n++] = problem32(columns_side(cg.hi), columns_side(cx.hi), cg, cx, hidden, width, rows, dwg, width);
+  if (dwu || !r.go) all.p[all.n++] = problem32(columns_side(cu.hi), columns_side(cx.hi), cu, cx, hidden, width, rows, dwu, width);
+  if (dwd || !r.go) all.p[all.n++] = problem32(columns_side(cy.hi), columns_side(ch.hi), cy, ch, out, hidden, rows, dwd, hidden);
+  if (all.n) r.products<_Float16, false, false, float>(all);
   return hipGetLastError();
 }
 
@@ -499,7 +681,7 @@ int check(const nerf_block_desc* d, const char* who) {
       d->out > (1 << 20))
     return set_error(NERF_E_INVALID, "%s: rows %ld, width %d, hidden %d, out %d", who, long(d->rows), d->width, d->hidden, d->out);
   const long widest = d->width > d->hidden ? (d->width > d->out ? d->width : d->out) : d->hidden > d->out ? d->hidden : d->out;
-  if (((d->rows + kT - 1) / kT) * ((widest + kT - 1) / kT) > 0x7fffffffL) return set_error(NERF_E_INVALID, "%s: too many tiles", who);
+  if (((d->rows + 63) / 64) * ((widest + 63) / 64) > 0x7fffffffL) return set_error(NERF_E_INVALID, "%s: too many tiles", who);
   if (d->ld_x < d->width || d->ld_gate < d->width || d->ld_up < d->width || d->ld_down < d->hidden)
     return set_error(NERF_E_INVALID, "%s: a row stride is shorter than its row", who);
   if ((d->rows && !d->x) || !d->w_gate || !d->w_up || !d->w_down) return set_error(NERF_E_INVALID, "%s: null operand", who);
@@ -525,9 +707,11 @@ extern "C" {
 
 size_t nerf_gated_block_workspace(const nerf_block_desc* d, int backward) {
   if (check(d, "nerf_gated_block_workspace") != NERF_OK) return 0;
-  if (d->dtype == NERF_F32) return size_t(d->rows) * d->hidden * 4 * (backward ? 3 : 1);
   Run r{nullptr, Arena{nullptr}, false};
-  if (backward) (void)backward_mma<__bf16>(*d, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, r);
+  if (d->dtype == NERF_F32) {
+    if (backward) (void)backward_halves(*d, nullptr, d->out, nullptr, 0, nullptr, nullptr, nullptr, r);
+    else (void)forward_halves(*d, nullptr, 0, r);
+  } else if (backward) (void)backward_mma<__bf16>(*d, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, r);
   else (void)forward_mma<__bf16>(*d, nullptr, 0, r);
   return r.a.used;
 }
@@ -542,7 +726,7 @@ int nerf_gated_block_forward(const nerf_block_desc* d, void* y, int64_t ld_y, vo
   if ((rc = check_workspace(d, 0, workspace, workspace_bytes, who)) != NERF_OK) return rc;
   const hipStream_t s = (hipStream_t)stream;
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
-  const hipError_t e = d->dtype == NERF_F32        ? forward<float>(*d, (float*)y, ld_y, workspace, s)
+  const hipError_t e = d->dtype == NERF_F32        ? forward_halves(*d, (float*)y, ld_y, r)
                        : d->dtype == NERF_BFLOAT16 ? forward_mma<__bf16>(*d, (__bf16*)y, ld_y, r)
                                                    : forward_mma<_Float16>(*d, (_Float16*)y, ld_y, r);
   if (e != hipSuccess) return set_error(NERF_E_HIP, "%s: %s", who, hipGetErrorString(e));
@@ -564,7 +748,7 @@ int nerf_gated_block_backward(const nerf_block_desc* d, const void* dy, int64_t 
   const hipStream_t s = (hipStream_t)stream;
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
   const hipError_t e =
-      d->dtype == NERF_F32 ? backward<float>(*d, dy, ld_dy, (float*)dx, ld_dx, (float*)dw_gate, (float*)dw_up, (float*)dw_down, workspace, s)
+      d->dtype == NERF_F32 ? backward_halves(*d, (const float*)dy, ld_dy, (float*)dx, ld_dx, (float*)dw_gate, (float*)dw_up, (float*)dw_down, r)
       : d->dtype == NERF_BFLOAT16
           ? backward_mma<__bf16>(*d, dy, ld_dy, (__bf16*)dx, ld_dx, (__bf16*)dw_gate, (__bf16*)dw_up, (__bf16*)dw_down, r)
           : backward_mma<_Float16>(*d, dy, ld_dy, (_Float16*)dx, ld_dx, (_Float16*)dw_gate, (_Float16*)dw_up, (_Float16*)dw_down, r);

@@ -85,7 +85,8 @@ def parse_insn(lineno, raw):
     # modifiers after the operands (offset:, op_sel:, ...) carry no registers but m0 forms
     ops = split_operands(rest)
     if op.startswith(NO_DST) or "_lds_" in op or (op.startswith("buffer_load") and " lds" in text) \
-            or op.startswith("global_load_lds"):
+            or op.startswith("global_load_lds") \
+            or (op.startswith(("global_atomic", "buffer_atomic")) and " sc0" not in text):   # returns nothing
         return Insn(lineno, op, set(), set().union(*[regs(o) for o in ops]) if ops else set(), text)
     if not ops:
         return Insn(lineno, op, set(), set(), text)
