@@ -5,6 +5,7 @@
 // g and u never reach memory: the forward's first kernel holds both accumulators of a tile and writes
 // h; the backward's first kernel recomputes them beside dh and writes h, dg and du.
 #include <cmath>
+#include <type_traits>
 
 #include "block_mma.h"
 #include "nerf_internal.h"
@@ -215,6 +216,132 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long ld, long ro
   to[0] = o[0];
   to[1] = o[1];
 }
+
+// ----------------------------------------------------------------------------------------- few rows --
+// Up to 64 rows (a token of each of a few sequences): the weights' bytes are the cost, so they go from
+// memory to fragments without LDS.  A workgroup owns 16 weight rows (of Wg and of Wu); its waves take
+// every WAVES-th step of k, so that together they read whole lines of each row, and add up their
+// accumulators in LDS in wave order.  fp32 runs on the f32 matrix instruction at full precision: at a few
+// rows it still outruns memory (4 x 32 cycles a KiB of weights a SIMD).
+template <typename T>
+struct FewStep {   // 16 bytes of k a lane: 32 values of k a step
+  static constexpr int kK = 32, kLane = 8;
+  typedef typename Frag<T>::type Data;
+  static __device__ __forceinline__ f32x4_t mma(Data w, Data x, f32x4_t c) { return Frag<T>::mma(w, x, c); }
+};
+template <>
+struct FewStep<float> {
+  static constexpr int kK = 16, kLane = 4;
+  typedef f32x4_t Data;
+  static __device__ __forceinline__ f32x4_t mma(Data w, Data x, f32x4_t c) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) c = __builtin_amdgcn_mfma_f32_16x16x4f32(w[m], x[m], c, 0, 0, 0);
+    return c;
+  }
+};
+// the lane's values of k from k0 (a multiple of kLane) of one row, zeros behind the end
+template <typename T, bool WHOLE>
+__device__ __forceinline__ typename FewStep<T>::Data few_load(const T* row, long k0, long k) {
+  typename FewStep<T>::Data v;
+  if (WHOLE) {
+    if (k0 < k) v = *reinterpret_cast<const typename FewStep<T>::Data*>(row + k0);
+    else
+      for (int r = 0; r < FewStep<T>::kLane; ++r) v[r] = T(0.0f);
+  } else {
+#pragma unroll
+    for (int r = 0; r < FewStep<T>::kLane; ++r) v[r] = k0 + r < k ? row[k0 + r] : T(0.0f);
+  }
+  return v;
+}
+struct Few {
+  const void *x, *w, *w2;
+  long ld_x, ld_w, ld_w2, ld_out;
+  int rows, n, n_out, kind;    // columns n .. n_out - 1 of out are zeros
+  long k;
+  void* out;
+};
+// GATE: out = act(x w^T) (x w2^T), else out = x w^T
+template <typename T, int NI, int WAVES, bool WHOLE, bool GATE>
+__global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
+  typedef FewStep<T> S;
+  constexpr int kU = 4, M = GATE ? 2 : 1;
+  __shared__ f32x4_t red[WAVES][M * NI][64];
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, e = l & 15, g = l >> 4;
+  const int j0 = blockIdx.x * 16;
+  const long wr = min(j0 + e, p.n - 1);
+  const T* w = static_cast<const T*>(p.w) + wr * p.ld_w;
+  const T* w2 = GATE ? static_cast<const T*>(p.w2) + wr * p.ld_w2 : nullptr;
+  const T* x[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) x[i] = static_cast<const T*>(p.x) + long(min(i * 16 + e, p.rows - 1)) * p.ld_x;
+  f32x4_t acc[M][NI] = {};
+  const auto steps = [&](long k0, auto count, auto checked) {
+    constexpr int U = decltype(count)::value;
+    const long k = decltype(checked)::value ? p.k : 0x7fffffffffffffffL;
+    typename S::Data fw[U][M], fx[U][NI];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long at = k0 + u * WAVES * S::kK + g * S::kLane;
+      fw[u][0] = few_load<T, WHOLE>(w, at, k);
+      if (GATE) fw[u][M - 1] = few_load<T, WHOLE>(w2, at, k);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) fx[u][i] = few_load<T, WHOLE>(x[i], at, k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[m][i] = S::mma(fw[u][m], fx[u][i], acc[m][i]);
+  };
+  long k0 = long(wave) * S::kK;
+  if (WHOLE)
+    for (; k0 + ((kU - 1) * WAVES + 1) * S::kK <= p.k; k0 += kU * WAVES * S::kK)
+      steps(k0, std::integral_constant<int, kU>{}, std::false_type{});
+  for (; k0 < p.k; k0 += WAVES * S::kK) steps(k0, std::integral_constant<int, 1>{}, std::true_type{});
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) red[wave][m * NI + i][l] = acc[m][i];
+  __syncthreads();
+  if (wave >= NI) return;
+  const int i = wave;
+  f32x4_t a = red[0][i][l], b = red[0][(M - 1) * NI + i][l];
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) {
+    a += red[v][i][l];
+    if (GATE) b += red[v][NI + i][l];
+  }
+  const int row = i * 16 + e, col = j0 + g * 4;
+  if (row >= p.rows) return;
+  T* out = static_cast<T*>(p.out) + row * p.ld_out;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float v = a[r], d;
+    if (GATE) {
+      activate(p.kind, a[r], v, d);
+      v *= b[r];
+    }
+    if (col + r < p.n_out) out[col + r] = T(col + r < p.n ? v : 0.0f);
+  }
+}
+template <typename T, bool GATE>
+void launch_few(const Few& p, bool all_whole, hipStream_t s) {
+  const dim3 grid(unsigned((p.n_out + 15) / 16));
+  const auto go = [&](auto ni, auto whole) {
+    constexpr int NI = decltype(ni)::value, WAVES = NI == 1 ? 16 : 8;
+    hipLaunchKernelGGL((few_kernel<T, NI, WAVES, decltype(whole)::value, GATE>), grid, dim3(WAVES * 64), 0, s, p);
+  };
+  const auto rows = [&](auto whole) {
+    if (p.rows <= 16) go(std::integral_constant<int, 1>{}, whole);
+    else if (p.rows <= 32) go(std::integral_constant<int, 2>{}, whole);
+    else go(std::integral_constant<int, 4>{}, whole);
+  };
+  if (all_whole) rows(std::true_type{});
+  else rows(std::false_type{});
+}
+// h's row stride for few rows: whole 16-byte pieces
+constexpr int kFewRows = 64;
 
 // 32-bit matrices on their way to halves: the largest finite |value| of each row and / or column (bits in
 // zeroed tables; a maximum does not depend on the order of the atomics), then the halves by either.
@@ -487,6 +614,26 @@ void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Sid
 }
 
 template <typename T>
+hipError_t forward_few(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
+  const long hp = align_up(d.hidden, 8);
+  T* h = static_cast<T*>(r.a.take(size_t(d.rows) * hp * sizeof(T)));
+  if (!r.go) return hipSuccess;
+  constexpr long kV = 16 / sizeof(T);
+  const auto whole16 = [](const void* p, long ld, long n) { return !(uintptr_t(p) & 15) && ld % kV == 0 && n % kV == 0; };
+  Few a{};
+  a.x = d.x, a.w = d.w_gate, a.w2 = d.w_up, a.out = h;
+  a.ld_x = d.ld_x, a.ld_w = d.ld_gate, a.ld_w2 = d.ld_up, a.ld_out = hp;
+  a.rows = int(d.rows), a.n = d.hidden, a.n_out = int(hp), a.kind = d.activation, a.k = d.width;
+  launch_few<T, true>(a, whole16(d.x, d.ld_x, d.width) && whole16(d.w_gate, d.ld_gate, d.width) && whole16(d.w_up, d.ld_up, d.width), r.s);
+  Few b{};
+  b.x = h, b.w = d.w_down, b.out = y;
+  b.ld_x = hp, b.ld_w = d.ld_down, b.ld_out = ld_y;
+  b.rows = int(d.rows), b.n = b.n_out = d.out, b.k = d.hidden;
+  launch_few<T, false>(b, whole16(d.w_down, d.ld_down, d.hidden), r.s);
+  return hipGetLastError();
+}
+
+template <typename T>
 hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const long rows = d.rows, hidden = d.hidden, hp = align_up(hidden, 8);
   const Matrix x = r.matrix<T>(d.x, d.ld_x, rows, d.width);
@@ -708,7 +855,10 @@ extern "C" {
 size_t nerf_gated_block_workspace(const nerf_block_desc* d, int backward) {
   if (check(d, "nerf_gated_block_workspace") != NERF_OK) return 0;
   Run r{nullptr, Arena{nullptr}, false};
-  if (d->dtype == NERF_F32) {
+  if (!backward && d->rows <= kFewRows) {
+    if (d->dtype == NERF_F32) (void)forward_few<float>(*d, nullptr, 0, r);
+    else (void)forward_few<__bf16>(*d, nullptr, 0, r);
+  } else if (d->dtype == NERF_F32) {
     if (backward) (void)backward_halves(*d, nullptr, d->out, nullptr, 0, nullptr, nullptr, nullptr, r);
     else (void)forward_halves(*d, nullptr, 0, r);
   } else if (backward) (void)backward_mma<__bf16>(*d, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, r);
@@ -726,9 +876,11 @@ int nerf_gated_block_forward(const nerf_block_desc* d, void* y, int64_t ld_y, vo
   if ((rc = check_workspace(d, 0, workspace, workspace_bytes, who)) != NERF_OK) return rc;
   const hipStream_t s = (hipStream_t)stream;
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
-  const hipError_t e = d->dtype == NERF_F32        ? forward_halves(*d, (float*)y, ld_y, r)
-                       : d->dtype == NERF_BFLOAT16 ? forward_mma<__bf16>(*d, (__bf16*)y, ld_y, r)
-                                                   : forward_mma<_Float16>(*d, (_Float16*)y, ld_y, r);
+  const bool few = d->rows <= kFewRows;
+  const hipError_t e =
+      d->dtype == NERF_F32        ? (few ? forward_few<float>(*d, (float*)y, ld_y, r) : forward_halves(*d, (float*)y, ld_y, r))
+      : d->dtype == NERF_BFLOAT16 ? (few ? forward_few<__bf16>(*d, (__bf16*)y, ld_y, r) : forward_mma<__bf16>(*d, (__bf16*)y, ld_y, r))
+                                  : (few ? forward_few<_Float16>(*d, (_Float16*)y, ld_y, r) : forward_mma<_Float16>(*d, (_Float16*)y, ld_y, r));
   if (e != hipSuccess) return set_error(NERF_E_HIP, "%s: %s", who, hipGetErrorString(e));
   return NERF_OK;
 }

@@ -14,49 +14,67 @@ The reference has no counterpart: its networks are ReLU chains on sin / cos enco
 """
 from __future__ import annotations
 
+import array
 import ctypes
-from contextlib import ExitStack
+import struct
+from contextlib import ExitStack, nullcontext
 from typing import Optional, Sequence
 
 from . import runtime as rt
 
 PAIRS = ("split", "interleaved")
 LADDERS = ("axis", "shared")
+_NOTHING = nullcontext()
 ACTIVATIONS = {"silu": rt.NERF_SILU, "gelu": rt.NERF_GELU, "relu": rt.NERF_RELU}
 
 
-def _dtypes():
-    import torch
+_TYPES: dict = {}
 
-    return {torch.float32: rt.NERF_F32, torch.bfloat16: rt.NERF_BFLOAT16, torch.float16: rt.NERF_FLOAT16}
+
+def _dtypes():
+    if not _TYPES:
+        import torch
+
+        _TYPES.update({torch.float32: rt.NERF_F32, torch.bfloat16: rt.NERF_BFLOAT16, torch.float16: rt.NERF_FLOAT16})
+    return _TYPES
+
+
+def _plain(torch, t, name) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: the operators are not recorded by autograd (detach it or use "
+                         "torch.no_grad(); the gradients are calls of their own)")
 
 
 def _check_plain(torch, **tensors) -> None:
     for name, t in tensors.items():
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires grad: the operators are not recorded by autograd (detach it or use "
-                             "torch.no_grad(); the gradients are calls of their own)")
+        _plain(torch, t, name)
 
 
-class _On(ExitStack):
-    """The device and stream a call runs on: current while tensors are allocated and work is queued."""
+def _on(torch, tensors, stream):
+    """(stream handle, contexts to enter) for a call on tensors of one device: its device and stream are
+    current while memory is allocated and work is queued."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index:
+            raise ValueError(f"tensors on {t.device} and {tensors[0].device}")
+    if index < 0 or tensors[0].device.type != "cuda":
+        raise ValueError(f"device tensors are needed, got {tensors[0].device}")
+    contexts = []
+    if torch.cuda.current_device() != index:
+        contexts.append(torch.cuda.device(index))
+    if stream is None:
+        return torch.cuda.current_stream(index).cuda_stream, contexts
+    if stream.device.index != index:
+        raise ValueError(f"the stream is on {stream.device}, not on {tensors[0].device}")
+    contexts.append(torch.cuda.stream(stream))
+    return stream.cuda_stream, contexts
 
-    def __init__(self, torch, device, stream, **tensors):
-        super().__init__()
-        for name, t in tensors.items():
-            if t.device != device:
-                raise ValueError(f"{name} is on {t.device}, not on {device}")
-        if device.type != "cuda":
-            raise ValueError(f"device tensors are needed, got {device}")
-        if stream is not None and stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, not on {device}")
-        if torch.cuda.current_device() != device.index:
-            self.enter_context(torch.cuda.device(device))
-        if stream is not None:
-            self.enter_context(torch.cuda.stream(stream))
-        self.stream = int(torch.cuda.current_stream(device).cuda_stream)
+
+# nerf_rotary_desc in one pack (the members of runtime.RotaryDesc in order, native alignment)
+_ROTARY = struct.Struct("@iii4iiiidPPi3qiqi" + "PPi3q3q" * 2)
+_NO_TENSOR = (0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
 def rotary_axes(x, positions, sections: Sequence[int], *, base: float = 10000.0, ladder: str = "axis",
@@ -79,42 +97,49 @@ def rotary_axes(x, positions, sections: Sequence[int], *, base: float = 10000.0,
     xs = (x,) if single else tuple(x)
     if not 1 <= len(xs) <= 2:
         raise ValueError(f"one or two tensors, got {len(xs)}")
-    _check_plain(torch, positions=positions, **{f"x[{i}]": t for i, t in enumerate(xs)})
+    for i, t in enumerate(xs):
+        _plain(torch, t, f"x[{i}]")
+    _plain(torch, positions, "positions")
     outs = None
     if out is not None:
         outs = (out,) if single else tuple(out)
         if len(outs) != len(xs):
             raise ValueError(f"{len(xs)} outputs needed, got {len(outs)}")
-        _check_plain(torch, **{f"out[{i}]": t for i, t in enumerate(outs)})
+        for i, t in enumerate(outs):
+            _plain(torch, t, f"out[{i}]")
     first = xs[0]
-    codes = _dtypes()
-    if first.dtype not in codes:
+    kind = _dtypes().get(first.dtype)
+    if kind is None:
         raise ValueError(f"x must be float32, bfloat16 or float16, got {first.dtype}")
     sections = [int(s) for s in sections]
-    total = sum(sections)
-    if not 1 <= len(sections) <= rt.NERF_ROTARY_MAX_AXES or min(sections) < 0:
+    axes, total = len(sections), sum(sections)
+    if not 1 <= axes <= rt.NERF_ROTARY_MAX_AXES or min(sections) < 0:
         raise ValueError(f"sections {sections}: 1 to {rt.NERF_ROTARY_MAX_AXES} counts of pairs")
     if pairs not in PAIRS:
         raise ValueError(f"pairs {pairs!r}: one of {PAIRS}")
     if ladder not in LADDERS:
         raise ValueError(f"ladder {ladder!r}: one of {LADDERS}")
-    if first.dim() not in (3, 4):
-        raise ValueError(f"x must be [tokens, heads, dim] or [batch, tokens, heads, dim], got {tuple(first.shape)}")
-    batched = first.dim() == 4
-    batch = first.shape[0] if batched else 1
-    tokens, dim = int(first.shape[-3]), int(first.shape[-1])
+    shape = first.shape
+    if len(shape) not in (3, 4):
+        raise ValueError(f"x must be [tokens, heads, dim] or [batch, tokens, heads, dim], got {tuple(shape)}")
+    batched = len(shape) == 4
+    batch = shape[0] if batched else 1
+    tokens, dim = shape[-3], shape[-1]
     if 2 * total > dim or total > rt.NERF_ROTARY_MAX_PAIRS:
         raise ValueError(f"sections {sections} hold {total} pairs: at most {min(dim // 2, rt.NERF_ROTARY_MAX_PAIRS)}")
+    strides = []
     for i, t in enumerate(xs):
-        if t.dim() != first.dim() or t.dtype != first.dtype or t.shape[:-2] != first.shape[:-2] or t.shape[-1] != dim:
-            raise ValueError(f"x[{i}] {tuple(t.shape)} {t.dtype} does not go with x[0] {tuple(first.shape)} {first.dtype}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if i and (t.dtype != first.dtype or t.shape[:-2] != shape[:-2] or t.shape[-1] != dim):
+            raise ValueError(f"x[{i}] {tuple(t.shape)} {t.dtype} does not go with x[0] {tuple(shape)} {first.dtype}")
+        stride = t.stride()
+        if dim > 1 and stride[-1] != 1:
             raise ValueError(f"x[{i}]'s last dimension must be contiguous")
-    shape = tuple(positions.shape)
-    if shape not in ((tokens, len(sections)), (batch, tokens, len(sections))):
-        raise ValueError(f"positions must be [{tokens}, {len(sections)}] or [{batch}, {tokens}, {len(sections)}], got {shape}")
-    kinds = {torch.float32: rt.NERF_F32, torch.int32: rt.NERF_INT32, torch.int64: rt.NERF_INT64}
-    if positions.dtype not in kinds:
+        strides.append(stride)
+    where = tuple(positions.shape)
+    if where != (tokens, axes) and where != (batch, tokens, axes):
+        raise ValueError(f"positions must be [{tokens}, {axes}] or [{batch}, {tokens}, {axes}], got {where}")
+    position = {torch.int64: rt.NERF_INT64, torch.int32: rt.NERF_INT32, torch.float32: rt.NERF_F32}.get(positions.dtype)
+    if position is None:
         raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
     if outs is not None:
         for i, (t, o) in enumerate(zip(xs, outs)):
@@ -126,73 +151,72 @@ def rotary_axes(x, positions, sections: Sequence[int], *, base: float = 10000.0,
                 raise ValueError(f"out[{i}] overlaps x[{i}] in another order")
         if len(outs) == 2 and outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel() and outs[1].numel():
             raise ValueError("the two outputs share their memory")
-    d = rt.RotaryDesc()
-    d.dtype, d.head_dim, d.n_axes = codes[first.dtype], dim, len(sections)
-    d.sections[:len(sections)] = sections
-    d.shared_ladder, d.interleaved, d.inverse = ladder == "shared", pairs == "interleaved", bool(inverse)
-    d.base = float(base)
+    table = None
     if frequencies is not None:
-        table = [float(f) for f in frequencies]
+        table = array.array("d", frequencies)
         if len(table) != total:
             raise ValueError(f"{total} frequencies needed, got {len(table)}")
-        d.frequencies = (ctypes.c_double * total)(*table)
-    stride = positions.stride()
-    d.position_stride[:] = stride if len(shape) == 3 else (0, *stride)
-    d.position_dtype, d.n_batch, d.n_tokens, d.n_tensors = kinds[positions.dtype], batch, tokens, len(xs)
-    named = {f"x[{i}]": t for i, t in enumerate(xs)}
-    named.update({f"out[{i}]": t for i, t in enumerate(outs or ())})
-    with _On(torch, first.device, stream, positions=positions, **named) as on:
+    handle, contexts = _on(torch, (*xs, positions, *(outs or ())), stream)
+    with ExitStack() if contexts else _NOTHING as stack:
+        for c in contexts:
+            stack.enter_context(c)
         if outs is None:
-            outs = tuple(torch.empty_like(t) for t in xs)
-        d.positions = positions.data_ptr()
-        for k, (t, o) in enumerate(zip(xs, outs)):
-            e = d.tensor[k]
-            e.x, e.out, e.heads = t.data_ptr(), o.data_ptr(), t.shape[-2]
-            e.x_stride[:] = t.stride()[:3] if batched else (0, *t.stride()[:2])
-            e.out_stride[:] = o.stride()[:3] if batched else (0, *o.stride()[:2])
-        rt._check(rt.load_library().nerf_rotary_axes(ctypes.byref(d), on.stream))
+            outs = tuple([torch.empty_like(t) for t in xs])
+        tensors = []
+        for t, o, st in zip(xs, outs, strides):
+            so = o.stride()
+            tensors += [t.data_ptr(), o.data_ptr(), t.shape[-2]]
+            tensors += st[:3] if batched else (0, *st[:2])
+            tensors += so[:3] if batched else (0, *so[:2])
+        if len(xs) == 1:
+            tensors += _NO_TENSOR
+        stride = positions.stride()
+        desc = _ROTARY.pack(kind, dim, axes, *sections, *(0,) * (rt.NERF_ROTARY_MAX_AXES - axes), ladder == "shared",
+                            pairs == "interleaved", bool(inverse), base, table.buffer_info()[0] if table else 0,
+                            positions.data_ptr(), position, *(stride if len(where) == 3 else (0, *stride)), batch, tokens,
+                            len(xs), *tensors)
+        rt._check(rt.load_library().nerf_rotary_axes(desc, handle))
     return outs[0] if single else outs
 
 
 def _rows(t, name: str, width: int):
-    """t [..., width] as [rows, width] without a copy, and its row stride."""
-    if t.dim() < 1 or t.shape[-1] != width:
-        raise ValueError(f"{name} must be [..., {width}], got {tuple(t.shape)}")
-    if width > 1 and t.stride(-1) != 1 and t.numel():
+    """(rows, row stride) of t [..., width] as a matrix, without a copy."""
+    shape, stride = t.shape, t.stride()
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{name} must be [..., {width}], got {tuple(shape)}")
+    if width > 1 and stride[-1] != 1 and t.numel():
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    if t.dim() != 2:
+    if len(shape) != 2:
         try:
             t = t.view(-1, width) if t.numel() else t.reshape(0, width)
         except RuntimeError:
-            raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()} is not rows of one stride") from None
-    stride = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
-    if stride < width:
-        raise ValueError(f"{name}'s rows overlap (stride {stride}, width {width})")
-    return t, stride
+            raise ValueError(f"{name} {tuple(shape)} with strides {stride} is not rows of one stride") from None
+        shape, stride = t.shape, t.stride()
+    step = stride[0] if shape[0] > 1 else max(stride[0], width)
+    if step < width:
+        raise ValueError(f"{name}'s rows overlap (stride {step}, width {width})")
+    return shape[0], step
 
 
 def _block(torch, x, w_gate, w_up, w_down, activation):
-    _check_plain(torch, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down)
-    codes = _dtypes()
-    if x.dtype not in codes:
+    _plain(torch, x, "x")
+    kind, codes = x.dtype, _dtypes()
+    if kind not in codes:
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r}: one of {tuple(ACTIVATIONS)}")
     for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        if w.dim() != 2 or w.dtype != x.dtype or 0 in w.shape:
+        _plain(torch, w, name)
+        if w.dim() != 2 or w.dtype != kind or 0 in w.shape:
             raise ValueError(f"{name} must be a matrix of x's type {x.dtype}, got {tuple(w.shape)} {w.dtype}")
     hidden, width = w_gate.shape
     if w_up.shape != w_gate.shape or w_down.shape[1] != hidden:
         raise ValueError(f"w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down {tuple(w_down.shape)} must be "
                          "[hidden, width], [hidden, width] and [out, hidden]")
-    d = rt.BlockDesc()
-    x2, d.ld_x = _rows(x, "x", width)
-    for name, w, n in (("gate", w_gate, width), ("up", w_up, width), ("down", w_down, hidden)):
-        setattr(d, f"ld_{name}", _rows(w, f"w_{name}", n)[1])
-    d.dtype, d.activation = codes[x.dtype], ACTIVATIONS[activation]
-    d.rows, d.width, d.hidden, d.out = x2.shape[0], width, hidden, w_down.shape[0]
-    d.x, d.w_gate, d.w_up, d.w_down = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
-    return d
+    rows, ld_x = _rows(x, "x", width)
+    return rt.BlockDesc(codes[kind], ACTIVATIONS[activation], rows, width, hidden, w_down.shape[0], x.data_ptr(),
+                        w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), ld_x, _rows(w_gate, "w_gate", width)[1],
+                        _rows(w_up, "w_up", width)[1], _rows(w_down, "w_down", hidden)[1])
 
 
 def _workspace(torch, d, backward: int, device):
@@ -215,14 +239,18 @@ def gated_block(x, w_gate, w_up, w_down, *, activation: str = "silu", out=None, 
         _check_plain(torch, out=out)
         if tuple(out.shape) != shape or out.dtype != x.dtype:
             raise ValueError(f"out must be {shape} {x.dtype}, got {tuple(out.shape)} {out.dtype}")
-    named = dict(w_gate=w_gate, w_up=w_up, w_down=w_down, **({} if out is None else {"out": out}))
-    with _On(torch, x.device, stream, **named) as on:
-        y = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
-        _, ld = _rows(y, "out", d.out)
-        _refuse_overlap(dict(out=y), dict(x=x, w_gate=w_gate, w_up=w_up, w_down=w_down))
+    handle, contexts = _on(torch, (x, w_gate, w_up, w_down) if out is None else (x, w_gate, w_up, w_down, out), stream)
+    with ExitStack() if contexts else _NOTHING as stack:
+        for c in contexts:
+            stack.enter_context(c)
+        if out is None:
+            out, ld = x.new_empty(shape), d.out
+        else:
+            ld = _rows(out, "out", d.out)[1]
+            _refuse_overlap(dict(out=out), dict(x=x, w_gate=w_gate, w_up=w_up, w_down=w_down))
         ws, n = _workspace(torch, d, 0, x.device)
-        rt._check(rt.load_library().nerf_gated_block_forward(ctypes.byref(d), y.data_ptr(), ld, ws.data_ptr(), n, on.stream))
-    return y
+        rt._check(rt.load_library().nerf_gated_block_forward(ctypes.byref(d), out.data_ptr(), ld, ws.data_ptr(), n, handle))
+    return out
 
 
 def gated_block_backward(dy, x, w_gate, w_up, w_down, *, activation: str = "silu",
@@ -249,15 +277,19 @@ def gated_block_backward(dy, x, w_gate, w_up, w_down, *, activation: str = "silu
         if o.shape != like.shape or o.dtype != like.dtype or (k != "dx" and not o.is_contiguous()):
             raise ValueError(f"{k} must be {tuple(like.shape)} {like.dtype}" + (", contiguous" if k != "dx" else ""))
     inputs = dict(dy=dy, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down)
-    with _On(torch, x.device, stream, **{k: v for k, v in inputs.items() if k != "x"}, **given) as on:
+    handle, contexts = _on(torch, (*inputs.values(), *given.values()), stream)
+    with ExitStack() if contexts else _NOTHING as stack:
+        for c in contexts:
+            stack.enter_context(c)
         got = [None if not n else given.get(k) if k in given else
                torch.empty(like.shape, dtype=like.dtype, device=like.device) for k, like, n in zip(names, likes, needs)]
-        _refuse_overlap({k: g for k, g in zip(names, got) if g is not None}, inputs)
+        if given:
+            _refuse_overlap(given, inputs)
         ld_dx = _rows(got[0], "dx", d.width)[1] if got[0] is not None else d.width
         ws, n = _workspace(torch, d, 1, x.device)
         ptr = [None if g is None else g.data_ptr() for g in got]
         rt._check(rt.load_library().nerf_gated_block_backward(ctypes.byref(d), dy.data_ptr(), ld_dy, ptr[0], ld_dx, ptr[1],
-                                                              ptr[2], ptr[3], ws.data_ptr(), n, on.stream))
+                                                              ptr[2], ptr[3], ws.data_ptr(), n, handle))
     return tuple(got)
 
 

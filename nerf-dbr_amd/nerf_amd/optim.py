@@ -7,6 +7,7 @@ with ``config["optimizer"] = "adamw"``.  The formula is torch.optim.AdamW's
 from __future__ import annotations
 
 import ctypes
+from contextlib import ExitStack, nullcontext
 from typing import Optional, Sequence, Union
 
 import numpy as np
@@ -131,6 +132,7 @@ class AdamW:
                 t.exp_avg_scale, t.exp_avg_sq_scale = self.exp_avg_scale[i].data_ptr(), self.exp_avg_sq_scale[i].data_ptr()
             t.numel, t.weight_decay = p.numel(), decay[i]
         self._shapes = [p.shape for p in self.params]
+        self._left_out = False          # the last step's gradients had gaps
         c = rt.AdamWConfig()
         c.beta1, c.beta2, c.eps = float(betas[0]), float(betas[1]), float(eps)
         c.max_norm = 0.0 if max_norm is None else float(max_norm)
@@ -159,45 +161,49 @@ class AdamW:
         overwrites) if one is computed, else None."""
         import torch
 
-        from .operators import _On
+        from .operators import _on
 
         grads = [p.grad for p in self.params] if grads is None else grads
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} gradients needed, got {len(grads)}")
         host, on_device = self._lr(self.lr if lr is None else lr)
-        codes, device, shapes = self._grad, self.device, self._shapes
-        ptr, kind, numel = [], [], self._numels
+        codes, index, shapes = self._grad, self.device.index, self._shapes
+        ptr, kind, none = [], [], []
         for i, g in enumerate(grads):
             if g is None:
+                none.append(i)
                 ptr.append(0)
                 kind.append(0)
                 continue
             k = codes.get(g.dtype)
-            if k is None or g.shape != shapes[i] or not g.is_contiguous() or g.device != device:
+            if k is None or g.shape != shapes[i] or not g.is_contiguous() or g.get_device() != index:
                 raise ValueError(f"gradient {i} {tuple(g.shape)} {g.dtype} on {g.device} must be contiguous, "
-                                 f"{tuple(shapes[i])} and on {device}")
+                                 f"{tuple(shapes[i])} and on {self.device}")
             ptr.append(g.data_ptr())
             kind.append(k)
         col = self._columns
         col["grad"] = ptr
         col["grad_dtype"] = kind
-        none = [i for i, g in enumerate(grads) if g is None]
-        col["numel"] = numel
-        if none:
+        if none or self._left_out:
+            col["numel"] = self._numels
             col["numel"][none] = 0
+            self._left_out = bool(none)
             if not col["numel"].any():
                 raise ValueError("no gradients")
         c = self._config
         c.lr = host
         c.lr_device = None if on_device is None else on_device.data_ptr()
         lib = rt.load_library()
-        with _On(torch, device, stream) as on:
+        handle, contexts = _on(torch, (self._control,), stream)
+        with ExitStack() if contexts else nullcontext() as stack:
+            for x in contexts:
+                stack.enter_context(x)
             n = self._workspace_bytes
             if none and n:    # fewer values can be cut into more, smaller pieces
                 n = max(n, lib.nerf_adamw_workspace(len(ptr), self._table))
-            ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
             rt._check(lib.nerf_adamw_step(ctypes.byref(c), len(ptr), self._table, self._control.data_ptr(),
-                                          None if ws is None else ws.data_ptr(), n, on.stream))
+                                          None if ws is None else ws.data_ptr(), n, handle))
         return self.grad_norm if self._norm else None
 
     @property

@@ -38,6 +38,16 @@ def test_structures_match_header(tmp_path):
         assert int(said[c]) == ctypes.sizeof(py), c
         for name, _ in py._fields_:
             assert int(said[f"{c}.{name}"]) == getattr(py, name).offset, f"{c}.{name}"
+    # the one-pack form of the rotary descriptor: every member where ctypes has it
+    values = list(range(1, 39))
+    d = rt.RotaryDesc.from_buffer_copy(ops._ROTARY.pack(*values))
+    assert ops._ROTARY.size == ctypes.sizeof(rt.RotaryDesc)
+    got = [d.dtype, d.head_dim, d.n_axes, *d.sections, d.shared_ladder, d.interleaved, d.inverse, int(d.base),
+           ctypes.cast(d.frequencies, ctypes.c_void_p).value, d.positions, d.position_dtype, *d.position_stride, d.n_batch,
+           d.n_tokens, d.n_tensors]
+    for t in d.tensor:
+        got += [t.x, t.out, t.heads, *t.x_stride, *t.out_stride]
+    assert got == values[:len(got)] and len(got) == len(values)
 
 
 # ------------------------------------------------------------------------------------------- rotary --
