@@ -451,17 +451,21 @@ int nerf_gated_block_backward(const nerf_block_desc* desc, const void* dy, int64
  *   m = m + (1 - beta1)(g - m), v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * param is the fp32 weight; with model != NULL it is the master of a 16-bit weight, which is
- * written as the rounded new value.  grad is NERF_F32, NERF_BFLOAT16 or NERF_FLOAT16.
- * state_bits 32: exp_avg and exp_avg_sq are fp32 [numel].  state_bits 8: they are e4m3 codes
- * [numel] of m and of sqrt(v), each block of NERF_ADAMW_BLOCK values (counted from the tensor's
- * start, the last one short) times its fp32 scale = absmax / 448 in *_scale; a sqrt(v) > 0 keeps at
- * least the smallest code.  The step itself uses the unrounded new m and v.
+ * written as the rounded new value.  state_bits 32: exp_avg and exp_avg_sq are fp32 [numel].
+ * state_bits 8: they are e4m3 codes [numel] of m and of sqrt(v), each block of NERF_ADAMW_BLOCK
+ * values (counted from the tensor's start, the last one short) times its fp32 scale = absmax / 448 in
+ * *_scale; a sqrt(v) > 0 keeps at least the smallest code.  The step itself uses the unrounded new m
+ * and v.
+ * plan: what a program lays out once for its tensors (their addresses and how they are cut among
+ * workgroups): nerf_adamw_plan writes nerf_adamw_plan_bytes bytes of host memory, and the caller keeps
+ * a copy of them in device memory (16-byte aligned).  grads: host array of n_tensors device addresses,
+ * NULL for a tensor to leave out; grad_dtypes NERF_F32, NERF_BFLOAT16 or NERF_FLOAT16 each.
  * control (device, zeroed once by the caller, one per optimizer): the step count t, which the call
  * advances on the device so that a captured call counts its replays; the gradient norm (max_norm
  * > 0 or NERF_ADAMW_SKIP_NONFINITE) and the steps skipped.  flags: NERF_ADAMW_SKIP_NONFINITE leaves
  * everything as it is when the norm is not finite (counted in control); NERF_ADAMW_WRITE_GRADS
  * stores the clipped gradients.  lr_device (device fp32, or NULL) replaces lr.
- * workspace: nerf_adamw_workspace(n_tensors, tensors, ...) bytes of device memory, 8-byte aligned. */
+ * workspace: nerf_adamw_workspace(plan) bytes of device memory, 8-byte aligned. */
 #define NERF_ADAMW_BLOCK 256
 #define NERF_ADAMW_SKIP_NONFINITE 1
 #define NERF_ADAMW_WRITE_GRADS 2
@@ -471,30 +475,33 @@ typedef struct nerf_adamw_control {
   int32_t skipped;
   float norm;
   float factor;      /* what the gradients were multiplied by */
-  float rate, root;  /* 1 / (1 - beta1^t), sqrt(1 - beta2^t) of the last step */
+  float rate, root;  /* 1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t) of the last step */
   int32_t reserved;
 } nerf_adamw_control;
 typedef struct nerf_adamw_tensor {
   float* param;
-  void* model;       /* 16-bit weight, or NULL */
-  void* grad;
+  void* model;             /* 16-bit weight, or NULL */
   void* exp_avg;
   void* exp_avg_sq;
   float* exp_avg_scale;    /* state_bits 8 */
   float* exp_avg_sq_scale;
   int64_t numel;
   double weight_decay;
-  int32_t model_dtype, grad_dtype;
+  int32_t model_dtype;
+  int32_t reserved;
 } nerf_adamw_tensor;
 typedef struct nerf_adamw_config {
   double lr, beta1, beta2, eps, max_norm;
   const float* lr_device;
-  int32_t state_bits;
   int32_t flags;
+  int32_t reserved;
 } nerf_adamw_config;
-size_t nerf_adamw_workspace(int n_tensors, const nerf_adamw_tensor* tensors);
-int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_adamw_tensor* tensors,
-                    nerf_adamw_control* control, void* workspace, size_t workspace_bytes, void* stream);
+size_t nerf_adamw_plan_bytes(int n_tensors, const nerf_adamw_tensor* tensors, int state_bits); /* 0: refused */
+int nerf_adamw_plan(int n_tensors, const nerf_adamw_tensor* tensors, int state_bits, void* plan);
+size_t nerf_adamw_workspace(const void* plan);
+int nerf_adamw_step(const nerf_adamw_config* config, const void* plan, const void* plan_device,
+                    const void* const* grads, const int32_t* grad_dtypes, nerf_adamw_control* control,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* The trainer's optimizer: NERF_OPT_ADAM (the reference's, default) or NERF_OPT_ADAMW on the
  * trainer's settings (decoupled weight decay on every tensor), with its moments in 32 or 8 bits.

@@ -2,9 +2,10 @@
 //   g = grad * min(1, max_norm / (|grads| + 1e-6))
 //   m = m + (1 - b1)(g - m),  v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// Bound by bytes: 28 per fp32 value with 32-bit moments, 16 + 16 / 256 with 8-bit ones.  The tensors'
-// addresses travel in the kernel arguments (48 tensors a launch), so nothing is uploaded, nothing is
-// kept between calls and a captured call replays as it was made.
+// Bound by bytes: 28 per fp32 value with 32-bit moments, 16 + 16 / 256 with 8-bit ones.  What a program
+// keeps (addresses, which workgroup takes which piece) is laid out once in a plan that lies on the device;
+// a step's gradients travel as addresses in the kernel arguments, 440 tensors a launch, so nothing is
+// uploaded and a captured call replays as it was made.
 #include <cmath>
 #include <cstring>
 
@@ -13,64 +14,72 @@
 namespace nerf {
 namespace {
 
-constexpr int kTensors = 48;   // per launch: 48 x 72 bytes of the 4 KiB of kernel arguments
-struct AdamTensor {
+constexpr int kStep = 1024;    // values a workgroup takes per iteration: 256 threads x 4
+constexpr unsigned kMagic = 0x4e414457u;
+struct Header {
+  unsigned magic;
+  int n, iters, bits;
+  long chunks;
+  long pad;
+};
+struct Entry {
   float* p;
   void* model;
-  void* g;
   void* m;
   void* v;
   float* ms;
   float* vs;
   long n;
-  float decay;      // 1 - lr * weight_decay with the host's lr; with lr_device the kernel forms it
+  unsigned first;   // the tensor's first chunk
+  int wide;         // every address allows vector access
   float wd;
+  int model_dtype;
 };
+// plan: Header, Entry [n], then the tensor of every chunk (unsigned [chunks])
+inline const Entry* entries(const void* plan) { return reinterpret_cast<const Entry*>(static_cast<const char*>(plan) + sizeof(Header)); }
+inline const unsigned* owners(const void* plan, int n) { return reinterpret_cast<const unsigned*>(entries(plan) + n); }
+
+constexpr int kGrads = 440;    // gradients per launch: 3.5 of the 4 KiB of kernel arguments
 struct AdamArgs {
-  AdamTensor t[kTensors];
-  unsigned first[kTensors];   // the tensor's first chunk in this launch
-  int n_tensors, iters, flags;
-  unsigned char wide[kTensors];   // every address allows vector access
+  const Entry* t;
+  const unsigned* owner;
   const nerf_adamw_control* ctl;
   const float* lr_dev;
-  float lr, b1c, b2, b2c, eps;   // b1c = 1 - beta1, b2c = 1 - beta2
+  unsigned chunk0;             // the launch's first chunk and tensor
+  int tensor0, iters, flags;
+  float lr, b1c, b2, b2c, eps; // b1c = 1 - beta1, b2c = 1 - beta2
+  const void* g[kGrads];
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
-constexpr int kStep = 1024;    // values a workgroup takes per iteration: 256 threads x 4
 
-// The tensor that a chunk belongs to: the last one whose first chunk is not behind it.
-__device__ __forceinline__ int find(const AdamArgs& a, unsigned chunk) {
-  int lo = 0, hi = a.n_tensors - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.first[mid] <= chunk) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
+// Addresses read from memory are generic to the compiler; these are global, and flat accesses would count
+// in two wait counters.
+#define NERF_GLOBAL __attribute__((address_space(1)))
+template <typename T>
+__device__ __forceinline__ NERF_GLOBAL T* global(void* p) { return (NERF_GLOBAL T*)(T*)p; }
 
 template <typename T>
-struct alignas(sizeof(T) * 4) Quad {
-  T v[4];
+struct Quad {
+  typedef T type __attribute__((ext_vector_type(4)));
 };
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, long i, long n, bool wide, float out[4]) {
+__device__ __forceinline__ void load4(const NERF_GLOBAL T* p, long i, long n, bool wide, float out[4]) {
   if (wide && i + 4 <= n) {
-    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(p + i);
+    const typename Quad<T>::type q = *(const NERF_GLOBAL typename Quad<T>::type*)(p + i);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = float(q.v[k]);
+    for (int k = 0; k < 4; ++k) out[k] = float(q[k]);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k) out[k] = i + k < n ? float(p[i + k]) : 0.0f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, long i, long n, bool wide, const float in[4]) {
+__device__ __forceinline__ void store4(NERF_GLOBAL T* p, long i, long n, bool wide, const float in[4]) {
   if (wide && i + 4 <= n) {
-    Quad<T> q;
+    typename Quad<T>::type q;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) q.v[k] = T(in[k]);
-    *reinterpret_cast<Quad<T>*>(p + i) = q;
+    for (int k = 0; k < 4; ++k) q[k] = T(in[k]);
+    *(NERF_GLOBAL typename Quad<T>::type*)(p + i) = q;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -78,9 +87,9 @@ __device__ __forceinline__ void store4(T* p, long i, long n, bool wide, const fl
   }
 }
 // four e4m3 codes (OCP, the hardware's conversion) as one word
-__device__ __forceinline__ void load_codes(const unsigned char* p, long i, long n, bool wide, float out[4]) {
+__device__ __forceinline__ void load_codes(const NERF_GLOBAL unsigned char* p, long i, long n, bool wide, float out[4]) {
   unsigned w = 0;
-  if (wide && i + 4 <= n) w = *reinterpret_cast<const unsigned*>(p + i);
+  if (wide && i + 4 <= n) w = *(const NERF_GLOBAL unsigned*)(p + i);
   else
     for (int k = 0; k < 4; ++k)
       if (i + k < n) w |= unsigned(p[i + k]) << (8 * k);
@@ -89,8 +98,8 @@ __device__ __forceinline__ void load_codes(const unsigned char* p, long i, long 
   out[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
   out[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
 }
-__device__ __forceinline__ void store_codes(unsigned char* p, long i, long n, bool wide, unsigned w) {
-  if (wide && i + 4 <= n) *reinterpret_cast<unsigned*>(p + i) = w;
+__device__ __forceinline__ void store_codes(NERF_GLOBAL unsigned char* p, long i, long n, bool wide, unsigned w) {
+  if (wide && i + 4 <= n) *(NERF_GLOBAL unsigned*)(p + i) = w;
   else
     for (int k = 0; k < 4; ++k)
       if (i + k < n) p[i + k] = (unsigned char)(w >> (8 * k));
@@ -111,13 +120,17 @@ __device__ __forceinline__ double pow_steps(double b, int t) {   // b^t, t > 0, 
 template <typename G>
 __global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part) {
   __shared__ double red[4];
-  const int k = find(a, blockIdx.x);
-  const AdamTensor& t = a.t[k];
-  long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
+  const unsigned chunk = a.chunk0 + blockIdx.x;
+  const unsigned k = a.owner[chunk];
+  const Entry& t = a.t[k];
+  const NERF_GLOBAL G* grad = global<G>(const_cast<void*>(a.g[k - a.tensor0]));
+  const bool wide = (uintptr_t(grad) & (4 * sizeof(G) - 1)) == 0;
+  const long n = grad ? t.n : 0;
+  long i = (long(chunk - t.first) * a.iters) * kStep + threadIdx.x * 4;
   double s = 0.0;
-  for (int it = 0; it < a.iters && i < t.n; ++it, i += kStep) {
+  for (int it = 0; it < a.iters && i < n; ++it, i += kStep) {
     float g[4];
-    load4(static_cast<const G*>(t.g), i, t.n, a.wide[k], g);
+    load4(grad, i, n, wide, g);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s += double(g[j]) * double(g[j]);
   }
@@ -125,7 +138,7 @@ __global__ __launch_bounds__(256) void norm_kernel(AdamArgs a, double* part) {
   for (int o = 32; o > 0; o >>= 1) s += __shfl_down(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+  if (threadIdx.x == 0) part[chunk] = red[0] + red[1] + red[2] + red[3];
 }
 
 // One workgroup: the norm from the partials, added in order (it does not depend on timing), the step
@@ -156,35 +169,45 @@ __global__ __launch_bounds__(1024) void prepare_kernel(nerf_adamw_control* c, co
   const int step = c->steps + 1;
   c->steps = step;
   c->rate = float(1.0 / (1.0 - pow_steps(b1, step)));
-  c->root = float(sqrt(1.0 - pow_steps(b2, step)));
+  c->root = float(1.0 / sqrt(1.0 - pow_steps(b2, step)));
+}
+
+// x / scale correctly rounded, for |x| <= 448 scale: Markstein's step on the correctly rounded reciprocal
+// (q + (x - q scale) inv, each an fma), where nothing it forms is subnormal; codes are decided on the
+// quotient itself, so an approximate one would move a value in ten million to the next code.
+__device__ __forceinline__ float quotient(float x, float scale, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, scale, x), inv, q);
 }
 
 template <typename G, typename M, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs a) {
-  const int k = find(a, blockIdx.x);
-  const AdamTensor& t = a.t[k];
-  const bool wide = a.wide[k];
-  if (!a.ctl->apply) return;
+  const unsigned chunk = a.chunk0 + blockIdx.x;
+  const unsigned k = a.owner[chunk];
+  const Entry& t = a.t[k];
+  NERF_GLOBAL G* grad = global<G>(const_cast<void*>(a.g[k - a.tensor0]));
+  const bool wide = t.wide && (uintptr_t(grad) & (4 * sizeof(G) - 1)) == 0;
+  if (!a.ctl->apply || !grad) return;
   const float factor = a.ctl->factor, root = a.ctl->root;
   float lr = a.lr;
   // (a global load: a plain one would be merged with the argument's into one through a flat address)
-  if (a.lr_dev) lr = *(const __attribute__((address_space(1))) float*)a.lr_dev;
-  const float decay = a.lr_dev ? 1.0f - lr * t.wd : t.decay, rate = lr * a.ctl->rate;
-  long i = (long(blockIdx.x - a.first[k]) * a.iters) * kStep + threadIdx.x * 4;
+  if (a.lr_dev) lr = *(const NERF_GLOBAL float*)a.lr_dev;
+  const float decay = 1.0f - lr * t.wd, rate = lr * a.ctl->rate;
+  long i = (long(chunk - t.first) * a.iters) * kStep + threadIdx.x * 4;
   for (int it = 0; it < a.iters; ++it, i += kStep) {
     if (BITS == 32 && i >= t.n) break;
     if (BITS == 8 && i - (threadIdx.x & 63) * 4 >= t.n) break;   // uniform in a wave: its block is behind the end
     float g[4], p[4], m[4], v[4], r[4];
-    load4(static_cast<const G*>(t.g), i, t.n, wide, g);
-    load4(t.p, i, t.n, wide, p);
+    load4(grad, i, t.n, wide, g);
+    load4(global<float>(t.p), i, t.n, wide, p);
     const long block = i >> 8;    // the wave's 256 values are one block
     if (BITS == 32) {
-      load4(static_cast<const float*>(t.m), i, t.n, wide, m);
-      load4(static_cast<const float*>(t.v), i, t.n, wide, v);
+      load4(global<float>(t.m), i, t.n, wide, m);
+      load4(global<float>(t.v), i, t.n, wide, v);
     } else {
-      load_codes(static_cast<const unsigned char*>(t.m), i, t.n, wide, m);
-      load_codes(static_cast<const unsigned char*>(t.v), i, t.n, wide, v);
-      const float ms = t.ms[block], vs = t.vs[block];
+      load_codes(global<unsigned char>(t.m), i, t.n, wide, m);
+      load_codes(global<unsigned char>(t.v), i, t.n, wide, v);
+      const float ms = global<float>(t.ms)[block], vs = global<float>(t.vs)[block];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         m[j] *= ms;
@@ -198,42 +221,52 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs a) {
       m[j] += (g[j] - m[j]) * a.b1c;
       v[j] = v[j] * a.b2 + g[j] * g[j] * a.b2c;
       r[j] = sqrtf(v[j]);
-      p[j] = p[j] * decay - rate * m[j] / (r[j] / root + a.eps);
+      p[j] = p[j] * decay - rate * m[j] * __builtin_amdgcn_rcpf(r[j] * root + a.eps);   // 1 ulp
     }
-    if (a.flags & NERF_ADAMW_WRITE_GRADS) store4(static_cast<G*>(t.g), i, t.n, wide, g);
-    store4(t.p, i, t.n, wide, p);
-    if (sizeof(M) == 2) store4(static_cast<M*>(t.model), i, t.n, wide, p);
+    if (a.flags & NERF_ADAMW_WRITE_GRADS) store4(grad, i, t.n, wide, g);
+    store4(global<float>(t.p), i, t.n, wide, p);
+    if (sizeof(M) == 2) store4(global<M>(t.model), i, t.n, wide, p);
     if (BITS == 32) {
-      store4(static_cast<float*>(t.m), i, t.n, wide, m);
-      store4(static_cast<float*>(t.v), i, t.n, wide, v);
+      store4(global<float>(t.m), i, t.n, wide, m);
+      store4(global<float>(t.v), i, t.n, wide, v);
     } else {
       // values behind the tensor's end were loaded as zeros: they do not raise the block's maximum
       const float top = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
       const float rtop = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
-      const float ms = top / 448.0f, vs = rtop / 448.0f;
+      const float ms = top * (1.0f / 448.0f), vs = rtop * (1.0f / 448.0f);
       unsigned mw = 0, vw = 0;
-      if (ms > 0.0f) {
+      if (ms > 1e-20f) {
+        const float inv = 1.0f / ms;
+        mw = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(m[0], ms, inv), quotient(m[1], ms, inv), mw, false);
+        mw = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(m[2], ms, inv), quotient(m[3], ms, inv), mw, true);
+      } else if (ms > 0.0f) {
         mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] / ms, m[1] / ms, mw, false);
         mw = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] / ms, m[3] / ms, mw, true);
       }
       if (vs > 0.0f) {
-        vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[0] / vs, r[1] / vs, vw, false);
-        vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[2] / vs, r[3] / vs, vw, true);
+        if (vs > 1e-20f) {
+          const float inv = 1.0f / vs;
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(r[0], vs, inv), quotient(r[1], vs, inv), vw, false);
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(r[2], vs, inv), quotient(r[3], vs, inv), vw, true);
+        } else {
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[0] / vs, r[1] / vs, vw, false);
+          vw = __builtin_amdgcn_cvt_pk_fp8_f32(r[2] / vs, r[3] / vs, vw, true);
+        }
         // a root that is not zero keeps the smallest code: m / (0 + eps) of a value whose v was
         // rounded away would be a step of any size
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (r[j] > 0.0f && ((vw >> (8 * j)) & 0xffu) == 0) vw |= 1u << (8 * j);
       }
-      store_codes(static_cast<unsigned char*>(t.m), i, t.n, wide, mw);
-      store_codes(static_cast<unsigned char*>(t.v), i, t.n, wide, vw);
-      if ((threadIdx.x & 63) == 0) t.ms[block] = ms, t.vs[block] = vs;
+      store_codes(global<unsigned char>(t.m), i, t.n, wide, mw);
+      store_codes(global<unsigned char>(t.v), i, t.n, wide, vw);
+      if ((threadIdx.x & 63) == 0) global<float>(t.ms)[block] = ms, global<float>(t.vs)[block] = vs;
     }
   }
 }
 
-// Chunks of a call: as many as fill the machine with one iteration each, at most 8 iterations (32 KiB
-// of fp32 per array) so that a workgroup's fixed cost (tensor search, bias corrections) is spread.
+// As many chunks as fill the machine with one iteration each, at most 8 iterations (32 KiB of fp32 per
+// array) so that a workgroup's fixed cost is spread.
 int iterations(int n, const nerf_adamw_tensor* t) {
   long steps = 0;
   for (int i = 0; i < n; ++i) steps += (t[i].numel + kStep - 1) / kStep;
@@ -254,33 +287,34 @@ void launch_step(const AdamArgs& a, int model, int bits, unsigned grid, hipStrea
   else launch_step<G, float>(a, bits, grid, s);
 }
 
-int check(const nerf_adamw_config* c, int n, const nerf_adamw_tensor* t) {
-  if (!c || (n > 0 && !t) || n < 0) return set_error(NERF_E_INVALID, "nerf_adamw_step: null argument");
-  if (!(c->lr >= 0.0) || !(c->beta1 >= 0.0 && c->beta1 < 1.0) || !(c->beta2 >= 0.0 && c->beta2 < 1.0) || !(c->eps >= 0.0))
-    return set_error(NERF_E_INVALID, "nerf_adamw_step: lr %g, betas %g %g, eps %g", c->lr, c->beta1, c->beta2, c->eps);
-  if (c->state_bits != 32 && c->state_bits != 8) return set_error(NERF_E_INVALID, "nerf_adamw_step: state_bits %d (32 or 8)", c->state_bits);
-  if (c->flags & ~(NERF_ADAMW_SKIP_NONFINITE | NERF_ADAMW_WRITE_GRADS)) return set_error(NERF_E_INVALID, "nerf_adamw_step: flags %d", c->flags);
+int check(int n, const nerf_adamw_tensor* t, int bits, long* total) {
+  if (n < 1 || !t) return set_error(NERF_E_INVALID, "nerf_adamw_plan: %d tensors", n);
+  if (bits != 32 && bits != 8) return set_error(NERF_E_INVALID, "nerf_adamw_plan: state_bits %d (32 or 8)", bits);
   bool any = false;
   for (int i = 0; i < n; ++i) {
     const nerf_adamw_tensor& x = t[i];
     any = any || x.numel > 0;
-    if (x.numel < 0 || x.numel > (1L << 40)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has %ld values", i, long(x.numel));
+    if (x.numel < 0 || x.numel > (1L << 40)) return set_error(NERF_E_INVALID, "nerf_adamw_plan: tensor %d has %ld values", i, long(x.numel));
     if (x.numel == 0) continue;
-    if (!x.param || !x.grad || !x.exp_avg || !x.exp_avg_sq || (c->state_bits == 8 && (!x.exp_avg_scale || !x.exp_avg_sq_scale)))
-      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has a null store", i);
-    if (x.grad_dtype != NERF_F32 && x.grad_dtype != NERF_BFLOAT16 && x.grad_dtype != NERF_FLOAT16)
-      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has gradient dtype %d", i, x.grad_dtype);
+    if (!x.param || !x.exp_avg || !x.exp_avg_sq || (bits == 8 && (!x.exp_avg_scale || !x.exp_avg_sq_scale)))
+      return set_error(NERF_E_INVALID, "nerf_adamw_plan: tensor %d has a null store", i);
     if (x.model && x.model_dtype != NERF_BFLOAT16 && x.model_dtype != NERF_FLOAT16)
-      return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has model dtype %d", i, x.model_dtype);
-    if (!(x.weight_decay >= 0.0)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d has weight decay %g", i, x.weight_decay);
+      return set_error(NERF_E_INVALID, "nerf_adamw_plan: tensor %d has model dtype %d", i, x.model_dtype);
+    if (!(x.weight_decay >= 0.0)) return set_error(NERF_E_INVALID, "nerf_adamw_plan: tensor %d has weight decay %g", i, x.weight_decay);
     uintptr_t four = uintptr_t(x.param) | uintptr_t(x.exp_avg_scale) | uintptr_t(x.exp_avg_sq_scale);
-    uintptr_t two = uintptr_t(x.model);
-    (x.grad_dtype == NERF_F32 ? four : two) |= uintptr_t(x.grad);
-    if (c->state_bits == 32) four |= uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq);
-    if ((four & 3) || (two & 1)) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d is not aligned to its type", i);
+    if (bits == 32) four |= uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq);
+    if ((four & 3) || (uintptr_t(x.model) & 1)) return set_error(NERF_E_INVALID, "nerf_adamw_plan: tensor %d is not aligned to its type", i);
   }
-  if (!any) return set_error(NERF_E_INVALID, "nerf_adamw_step: no values to step");
+  if (!any) return set_error(NERF_E_INVALID, "nerf_adamw_plan: no values to step");
+  const int iters = iterations(n, t);
+  *total = 0;
+  for (int i = 0; i < n; ++i) *total += chunks(t[i], iters);
+  if (*total > 0x7fffffffL) return set_error(NERF_E_INVALID, "nerf_adamw_plan: too many values");
   return NERF_OK;
+}
+const Header* header(const void* plan) {
+  const Header* h = static_cast<const Header*>(plan);
+  return h && !(uintptr_t(plan) & 7) && h->magic == kMagic ? h : nullptr;
 }
 
 }  // namespace
@@ -290,83 +324,106 @@ using namespace nerf;
 
 extern "C" {
 
-size_t nerf_adamw_workspace(int n_tensors, const nerf_adamw_tensor* tensors) {
-  if (n_tensors <= 0 || !tensors) return 0;
-  const int iters = iterations(n_tensors, tensors);
-  long n = 0;
-  for (int i = 0; i < n_tensors; ++i) n += chunks(tensors[i], iters);
-  return sizeof(double) * size_t(n);
+size_t nerf_adamw_plan_bytes(int n_tensors, const nerf_adamw_tensor* tensors, int state_bits) {
+  long total = 0;
+  if (check(n_tensors, tensors, state_bits, &total) != NERF_OK) return 0;
+  return sizeof(Header) + sizeof(Entry) * size_t(n_tensors) + (sizeof(unsigned) * size_t(total) + 15) / 16 * 16;
 }
 
-int nerf_adamw_step(const nerf_adamw_config* config, int n_tensors, const nerf_adamw_tensor* tensors,
-                    nerf_adamw_control* control, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check(config, n_tensors, tensors);
+int nerf_adamw_plan(int n_tensors, const nerf_adamw_tensor* tensors, int state_bits, void* plan) {
+  long total = 0;
+  const int rc = check(n_tensors, tensors, state_bits, &total);
   if (rc != NERF_OK) return rc;
-  if (!control) return set_error(NERF_E_INVALID, "nerf_adamw_step: null control");
-  const bool clip = config->max_norm > 0.0, norm = clip || (config->flags & NERF_ADAMW_SKIP_NONFINITE);
-  if (norm && (workspace_bytes < nerf_adamw_workspace(n_tensors, tensors) ||
-               (workspace_bytes && (!workspace || (uintptr_t(workspace) & 7)))))
-    return set_error(NERF_E_INVALID, "nerf_adamw_step: workspace of %zu bytes, %zu needed (8-byte aligned)", workspace_bytes,
-                     nerf_adamw_workspace(n_tensors, tensors));
-  const hipStream_t s = (hipStream_t)stream;
+  if (!plan || (uintptr_t(plan) & 7)) return set_error(NERF_E_INVALID, "nerf_adamw_plan: null or unaligned plan");
   const int iters = iterations(n_tensors, tensors);
+  *static_cast<Header*>(plan) = Header{kMagic, n_tensors, iters, state_bits, total, 0};
+  Entry* e = const_cast<Entry*>(entries(plan));
+  unsigned* owner = const_cast<unsigned*>(owners(plan, n_tensors));
+  unsigned first = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    const nerf_adamw_tensor& x = tensors[i];
+    const int wide = !(uintptr_t(x.param) & 15) && !(uintptr_t(x.model) & 7) &&
+                     !((uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq)) & (state_bits == 32 ? 15 : 3));
+    e[i] = Entry{x.param, x.model, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, long(x.numel), first, wide,
+                 float(x.weight_decay), x.model ? x.model_dtype : NERF_F32};
+    for (long c = chunks(x, iters); c > 0; --c) owner[first++] = unsigned(i);
+  }
+  return NERF_OK;
+}
+
+size_t nerf_adamw_workspace(const void* plan) {
+  const Header* h = header(plan);
+  return h ? sizeof(double) * size_t(h->chunks) : 0;
+}
+
+int nerf_adamw_step(const nerf_adamw_config* c, const void* plan, const void* plan_device, const void* const* grads,
+                    const int32_t* grad_dtypes, nerf_adamw_control* control, void* workspace, size_t workspace_bytes, void* stream) {
+  static const char* who = "nerf_adamw_step";
+  const Header* h = header(plan);
+  if (!c || !h || !grads || !grad_dtypes) return set_error(NERF_E_INVALID, "%s: null argument or no plan", who);
+  if (!plan_device || (uintptr_t(plan_device) & 15)) return set_error(NERF_E_INVALID, "%s: null or unaligned plan_device", who);
+  if (!control || (uintptr_t(control) & 3)) return set_error(NERF_E_INVALID, "%s: null or unaligned control", who);
+  if (!(c->lr >= 0.0) || !(c->beta1 >= 0.0 && c->beta1 < 1.0) || !(c->beta2 >= 0.0 && c->beta2 < 1.0) || !(c->eps >= 0.0) ||
+      !(c->max_norm == c->max_norm))
+    return set_error(NERF_E_INVALID, "%s: lr %g, betas %g %g, eps %g, max_norm %g", who, c->lr, c->beta1, c->beta2, c->eps, c->max_norm);
+  if (c->flags & ~(NERF_ADAMW_SKIP_NONFINITE | NERF_ADAMW_WRITE_GRADS)) return set_error(NERF_E_INVALID, "%s: flags %d", who, c->flags);
+  bool any = false;
+  const Entry* e = entries(plan);
+  for (int i = 0; i < h->n; ++i) {
+    if (!grads[i]) continue;
+    if (grad_dtypes[i] != NERF_F32 && grad_dtypes[i] != NERF_BFLOAT16 && grad_dtypes[i] != NERF_FLOAT16)
+      return set_error(NERF_E_INVALID, "%s: gradient %d has dtype %d", who, i, grad_dtypes[i]);
+    if (uintptr_t(grads[i]) & (grad_dtypes[i] == NERF_F32 ? 3 : 1)) return set_error(NERF_E_INVALID, "%s: gradient %d is not aligned to its type", who, i);
+    any = any || e[i].n > 0;
+  }
+  if (!any) return set_error(NERF_E_INVALID, "%s: no gradients", who);
+  const bool clip = c->max_norm > 0.0, norm = clip || (c->flags & NERF_ADAMW_SKIP_NONFINITE);
+  if (norm && (workspace_bytes < nerf_adamw_workspace(plan) || !workspace || (uintptr_t(workspace) & 7)))
+    return set_error(NERF_E_INVALID, "%s: workspace of %zu bytes, %zu needed (8-byte aligned)", who, workspace_bytes, nerf_adamw_workspace(plan));
+  const hipStream_t s = (hipStream_t)stream;
   double* part = static_cast<double*>(workspace);
-  // launches of up to kTensors tensors of the same types, in order; pass 0 sums squares, pass 1 steps
+  AdamArgs a{};
+  a.t = entries(plan_device), a.owner = owners(plan_device, h->n);
+  a.ctl = control, a.lr_dev = c->lr_device, a.iters = h->iters, a.flags = c->flags;
+  a.lr = float(c->lr), a.b1c = float(1.0 - c->beta1), a.b2 = float(c->beta2), a.b2c = float(1.0 - c->beta2), a.eps = float(c->eps);
+  const auto failed = [&]() -> int {
+    const hipError_t x = hipGetLastError();
+    return x == hipSuccess ? NERF_OK : set_error(NERF_E_HIP, "%s: %s", who, hipGetErrorString(x));
+  };
+  // pass 0 sums squares, pass 1 steps: a launch for each run of tensors of the same types
   for (int pass = norm ? 0 : 1; pass < 2; ++pass) {
-    AdamArgs a;
-    std::memset(&a, 0, sizeof a);
-    int grad = -1, model = -1;
-    unsigned grid = 0;
-    long done = 0;      // partials of the launches before
-    auto launched = [&]() -> int {
-      const hipError_t e = hipGetLastError();
-      return e == hipSuccess ? NERF_OK : set_error(NERF_E_HIP, "nerf_adamw_step: %s", hipGetErrorString(e));
-    };
-    auto flush = [&]() -> int {
-      if (a.n_tensors == 0) return NERF_OK;
-      if (pass == 0) {
-        if (grad == NERF_F32) hipLaunchKernelGGL((norm_kernel<float>), dim3(grid), dim3(256), 0, s, a, part + done);
-        else if (grad == NERF_BFLOAT16) hipLaunchKernelGGL((norm_kernel<__bf16>), dim3(grid), dim3(256), 0, s, a, part + done);
-        else hipLaunchKernelGGL((norm_kernel<_Float16>), dim3(grid), dim3(256), 0, s, a, part + done);
-      } else {
-        if (grad == NERF_F32) launch_step<float>(a, model, config->state_bits, grid, s);
-        else if (grad == NERF_BFLOAT16) launch_step<__bf16>(a, model, config->state_bits, grid, s);
-        else launch_step<_Float16>(a, model, config->state_bits, grid, s);
-      }
-      done += grid;
-      a.n_tensors = 0, grid = 0;
-      return launched();
-    };
+    int rc;
     if (pass == 1) {
-      long n = 0;
-      if (norm)
-        for (int i = 0; i < n_tensors; ++i) n += chunks(tensors[i], iters);
-      hipLaunchKernelGGL(prepare_kernel, dim3(1), dim3(1024), 0, s, control, (const double*)part, n, float(clip ? config->max_norm : 0.0),
-                         config->beta1, config->beta2, config->flags & NERF_ADAMW_SKIP_NONFINITE);
-      if ((rc = launched()) != NERF_OK) return rc;
+      hipLaunchKernelGGL(prepare_kernel, dim3(1), dim3(1024), 0, s, control, (const double*)part, norm ? h->chunks : 0L,
+                         float(clip ? c->max_norm : 0.0), c->beta1, c->beta2, c->flags & NERF_ADAMW_SKIP_NONFINITE);
+      if ((rc = failed()) != NERF_OK) return rc;
     }
-    a.iters = iters, a.flags = config->flags, a.ctl = control, a.lr_dev = config->lr_device;
-    a.lr = float(config->lr), a.b1c = float(1.0 - config->beta1), a.b2 = float(config->beta2), a.b2c = float(1.0 - config->beta2);
-    a.eps = float(config->eps);
-    for (int i = 0; i < n_tensors; ++i) {
-      const nerf_adamw_tensor& x = tensors[i];
-      if (x.numel == 0) continue;
-      const int md = x.model ? x.model_dtype : NERF_F32;
-      const long c = chunks(x, iters);
-      if (c > 0x40000000L) return set_error(NERF_E_INVALID, "nerf_adamw_step: tensor %d is too large", i);
-      if (a.n_tensors == kTensors || x.grad_dtype != grad || md != model || grid + c > 0x7fffffffL)
-        if ((rc = flush()) != NERF_OK) return rc;
-      grad = x.grad_dtype, model = md;
-      const int k = a.n_tensors++;
-      a.t[k] = AdamTensor{x.param, x.model, x.grad, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, long(x.numel),
-                          float(1.0 - config->lr * x.weight_decay), float(x.weight_decay)};
-      a.first[k] = grid;
-      const uintptr_t gsize = x.grad_dtype == NERF_F32 ? 15 : 7;
-      a.wide[k] = !(uintptr_t(x.param) & 15) && !(uintptr_t(x.grad) & gsize) && !(uintptr_t(x.model) & 7) &&
-                  !((uintptr_t(x.exp_avg) | uintptr_t(x.exp_avg_sq)) & (config->state_bits == 32 ? 15 : 3));
-      grid += unsigned(c);
+    for (int i = 0; i < h->n;) {
+      int grad = -1, model = -1, n = 0;
+      for (; i + n < h->n && n < kGrads; ++n) {
+        const int k = i + n;
+        if (e[k].n && grads[k]) {
+          if (grad >= 0 && (grad != grad_dtypes[k] || (pass == 1 && model != e[k].model_dtype))) break;
+          grad = grad_dtypes[k], model = e[k].model_dtype;
+        }
+        a.g[n] = grads[k];
+      }
+      const unsigned end = i + n < h->n ? e[i + n].first : unsigned(h->chunks), grid = end - e[i].first;
+      a.chunk0 = e[i].first, a.tensor0 = i;
+      i += n;
+      if (!grid) continue;
+      if (grad < 0) grad = NERF_F32, model = NERF_F32;    // nothing but gaps: their partials are zeros
+      if (pass == 0) {
+        if (grad == NERF_F32) hipLaunchKernelGGL((norm_kernel<float>), dim3(grid), dim3(256), 0, s, a, part);
+        else if (grad == NERF_BFLOAT16) hipLaunchKernelGGL((norm_kernel<__bf16>), dim3(grid), dim3(256), 0, s, a, part);
+        else hipLaunchKernelGGL((norm_kernel<_Float16>), dim3(grid), dim3(256), 0, s, a, part);
+      } else {
+        if (grad == NERF_F32) launch_step<float>(a, model, h->bits, grid, s);
+        else if (grad == NERF_BFLOAT16) launch_step<__bf16>(a, model, h->bits, grid, s);
+        else launch_step<_Float16>(a, model, h->bits, grid, s);
+      }
+      if ((rc = failed()) != NERF_OK) return rc;
     }
-    if ((rc = flush()) != NERF_OK) return rc;
   }
   return NERF_OK;
 }

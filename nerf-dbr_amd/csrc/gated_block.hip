@@ -219,10 +219,17 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long ld, long ro
 
 // ----------------------------------------------------------------------------------------- few rows --
 // Up to 64 rows (a token of each of a few sequences): the weights' bytes are the cost, so they go from
-// memory to fragments without LDS.  A workgroup owns 16 weight rows (of Wg and of Wu); its waves take
-// every WAVES-th step of k, so that together they read whole lines of each row, and add up their
-// accumulators in LDS in wave order.  fp32 runs on the f32 matrix instruction at full precision: at a few
-// rows it still outruns memory (4 x 32 cycles a KiB of weights a SIMD).
+// memory to fragments without LDS.  The waves of a workgroup take every WAVES-th step of k, so that
+// together they read whole lines of each weight row, and add up their accumulators in LDS in wave order.
+// A fragment's 16 rows are, by what fills the machine:
+//   kRows    16 rows of w;
+//   kGate    8 rows of Wg and the same 8 of Wu: twice the workgroups of 16 and 16, and an accumulator
+//            fewer;
+//   kHalves  8 rows of w and the two halves of k: the fragment's rows 8.. hold the second half and meet
+//            the rows of x, repeated in columns 8.. with their second half; up to 8 rows of x.
+// fp32 runs on the f32 matrix instruction at full precision: at a few rows it still outruns memory
+// (4 x 32 cycles a KiB of weights a SIMD).
+enum { kRows, kGate, kHalves };
 template <typename T>
 struct FewStep {   // 16 bytes of k a lane: 32 values of k a step
   static constexpr int kK = 32, kLane = 8;
@@ -260,82 +267,91 @@ struct Few {
   long k;
   void* out;
 };
-// GATE: out = act(x w^T) (x w2^T), else out = x w^T
-template <typename T, int NI, int WAVES, bool WHOLE, bool GATE>
+template <typename T, int NI, int WAVES, bool WHOLE, int MODE>
 __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
   typedef FewStep<T> S;
-  constexpr int kU = 4, M = GATE ? 2 : 1;
-  __shared__ f32x4_t red[WAVES][M * NI][64];
+  constexpr int kU = NI == 1 ? 8 : 4, kCols = MODE == kRows ? 16 : 8;
+  __shared__ f32x4_t red[WAVES][NI][64];
   const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, e = l & 15, g = l >> 4;
-  const int j0 = blockIdx.x * 16;
-  const long wr = min(j0 + e, p.n - 1);
-  const T* w = static_cast<const T*>(p.w) + wr * p.ld_w;
-  const T* w2 = GATE ? static_cast<const T*>(p.w2) + wr * p.ld_w2 : nullptr;
+  const int j0 = blockIdx.x * kCols;
+  const long wr = min(j0 + (e & (kCols - 1)), p.n - 1);
+  // kHalves: lanes of the second half start at k_off and end at k; the first half is the longer one
+  const long half = MODE == kHalves ? ((p.k + 1) / 2 + S::kK - 1) / S::kK * S::kK : p.k;
+  const bool second = MODE == kHalves && e >= 8;
+  const long k_off = second ? half : 0, k_end = second ? p.k : half < p.k ? half : p.k;
+  const long k_all = MODE == kHalves ? (p.k > half ? p.k - half : 0) : p.k;   // steps up to here are whole for every lane
+  const bool up = MODE == kGate && e >= 8;
+  const T* w = static_cast<const T*>(up ? p.w2 : p.w) + wr * (up ? p.ld_w2 : p.ld_w) + k_off + g * S::kLane;
   const T* x[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) x[i] = static_cast<const T*>(p.x) + long(min(i * 16 + e, p.rows - 1)) * p.ld_x;
-  f32x4_t acc[M][NI] = {};
+  for (int i = 0; i < NI; ++i) {
+    const int row = MODE == kHalves ? e & 7 : i * 16 + e;
+    x[i] = static_cast<const T*>(p.x) + long(min(row, p.rows - 1)) * p.ld_x + k_off + g * S::kLane;
+  }
+  f32x4_t acc[NI] = {};
   const auto steps = [&](long k0, auto count, auto checked) {
     constexpr int U = decltype(count)::value;
-    const long k = decltype(checked)::value ? p.k : 0x7fffffffffffffffL;
-    typename S::Data fw[U][M], fx[U][NI];
+    const long k = decltype(checked)::value ? k_end - k_off - g * S::kLane : 0x7fffffffffffffffL;
+    typename S::Data fw[U], fx[U][NI];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long at = k0 + u * WAVES * S::kK + g * S::kLane;
-      fw[u][0] = few_load<T, WHOLE>(w, at, k);
-      if (GATE) fw[u][M - 1] = few_load<T, WHOLE>(w2, at, k);
+      const long at = k0 + u * WAVES * S::kK;
+      fw[u] = few_load<T, WHOLE>(w, at, k);
 #pragma unroll
       for (int i = 0; i < NI; ++i) fx[u][i] = few_load<T, WHOLE>(x[i], at, k);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int i = 0; i < NI; ++i) acc[m][i] = S::mma(fw[u][m], fx[u][i], acc[m][i]);
+      for (int i = 0; i < NI; ++i) acc[i] = S::mma(fw[u], fx[u][i], acc[i]);
   };
   long k0 = long(wave) * S::kK;
-  if (WHOLE)
-    for (; k0 + ((kU - 1) * WAVES + 1) * S::kK <= p.k; k0 += kU * WAVES * S::kK)
+  if (WHOLE) {
+    for (; k0 + ((kU - 1) * WAVES + 1) * S::kK <= k_all; k0 += kU * WAVES * S::kK)
       steps(k0, std::integral_constant<int, kU>{}, std::false_type{});
-  for (; k0 < p.k; k0 += WAVES * S::kK) steps(k0, std::integral_constant<int, 1>{}, std::true_type{});
+    for (; k0 + (WAVES + 1) * S::kK <= k_all; k0 += 2 * WAVES * S::kK)
+      steps(k0, std::integral_constant<int, 2>{}, std::false_type{});
+  }
+  for (; k0 < half; k0 += WAVES * S::kK) steps(k0, std::integral_constant<int, 1>{}, std::true_type{});
 #pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int i = 0; i < NI; ++i) red[wave][m * NI + i][l] = acc[m][i];
+  for (int i = 0; i < NI; ++i) red[wave][i][l] = acc[i];
   __syncthreads();
   if (wave >= NI) return;
   const int i = wave;
-  f32x4_t a = red[0][i][l], b = red[0][(M - 1) * NI + i][l];
+  // a lane holds rows 4 g .. 4 g + 3 of the fragment for column e: row r + 8 is 32 lanes on
+  f32x4_t a = red[0][i][l], b = red[0][i][(l + (MODE == kHalves ? 40 : 32)) & 63];
 #pragma unroll
   for (int v = 1; v < WAVES; ++v) {
     a += red[v][i][l];
-    if (GATE) b += red[v][NI + i][l];
+    if (MODE != kRows) b += red[v][i][(l + (MODE == kHalves ? 40 : 32)) & 63];
   }
+  if (MODE != kRows && g >= 2) return;
   const int row = i * 16 + e, col = j0 + g * 4;
   if (row >= p.rows) return;
   T* out = static_cast<T*>(p.out) + row * p.ld_out;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     float v = a[r], d;
-    if (GATE) {
+    if (MODE == kGate) {
       activate(p.kind, a[r], v, d);
       v *= b[r];
+    } else if (MODE == kHalves) {
+      v += b[r];
     }
     if (col + r < p.n_out) out[col + r] = T(col + r < p.n ? v : 0.0f);
   }
 }
-template <typename T, bool GATE>
+template <typename T, int MODE>
 void launch_few(const Few& p, bool all_whole, hipStream_t s) {
-  const dim3 grid(unsigned((p.n_out + 15) / 16));
+  const dim3 grid(unsigned((p.n_out + (MODE == kRows ? 15 : 7)) / (MODE == kRows ? 16 : 8)));
   const auto go = [&](auto ni, auto whole) {
-    constexpr int NI = decltype(ni)::value, WAVES = NI == 1 ? 16 : 8;
-    hipLaunchKernelGGL((few_kernel<T, NI, WAVES, decltype(whole)::value, GATE>), grid, dim3(WAVES * 64), 0, s, p);
+    constexpr int NI = decltype(ni)::value, WAVES = MODE == kGate ? 8 : NI == 1 ? 16 : 8;
+    hipLaunchKernelGGL((few_kernel<T, NI, WAVES, decltype(whole)::value, MODE>), grid, dim3(WAVES * 64), 0, s, p);
   };
   const auto rows = [&](auto whole) {
-    if (p.rows <= 16) go(std::integral_constant<int, 1>{}, whole);
-    else if (p.rows <= 32) go(std::integral_constant<int, 2>{}, whole);
-    else go(std::integral_constant<int, 4>{}, whole);
+    if (MODE == kHalves || p.rows <= 16) go(std::integral_constant<int, 1>{}, whole);
+    else if (p.rows <= 32) go(std::integral_constant<int, MODE == kHalves ? 1 : 2>{}, whole);
+    else go(std::integral_constant<int, MODE == kHalves ? 1 : 4>{}, whole);
   };
   if (all_whole) rows(std::true_type{});
   else rows(std::false_type{});
@@ -624,12 +640,14 @@ hipError_t forward_few(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   a.x = d.x, a.w = d.w_gate, a.w2 = d.w_up, a.out = h;
   a.ld_x = d.ld_x, a.ld_w = d.ld_gate, a.ld_w2 = d.ld_up, a.ld_out = hp;
   a.rows = int(d.rows), a.n = d.hidden, a.n_out = int(hp), a.kind = d.activation, a.k = d.width;
-  launch_few<T, true>(a, whole16(d.x, d.ld_x, d.width) && whole16(d.w_gate, d.ld_gate, d.width) && whole16(d.w_up, d.ld_up, d.width), r.s);
+  launch_few<T, kGate>(a, whole16(d.x, d.ld_x, d.width) && whole16(d.w_gate, d.ld_gate, d.width) && whole16(d.w_up, d.ld_up, d.width), r.s);
   Few b{};
   b.x = h, b.w = d.w_down, b.out = y;
   b.ld_x = hp, b.ld_w = d.ld_down, b.ld_out = ld_y;
   b.rows = int(d.rows), b.n = b.n_out = d.out, b.k = d.hidden;
-  launch_few<T, false>(b, whole16(d.w_down, d.ld_down, d.hidden), r.s);
+  const bool w = whole16(d.w_down, d.ld_down, d.hidden);
+  if (d.rows <= 8) launch_few<T, kHalves>(b, w, r.s);
+  else launch_few<T, kRows>(b, w, r.s);
   return hipGetLastError();
 }
 

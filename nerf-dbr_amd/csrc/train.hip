@@ -1313,8 +1313,9 @@ struct nerf_trainer {
   int optimizer = NERF_OPT_ADAM;
   int state_bits = 32;
   nerf_adamw_control* control = nullptr;
+  std::vector<long> plan;          // host copy (8-byte aligned)
+  void* plan_dev = nullptr;
   void* norm_ws = nullptr;
-  size_t norm_ws_bytes = 0;
   unsigned char* codes[2] = {};
   float* scales[2] = {};
 };
@@ -1655,7 +1656,6 @@ void adamw_tensors(const nerf_trainer* tr, nerf_adamw_tensor* out) {
       nerf_adamw_tensor& t = *out++;
       t = nerf_adamw_tensor{};
       t.param = tr->params + at;
-      t.grad = tr->grads + at;
       const bool eight = tr->state_bits == 8;
       t.exp_avg = eight ? (void*)(tr->codes[0] + at) : (void*)(tr->m + at);
       t.exp_avg_sq = eight ? (void*)(tr->codes[1] + at) : (void*)(tr->v + at);
@@ -1663,19 +1663,22 @@ void adamw_tensors(const nerf_trainer* tr, nerf_adamw_tensor* out) {
       t.exp_avg_sq_scale = eight ? tr->scales[1] + b : nullptr;
       t.numel = int64_t(param_count(i));
       t.weight_decay = tr->cfg.weight_decay;
-      t.grad_dtype = NERF_F32;
     }
 }
 
 int adamw_update(nerf_trainer* tr, hipStream_t s) {
-  nerf_adamw_tensor t[2 * NERF_N_PARAMS];
-  adamw_tensors(tr, t);
+  const void* grads[2 * NERF_N_PARAMS];
+  int32_t kinds[2 * NERF_N_PARAMS];
+  for (int k = 0; k < 2 * NERF_N_PARAMS; ++k) {
+    grads[k] = tr->grads + k / NERF_N_PARAMS * size_t(kNetFloats) + param_offset(k % NERF_N_PARAMS);
+    kinds[k] = NERF_F32;
+  }
   nerf_adamw_config c{};
   c.lr = tr->lr, c.beta1 = tr->cfg.beta1, c.beta2 = tr->cfg.beta2, c.eps = tr->cfg.eps;
   c.max_norm = tr->cfg.grad_clip > 0.0 ? tr->cfg.grad_clip : 0.0;
-  c.state_bits = tr->state_bits;
   c.flags = c.max_norm > 0.0 ? NERF_ADAMW_WRITE_GRADS : 0;   // param.grad after the step: the clipped gradient
-  const int rc = nerf_adamw_step(&c, 2 * NERF_N_PARAMS, t, tr->control, tr->norm_ws, tr->norm_ws_bytes, s);
+  const int rc = nerf_adamw_step(&c, tr->plan.data(), tr->plan_dev, grads, kinds, tr->control, tr->norm_ws,
+                                 nerf_adamw_workspace(tr->plan.data()), s);
   if (rc != NERF_OK) return rc;
   HIP_TRY(pack_operands(tr, s));
   tr->steps += 1;
@@ -1807,6 +1810,7 @@ void nerf_trainer_destroy(nerf_trainer* tr) {
   if (tr->bad) (void)hipFree(tr->bad);
   if (tr->control) (void)hipFree(tr->control);
   if (tr->norm_ws) (void)hipFree(tr->norm_ws);
+  if (tr->plan_dev) (void)hipFree(tr->plan_dev);
   for (int k = 0; k < 2; ++k) {
     if (tr->codes[k]) (void)hipFree(tr->codes[k]);
     if (tr->scales[k]) (void)hipFree(tr->scales[k]);
@@ -2022,13 +2026,7 @@ int nerf_trainer_set_optimizer(nerf_trainer* tr, int optimizer, int state_bits) 
   DeviceGuardT dg(tr->device);
   HIP_TRY(hipDeviceSynchronize());
   const size_t n = 2 * size_t(kNetFloats), blocks = 2 * moment_block(NERF_N_PARAMS);
-  if (optimizer == NERF_OPT_ADAMW && !tr->control) {
-    nerf_adamw_tensor t[2 * NERF_N_PARAMS];
-    adamw_tensors(tr, t);
-    tr->norm_ws_bytes = nerf_adamw_workspace(2 * NERF_N_PARAMS, t);
-    if (!tr->norm_ws) HIP_TRY(hipMalloc(&tr->norm_ws, tr->norm_ws_bytes));
-    HIP_TRY(hipMalloc((void**)&tr->control, sizeof(nerf_adamw_control)));
-  }
+  if (optimizer == NERF_OPT_ADAMW && !tr->control) HIP_TRY(hipMalloc((void**)&tr->control, sizeof(nerf_adamw_control)));
   if (state_bits == 8)
     for (int k = 0; k < 2; ++k) {
       if (!tr->codes[k]) HIP_TRY(hipMalloc((void**)&tr->codes[k], n));
@@ -2053,6 +2051,17 @@ int nerf_trainer_set_optimizer(nerf_trainer* tr, int optimizer, int state_bits) 
           return rc;
         }
       }
+  }
+  if (optimizer == NERF_OPT_ADAMW) {
+    nerf_adamw_tensor t[2 * NERF_N_PARAMS];
+    adamw_tensors(tr, t);
+    const size_t bytes = nerf_adamw_plan_bytes(2 * NERF_N_PARAMS, t, state_bits);   // the same for both state_bits
+    tr->plan.assign((bytes + sizeof(long) - 1) / sizeof(long), 0);
+    const int rc = nerf_adamw_plan(2 * NERF_N_PARAMS, t, state_bits, tr->plan.data());
+    if (rc != NERF_OK) return rc;
+    if (!tr->plan_dev) HIP_TRY(hipMalloc(&tr->plan_dev, bytes));
+    if (!tr->norm_ws) HIP_TRY(hipMalloc(&tr->norm_ws, nerf_adamw_workspace(tr->plan.data())));
+    HIP_TRY(hipMemcpy(tr->plan_dev, tr->plan.data(), bytes, hipMemcpyHostToDevice));
   }
   tr->optimizer = optimizer;
   return sync_control(tr);

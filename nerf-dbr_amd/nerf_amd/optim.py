@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 from contextlib import ExitStack, nullcontext
+from operator import attrgetter
 from typing import Optional, Sequence, Union
 
 import numpy as np
@@ -15,6 +16,8 @@ import numpy as np
 from . import runtime as rt
 
 BLOCK = rt.NERF_ADAMW_BLOCK
+_NONE = type(None)
+_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
 
 
 def blocks(numel: int) -> int:
@@ -23,7 +26,7 @@ def blocks(numel: int) -> int:
 
 
 class AdamW:
-    """AdamW on device tensors: ``step(grads)`` updates every parameter in one or two kernel launches per 48 tensors.
+    """AdamW on device tensors: ``step(grads)`` updates every parameter in two launches (three with a norm) for each 440 tensors of one type.
 
     params: contiguous float32, bfloat16 or float16 tensors on one device, none twice.  A 16-bit
     parameter has a float32 master here: the step updates the master and writes its rounded value.
@@ -119,11 +122,9 @@ class AdamW:
         self.grad_norm = self._control.view(torch.float32)[3]
 
         n = len(self.params)
-        self._table = (rt.AdamWTensor * n)()
-        self._columns = np.frombuffer(self._table, dtype=np.dtype(rt.AdamWTensor))
-        self._numels = np.array(numels, np.int64)
+        table = (rt.AdamWTensor * n)()
         for i, p in enumerate(self.params):
-            t, m = self._table[i], self.masters[i]
+            t, m = table[i], self.masters[i]
             t.param = (p if m is None else m).data_ptr()
             t.model = 0 if m is None else p.data_ptr()
             t.model_dtype = 0 if m is None else self._model[p.dtype]
@@ -132,14 +133,19 @@ class AdamW:
                 t.exp_avg_scale, t.exp_avg_sq_scale = self.exp_avg_scale[i].data_ptr(), self.exp_avg_sq_scale[i].data_ptr()
             t.numel, t.weight_decay = p.numel(), decay[i]
         self._shapes = [p.shape for p in self.params]
-        self._left_out = False          # the last step's gradients had gaps
         c = rt.AdamWConfig()
         c.beta1, c.beta2, c.eps = float(betas[0]), float(betas[1]), float(eps)
         c.max_norm = 0.0 if max_norm is None else float(max_norm)
-        c.state_bits = state_bits
         c.flags = (rt.NERF_ADAMW_SKIP_NONFINITE if skip_nonfinite else 0) | (rt.NERF_ADAMW_WRITE_GRADS if write_grads else 0)
         self._config = c
-        self._workspace_bytes = rt.load_library().nerf_adamw_workspace(n, self._table) if self._norm else 0
+        lib = rt.load_library()
+        size = lib.nerf_adamw_plan_bytes(n, table, state_bits)
+        if not size:
+            raise rt.NerfError(lib.nerf_last_error().decode(errors="replace"))
+        self._plan = np.zeros(size // 8, np.int64)      # its device copy lies beside it
+        rt._check(lib.nerf_adamw_plan(n, table, state_bits, self._plan.ctypes.data))
+        self._plan_device = torch.from_numpy(self._plan).to(device)
+        self._workspace_bytes = lib.nerf_adamw_workspace(self._plan.ctypes.data) if self._norm else 0
 
     def _lr(self, lr):
         """(host value, device tensor or None) of a learning rate."""
@@ -167,43 +173,43 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} gradients needed, got {len(grads)}")
         host, on_device = self._lr(self.lr if lr is None else lr)
-        codes, index, shapes = self._grad, self.device.index, self._shapes
-        ptr, kind, none = [], [], []
-        for i, g in enumerate(grads):
-            if g is None:
-                none.append(i)
-                ptr.append(0)
-                kind.append(0)
-                continue
-            k = codes.get(g.dtype)
-            if k is None or g.shape != shapes[i] or not g.is_contiguous() or g.get_device() != index:
-                raise ValueError(f"gradient {i} {tuple(g.shape)} {g.dtype} on {g.device} must be contiguous, "
-                                 f"{tuple(shapes[i])} and on {self.device}")
-            ptr.append(g.data_ptr())
-            kind.append(k)
-        col = self._columns
-        col["grad"] = ptr
-        col["grad_dtype"] = kind
-        if none or self._left_out:
-            col["numel"] = self._numels
-            col["numel"][none] = 0
-            self._left_out = bool(none)
-            if not col["numel"].any():
+        n, index, shapes = len(grads), self.device.index, self._shapes
+        # every gradient is looked at in four passes of C loops: there may be hundreds
+        given = [g for g in grads if g is not None] if _NONE in set(map(type, grads)) else grads
+        if given is not grads:
+            shapes = [s for s, g in zip(shapes, grads) if g is not None]
+        kinds = list(map(_dtype_of, given))
+        if (not set(kinds) <= set(self._grad) or list(map(_shape_of, given)) != shapes
+                or not all(map(torch.Tensor.is_contiguous, given)) or set(map(torch.Tensor.get_device, given)) - {index}):
+            for i, g in enumerate(grads):
+                if g is not None and (g.dtype not in self._grad or g.shape != self._shapes[i] or not g.is_contiguous()
+                                      or g.get_device() != index):
+                    raise ValueError(f"gradient {i} {tuple(g.shape)} {g.dtype} on {g.device} must be contiguous, "
+                                     f"{tuple(self._shapes[i])} and on {self.device}")
+        addresses = np.fromiter(map(torch.Tensor.data_ptr, given), np.uint64, len(given))
+        if len(set(kinds)) == 1:
+            codes = np.full(len(given), self._grad[kinds[0]], np.int32)
+        else:
+            codes = np.fromiter((self._grad[k] for k in kinds), np.int32, len(given))
+        if given is not grads:
+            have = [g is not None for g in grads]
+            if not any(h and s.numel() for h, s in zip(have, self._shapes)):
                 raise ValueError("no gradients")
+            full, kind = np.zeros(n, np.uint64), np.zeros(n, np.int32)
+            full[have], kind[have] = addresses, codes
+            addresses, codes = full, kind
         c = self._config
         c.lr = host
         c.lr_device = None if on_device is None else on_device.data_ptr()
-        lib = rt.load_library()
         handle, contexts = _on(torch, (self._control,), stream)
         with ExitStack() if contexts else nullcontext() as stack:
             for x in contexts:
                 stack.enter_context(x)
-            n = self._workspace_bytes
-            if none and n:    # fewer values can be cut into more, smaller pieces
-                n = max(n, lib.nerf_adamw_workspace(len(ptr), self._table))
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-            rt._check(lib.nerf_adamw_step(ctypes.byref(c), len(ptr), self._table, self._control.data_ptr(),
-                                          None if ws is None else ws.data_ptr(), n, handle))
+            size = self._workspace_bytes
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+            rt._check(rt.load_library().nerf_adamw_step(
+                ctypes.byref(c), self._plan.ctypes.data, self._plan_device.data_ptr(), addresses.ctypes.data,
+                codes.ctypes.data, self._control.data_ptr(), None if ws is None else ws.data_ptr(), size, handle))
         return self.grad_norm if self._norm else None
 
     @property

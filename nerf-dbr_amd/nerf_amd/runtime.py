@@ -101,8 +101,10 @@ SIGNATURES = {
     "nerf_gated_block_workspace": (_c.c_size_t, [_P, _c.c_int]),
     "nerf_gated_block_forward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_size_t, _P]),
     "nerf_gated_block_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P, _c.c_size_t, _P]),
-    "nerf_adamw_workspace": (_c.c_size_t, [_c.c_int, _P]),
-    "nerf_adamw_step": (_c.c_int, [_P, _c.c_int, _P, _P, _P, _c.c_size_t, _P]),
+    "nerf_adamw_plan_bytes": (_c.c_size_t, [_c.c_int, _P, _c.c_int]),
+    "nerf_adamw_plan": (_c.c_int, [_c.c_int, _P, _c.c_int, _P]),
+    "nerf_adamw_workspace": (_c.c_size_t, [_P]),
+    "nerf_adamw_step": (_c.c_int, [_P, _P, _P, _P, _P, _P, _P, _c.c_size_t, _P]),
     "nerf_trainer_set_optimizer": (_c.c_int, [_P, _c.c_int, _c.c_int]),
 }
 
@@ -152,16 +154,15 @@ class AdamWControl(_c.Structure):
 
 class AdamWTensor(_c.Structure):
     """nerf_adamw_tensor (addresses as integers)."""
-    _fields_ = [("param", _c.c_uint64), ("model", _c.c_uint64), ("grad", _c.c_uint64), ("exp_avg", _c.c_uint64),
-                ("exp_avg_sq", _c.c_uint64), ("exp_avg_scale", _c.c_uint64), ("exp_avg_sq_scale", _c.c_uint64),
-                ("numel", _c.c_int64), ("weight_decay", _c.c_double), ("model_dtype", _c.c_int32),
-                ("grad_dtype", _c.c_int32)]
+    _fields_ = [("param", _c.c_uint64), ("model", _c.c_uint64), ("exp_avg", _c.c_uint64), ("exp_avg_sq", _c.c_uint64),
+                ("exp_avg_scale", _c.c_uint64), ("exp_avg_sq_scale", _c.c_uint64), ("numel", _c.c_int64),
+                ("weight_decay", _c.c_double), ("model_dtype", _c.c_int32), ("reserved", _c.c_int32)]
 
 
 class AdamWConfig(_c.Structure):
     """nerf_adamw_config."""
     _fields_ = [("lr", _c.c_double), ("beta1", _c.c_double), ("beta2", _c.c_double), ("eps", _c.c_double),
-                ("max_norm", _c.c_double), ("lr_device", _P), ("state_bits", _c.c_int32), ("flags", _c.c_int32)]
+                ("max_norm", _c.c_double), ("lr_device", _P), ("flags", _c.c_int32), ("reserved", _c.c_int32)]
 
 
 NERF_TRAIN_NO_UPDATE = 1

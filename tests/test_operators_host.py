@@ -275,55 +275,74 @@ def test_adamw_refuses_shared_memory():
         optim.AdamW([a[:6], a[5:]])
 
 
-def _adam():
+def _adam(bits=32):
     c = rt.AdamWConfig()
-    c.lr, c.beta1, c.beta2, c.eps, c.state_bits = 1e-3, 0.9, 0.999, 1e-8, 32
+    c.lr, c.beta1, c.beta2, c.eps = 1e-3, 0.9, 0.999, 1e-8
     t = (rt.AdamWTensor * 1)()
-    t[0].param = t[0].grad = t[0].exp_avg = t[0].exp_avg_sq = 256
+    t[0].param = t[0].exp_avg = t[0].exp_avg_sq = 256
     t[0].numel = 5
+    if bits == 8:
+        t[0].exp_avg_scale = t[0].exp_avg_sq_scale = 256
     return c, t
 
 
+def _plan(t, bits=32):
+    lib = rt.load_library()
+    plan = (ctypes.c_int64 * (lib.nerf_adamw_plan_bytes(len(t), t, bits) // 8))()
+    assert lib.nerf_adamw_plan(len(t), t, bits, plan) == 0
+    return plan
+
+
 @pytest.mark.parametrize("field, value", [
-    ("lr", -1.0), ("beta1", 1.0), ("beta2", -0.1), ("eps", -1.0), ("state_bits", 16), ("flags", 8), ("lr", float("nan"))])
+    ("param", 0), ("exp_avg", 0), ("exp_avg_sq", 0), ("numel", -1), ("weight_decay", -1.0), ("weight_decay", float("nan")),
+    ("param", 257), ("exp_avg", 254), ("numel", 0), ("numel", 1 << 41)])
+def test_adamw_plan_refuses(field, value):
+    lib = rt.load_library()
+    _, t = _adam()
+    setattr(t[0], field, value)
+    assert lib.nerf_adamw_plan_bytes(1, t, 32) == 0
+    assert lib.nerf_adamw_plan(1, t, 32, (ctypes.c_int64 * 64)()) == -1
+
+
+def test_adamw_plan_refuses_the_rest():
+    lib = rt.load_library()
+    _, t = _adam()
+    assert lib.nerf_adamw_plan_bytes(1, None, 32) == 0 and lib.nerf_adamw_plan_bytes(0, t, 32) == 0
+    assert lib.nerf_adamw_plan_bytes(1, t, 16) == 0
+    assert lib.nerf_adamw_plan_bytes(1, t, 8) == 0          # scales missing
+    assert lib.nerf_adamw_plan(1, t, 32, None) == -1
+    t[0].model, t[0].model_dtype = 256, rt.NERF_F32
+    assert lib.nerf_adamw_plan_bytes(1, t, 32) == 0
+    assert lib.nerf_adamw_workspace(None) == 0 and lib.nerf_adamw_workspace((ctypes.c_int64 * 8)()) == 0
+
+
+@pytest.mark.parametrize("field, value", [
+    ("lr", -1.0), ("beta1", 1.0), ("beta2", -0.1), ("eps", -1.0), ("flags", 8), ("lr", float("nan")), ("max_norm", float("nan"))])
 def test_adamw_c_refuses_settings(field, value):
     lib = rt.load_library()
     c, t = _adam()
+    plan = _plan(t)
+    g, k = (ctypes.c_uint64 * 1)(256), (ctypes.c_int32 * 1)(0)
     setattr(c, field, value)
-    assert lib.nerf_adamw_step(ctypes.byref(c), 1, t, 256, None, 0, None) == -1
-
-
-@pytest.mark.parametrize("field, value", [
-    ("param", 0), ("grad", 0), ("exp_avg", 0), ("exp_avg_sq", 0), ("numel", -1), ("grad_dtype", 3), ("weight_decay", -1.0),
-    ("param", 257), ("grad", 258), ("exp_avg", 255), ("numel", 0)])
-def test_adamw_c_refuses_tensors(field, value):
-    lib = rt.load_library()
-    c, t = _adam()
-    setattr(t[0], field, value)
-    assert lib.nerf_adamw_step(ctypes.byref(c), 1, t, 256, None, 0, None) == -1
+    assert lib.nerf_adamw_step(ctypes.byref(c), plan, 256, g, k, 256, None, 0, None) == -1
 
 
 def test_adamw_c_refuses_the_rest():
     lib = rt.load_library()
     c, t = _adam()
-    step = lib.nerf_adamw_step
-    assert step(None, 1, t, 256, None, 0, None) == -1
-    assert step(ctypes.byref(c), 1, None, 256, None, 0, None) == -1
-    assert step(ctypes.byref(c), -1, t, 256, None, 0, None) == -1
-    assert step(ctypes.byref(c), 0, t, 256, None, 0, None) == -1
-    assert step(ctypes.byref(c), 1, t, None, None, 0, None) == -1
-    t[0].model, t[0].model_dtype = 256, rt.NERF_F32
-    assert step(ctypes.byref(c), 1, t, 256, None, 0, None) == -1
-    c, t = _adam()
-    c.state_bits = 8                                 # scales missing
-    assert step(ctypes.byref(c), 1, t, 256, None, 0, None) == -1
-    c, t = _adam()
+    plan = _plan(t)
+    g, k = (ctypes.c_uint64 * 1)(256), (ctypes.c_int32 * 1)(0)
+    ok = [ctypes.byref(c), plan, 256, g, k, 256, None, 0, None]
+    for at, value in ((0, None), (1, None), (1, (ctypes.c_int64 * 8)()), (2, None), (2, 264), (3, None), (4, None), (5, None),
+                      (5, 258), (3, (ctypes.c_uint64 * 1)(258)), (3, (ctypes.c_uint64 * 1)(0)), (4, (ctypes.c_int32 * 1)(3))):
+        args = list(ok)
+        args[at] = value
+        assert lib.nerf_adamw_step(*args) == -1, at
     c.max_norm = 1.0                                 # a norm needs its workspace
-    need = lib.nerf_adamw_workspace(1, t)
+    need = lib.nerf_adamw_workspace(plan)
     assert need >= 8
-    assert step(ctypes.byref(c), 1, t, 256, None, need, None) == -1
-    assert step(ctypes.byref(c), 1, t, 256, 256, need - 1, None) == -1
-    assert step(ctypes.byref(c), 1, t, 256, 260, need, None) == -1
+    for ws, size in ((None, need), (256, need - 1), (260, need)):
+        assert lib.nerf_adamw_step(*ok[:6], ws, size, None) == -1
 
 
 def test_trainer_options_are_checked():
