@@ -14,6 +14,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "nerf_asm.h"
 
 namespace nerf {
@@ -72,9 +74,11 @@ template <int E, int NT, bool KC, int PARTS>
 struct Stage {
   static constexpr int kBytes = E * 64 * 2;
   static constexpr int kChunks = E * 8 / NT;   // 16-byte pieces a thread fetches per step
-  long off[kChunks];                           // from p, without k
+  static_assert(PARTS == 1 || (KC && kChunks % 2 == 0), "a piece lies in one half");
+  unsigned off[kChunks];                       // from the tile's first row (KC) or column
 
   static __device__ __forceinline__ int gran(int k) { return ((k & 3) | (((k >> 3) & 3) << 2)) & (E / 16 - 1); }
+  static __device__ __forceinline__ long half(int c) { return PARTS == 2 && c >= kChunks / 2; }
 
   __device__ __forceinline__ void init(const Side& s, long i0) {
 #pragma unroll
@@ -83,108 +87,201 @@ struct Stage {
       if (KC) {
         const int r = q >> 3, chunk = (q & 7) ^ (r & 7);
         const int rr = PARTS == 2 ? r & (E / 2 - 1) : r;
-        long row = i0 + rr;
-        row = row < s.n ? row : s.n - 1;      // behind the edge: any row, its results are not stored
-        off[c] = row * s.ld + chunk * 16 + (PARTS == 2 && r >= E / 2 ? s.split : 0);
+        const long most = s.n - 1 - i0;       // behind the edge: the last row, its results are not stored
+        off[c] = unsigned((rr < most ? rr : most) * s.ld) + chunk * 16;
       } else {
         const int k = q / (E / 8), slot = q & (E / 8 - 1);
-        long col = i0 + ((slot >> 1) ^ gran(k)) * 16 + (slot & 1) * 8;
-        col = col < s.n ? col : s.n - 8;
-        off[c] = k * s.ld + col * 2;
+        const long col = ((slot >> 1) ^ gran(k)) * 16 + (slot & 1) * 8, most = s.n - 8 - i0;
+        off[c] = unsigned(k * s.ld) + unsigned(col < most ? col : most) * 2;
       }
     }
   }
-  // fetch the 64 values of k from k0 of one segment into the stage at LDS byte `lds`
-  __device__ __forceinline__ void fetch(const char* p, const Side& s, long k0, unsigned lds) const {
-    const char* base = p + (KC ? k0 * 2 : k0 * s.ld);
-    const unsigned wave = threadIdx.x & ~63u;
-    if (k0 + 64 <= s.k_n) {
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) lds_dma_16(base + off[c], lds + (c * NT + wave) * 16);
+  // where a segment's 64 values of k from k0 begin (uniform)
+  __device__ __forceinline__ const char* base(const char* p, const Side& s, long i0, long k0) const {
+    return p + (KC ? i0 * s.ld + k0 * 2 : k0 * s.ld + i0 * 2);
+  }
+  // fetch piece c of them into the stage at LDS byte `lds`; CHECKED: k may end inside
+  template <bool CHECKED>
+  __device__ __forceinline__ void fetch(int c, const char* from, const Side& s, long k0, unsigned lds) const {
+    const unsigned to = lds + (c * NT + (threadIdx.x & ~63u)) * 16;
+    const char* at = from + (half(c) ? s.split : 0);
+    if constexpr (CHECKED) {
+      const int q = c * NT + threadIdx.x;
+      const long k = k0 + (KC ? ((q & 7) ^ ((q >> 3) & 7)) * 8 : q / (E / 8));
+      lds_dma_16(k < s.k_n ? at + off[c] : reinterpret_cast<const char*>(kZeros), to);
     } else {
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int q = c * NT + threadIdx.x;
-        const long k = k0 + (KC ? ((q & 7) ^ ((q >> 3) & 7)) * 8 : q / (E / 8));
-        const char* at = base + off[c];
-        lds_dma_16(k < s.k_n ? at : reinterpret_cast<const char*>(kZeros), lds + (c * NT + wave) * 16);
-      }
+      lds_dma_16_s(at, off[c], to);
     }
   }
 };
 
-// The fragment of 16 rows from `row` (a multiple of 16) and 32 values of k from 32 * ks.
+// Reads a wave's fragments of a staged side: rows 16 t .. 16 t + 15 behind the wave's first (a multiple of
+// 16, of 16 x its fragments where the side's own index is contiguous), 32 values of k from 32 * ks.
 template <typename T, int E, bool KC>
-__device__ __forceinline__ typename Frag<T>::type fragment(unsigned lds, int row, int ks) {
-  const int l = threadIdx.x & 63, g = l >> 4, e = l & 15;
-  if (KC) {
-    const unsigned at = lds + (row + e) * 128 + (((4 * ks + g) ^ (e & 7)) << 4);
-    return *lds_ptr<typename Frag<T>::type>(at, 0);
+struct Reader {
+  typedef typename Frag<T>::type F;
+  unsigned lane[KC ? 2 : 1];     // from the stage's start, without the fragment
+
+  __device__ __forceinline__ void init(int first) {
+    const int l = threadIdx.x & 63, g = l >> 4, e = l & 15;
+    if constexpr (KC) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) lane[ks] = (first + e) * 128 + (((4 * ks + g) ^ (e & 7)) << 4);
+    } else {
+      const int k = 8 * g + (e >> 2);
+      lane[0] = k * (E * 2) + (((first >> 4) ^ Stage<E, 64, false, 1>::gran(k)) << 5) + ((e & 3) << 3);
+    }
   }
-  typedef __attribute__((address_space(3))) short4_t lds_short4;
-  const int k = 32 * ks + 8 * g + (e >> 2);
-  const int f = Stage<E, 64, false, 1>::gran(8 * g + (e >> 2));
-  const unsigned at = lds + k * (E * 2) + (((row >> 4) ^ f) << 5) + ((e & 3) << 3);
-  const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)at);
-  const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(at + 4 * E * 2));
-  struct {
-    short4_t a, b;
-  } both{lo, hi};
-  return __builtin_bit_cast(typename Frag<T>::type, both);
-}
+  // rows: the fragment's distance in rows, known at compile time
+  __device__ __forceinline__ F read(unsigned stage, int rows, int ks) const {
+    if constexpr (KC) {
+      const auto* p = (const __attribute__((address_space(3))) char*)(uintptr_t)(stage + lane[ks]);
+      return *(const __attribute__((address_space(3))) F*)(p + rows * 128);
+    } else {
+      typedef __attribute__((address_space(3))) short4_t lds_short4;
+      // the granule is an exclusive or with the lane's swizzle, and the fragment's number is in bits of
+      // their own: one v_xor a fragment, nothing kept
+      const auto* p = (const __attribute__((address_space(3))) char*)(uintptr_t)((stage + lane[0]) ^ (unsigned(rows) << 1));
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + ks * (64 * E)));
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + ks * (64 * E) + 8 * E));
+      struct {
+        short4_t a, b;
+      } both{lo, hi};
+      return __builtin_bit_cast(F, both);
+    }
+  }
+};
 
 // A workgroup of WI x WJ waves; a wave owns NI x NJ fragments of 16 x 16.
 template <int WI_, int WJ_, int NI_, int NJ_>
 struct Tile {
   static constexpr int WI = WI_, WJ = WJ_, NI = NI_, NJ = NJ_;
+  static constexpr int kWaves = NI * NJ > 32 ? 1 : 2;   // waves a SIMD: 512 or 256 registers
   static constexpr int NT = WI * WJ * 64, TI = WI * NI * 16, TJ = WJ * NJ * 16;
 };
 
 // acc[j][i] += the products of steps [first, last) of the segments' steps (steps_per = ceil(k / 64) each).
 // J fragments are the MFMA's first operand: a lane holds 4 neighbouring j of one i.
+//
+// A step is 2 NI groups of NJ matrix instructions: group q multiplies the I fragment q % NI of the half
+// q / NI by the half's J fragments.  I fragments are read L = NI / 2 groups ahead and J fragments over the
+// L groups before their half, so the last L groups of a step read from the next stage: the step's one
+// barrier stands before them.  By then a wave has read all of its own stage, which the step after next
+// may overwrite (its pieces are fetched over the same L groups), and its pieces of the next one have been
+// in flight for a step.  The compiler would place each read before its use and wait for it there, so the
+// order of the groups is pinned.
+template <typename T, typename C, bool IK, bool JK, int PARTS>
+struct Product {
+  typedef Stage<C::TI, C::NT, IK, 1> SI;
+  typedef Stage<C::TJ, C::NT, JK, PARTS> SJ;
+  typedef typename Frag<T>::type F;
+  static constexpr unsigned kStage = SI::kBytes + SJ::kBytes;
+  static constexpr int kPieces = SI::kChunks + SJ::kChunks;
+  static constexpr int L = C::NI / 2, G = 2 * C::NI;
+  static constexpr int kJ = (C::NJ + L - 1) / L, kP = (kPieces + L - 1) / L;   // J reads and pieces a group
+  F fi[2][C::NI], fj[2][C::NJ];
+  Reader<T, C::TI, IK> ri;
+  Reader<T, C::TJ, JK> rj;
+
+  __device__ __forceinline__ F read_j(int j, unsigned at, int ks) const {
+    constexpr int per = C::NJ / PARTS;
+    return rj.read(at + SI::kBytes, (j / per) * (C::TJ / PARTS) + (j % per) * 16, ks);
+  }
+  __device__ __forceinline__ F read_i(int i, unsigned at, int ks) const { return ri.read(at, i * 16, ks); }
+  __device__ __forceinline__ void run(f32x4_t (&acc)[C::NJ][C::NI], const Side& si, const Side& sj, long i0, long j0, int steps_per,
+                                      int first, int last, unsigned lds) {
+    if (first >= last) return;
+    const int wave = threadIdx.x >> 6;
+    ri.init(wave / C::WJ * C::NI * 16);
+    rj.init(wave % C::WJ * (C::NJ / PARTS) * 16);
+    SI a;
+    SJ b;
+    a.init(si, i0);
+    b.init(sj, j0);
+    int seg = first / steps_per, step = first - seg * steps_per;
+    const int n = last - first;
+    const auto advance = [&] {
+      if (++step == steps_per) step = 0, ++seg;
+    };
+    const auto fetch_all = [&](unsigned at) {
+      const long k0 = long(step) * 64;
+      const char *pa = a.base(si.p[seg], si, i0, k0), *pb = b.base(sj.p[seg], sj, j0, k0);
+#pragma unroll
+      for (int c = 0; c < SI::kChunks; ++c) a.template fetch<true>(c, pa, si, k0, at);
+#pragma unroll
+      for (int c = 0; c < SJ::kChunks; ++c) b.template fetch<true>(c, pb, sj, k0, at + SI::kBytes);
+      advance();
+    };
+    fetch_all(lds);
+    wait_vmcnt(0);
+    __syncthreads();
+    if (n > 1) fetch_all(lds + kStage);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) fj[0][j] = read_j(j, lds, 0);
+#pragma unroll
+    for (int i = 0; i < L; ++i) fi[0][i] = read_i(i, lds, 0);
+    // fetching: 0 nothing, 1 a whole step, 2 checked
+    const auto one_step = [&](int t, auto more, auto fetching) {
+      constexpr int kFetch = decltype(fetching)::value;
+      const unsigned now = lds + (t & 1) * kStage, next = lds + (~t & 1) * kStage;
+      const long k0 = long(step) * 64;
+      const char *pa = nullptr, *pb = nullptr;
+      if constexpr (kFetch != 0) pa = a.base(si.p[seg], si, i0, k0), pb = b.base(sj.p[seg], sj, j0, k0);
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        if (q == G - L) {
+          wait_vmcnt(0);      // this wave's pieces of the next stage; the barrier makes it every wave's
+          __syncthreads();
+        }
+        const int ahead = q + L;
+        if (ahead < G) fi[ahead / C::NI][ahead % C::NI] = read_i(ahead % C::NI, now, ahead / C::NI);
+        if (q >= C::NI - L - 1 && q < C::NI - 1)
+#pragma unroll
+          for (int j = (q - (C::NI - L - 1)) * kJ; j < (q - (C::NI - L - 1) + 1) * kJ; ++j)
+            if (j < C::NJ) fj[1][j] = read_j(j, now, 1);
+        if (ahead >= G) {
+          if constexpr (decltype(more)::value) {
+#pragma unroll
+            for (int j = (ahead - G) * kJ; j < (ahead - G + 1) * kJ; ++j)
+              if (j < C::NJ) fj[0][j] = read_j(j, next, 0);
+            fi[0][ahead - G] = read_i(ahead - G, next, 0);
+          }
+          if constexpr (kFetch != 0)
+#pragma unroll
+            for (int c = (ahead - G) * kP; c < (ahead - G + 1) * kP; ++c) {
+              if (c < SI::kChunks) a.template fetch<kFetch == 2>(c, pa, si, k0, now);
+              else if (c < kPieces) b.template fetch<kFetch == 2>(c - SI::kChunks, pb, sj, k0, now + SI::kBytes);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) acc[j][q % C::NI] = Frag<T>::mma(fj[q / C::NI][j], fi[q / C::NI][q % C::NI], acc[j][q % C::NI]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (kFetch != 0) advance();
+    };
+    // steps whose fetch is whole: all of them, or up to the first end of k inside a step (two counted loops:
+    // one with the choice, or an exit, inside took new registers for every accumulator and spilled 390)
+    const long most = long(steps_per) * 64;
+    const bool tail = si.k_n < most || sj.k_n < most;
+    int quick = tail && steps_per - 1 - step < n - 2 ? steps_per - 1 - step : n - 2;
+    int t = 0;
+    if (quick > 0)
+      do one_step(t, std::true_type{}, std::integral_constant<int, 1>{});
+      while (++t < quick);
+    if (t < n - 2)
+      do one_step(t, std::true_type{}, std::integral_constant<int, 2>{});
+      while (++t < n - 2);
+    if (t + 1 < n) one_step(t++, std::true_type{}, std::integral_constant<int, 0>{});
+    one_step(t, std::false_type{}, std::integral_constant<int, 0>{});
+    __syncthreads();      // the stages may be used again
+  }
+};
 template <typename T, typename C, bool IK, bool JK, int PARTS>
 __device__ __forceinline__ void accumulate(f32x4_t (&acc)[C::NJ][C::NI], const Side& si, const Side& sj, long i0, long j0,
                                            int steps_per, int first, int last, unsigned lds) {
-  typedef Stage<C::TI, C::NT, IK, 1> SI;
-  typedef Stage<C::TJ, C::NT, JK, PARTS> SJ;
-  constexpr unsigned kStage = SI::kBytes + SJ::kBytes;
-  if (first >= last) return;
-  SI a;
-  SJ b;
-  a.init(si, i0);
-  b.init(sj, j0);
-  const int wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ;
-  int seg = first / steps_per, step = first - seg * steps_per;
-  auto fetch = [&](unsigned at) {
-    a.fetch(si.p[seg], si, long(step) * 64, at);
-    b.fetch(sj.p[seg], sj, long(step) * 64, at + SI::kBytes);
-    if (++step == steps_per) step = 0, ++seg;
-  };
-  fetch(lds);
-  wait_vmcnt(0);
-  __syncthreads();
-  for (int t = first; t < last; ++t) {
-    const unsigned now = lds + ((t - first) & 1) * kStage;
-    if (t + 1 < last) fetch(lds + ((t - first + 1) & 1) * kStage);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      typename Frag<T>::type fj[C::NJ];
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) {
-        constexpr int per = C::NJ / PARTS;
-        const int row = (j / per) * (C::TJ / PARTS) + wj * per * 16 + (j % per) * 16;
-        fj[j] = fragment<T, C::TJ, JK>(now + SI::kBytes, row, ks);
-      }
-#pragma unroll
-      for (int i = 0; i < C::NI; ++i) {
-        const typename Frag<T>::type fi = fragment<T, C::TI, IK>(now, (wi * C::NI + i) * 16, ks);
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) acc[j][i] = Frag<T>::mma(fj[j], fi, acc[j][i]);
-      }
-    }
-    wait_vmcnt(0);      // the next step's pieces of this wave; the barrier makes it every wave's
-    __syncthreads();
-  }
+  Product<T, C, IK, JK, PARTS> p;
+  p.run(acc, si, sj, i0, j0, steps_per, first, last, lds);
 }
 
 // Four neighbouring values of a row; `wide`: the row's address allows one store.

@@ -33,6 +33,8 @@ __device__ __forceinline__ void activate(int kind, float g, float& a, float& d) 
 // The 256 x 256 tile of 8 waves carries long products; the 128 x 128 tile of 4 waves (two workgroups a CU)
 // fills the machine where there are few tiles.
 typedef Tile<2, 4, 8, 4> Large;
+typedef Tile<4, 2, 4, 8> LargeBack;
+
 typedef Tile<2, 2, 4, 4> Small;
 
 // 32-bit operands run on the f16 matrix cores as two halves each, x 2^e = hi + lo with e from the largest
@@ -49,7 +51,7 @@ __device__ __forceinline__ int exponent(unsigned top) { return 141 - max(int(top
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
 template <typename T, typename C, typename O>
-__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
+__global__ __launch_bounds__(C::NT, C::kWaves) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
   __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
 // and h, dg and du of the tile from the three.
 template <typename T, typename C, typename O>
-__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
+__global__ __launch_bounds__(C::NT, C::kWaves) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
                                                                  int kind, O* h, O* dg, O* du, long ld_h, long rows, long hidden,
                                                                  unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
@@ -164,7 +166,7 @@ __device__ __forceinline__ void store_tile(const Problem& p, unsigned ti, unsign
   store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, v);
 }
 template <typename T, typename C, bool IK, bool JK, typename O>
-__global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
+__global__ __launch_bounds__(C::NT, C::kWaves) void product_mma_kernel(Problems all) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
   int k = 0;
   while (k + 1 < all.n && blockIdx.x >= all.p[k + 1].first) ++k;
@@ -537,7 +539,7 @@ struct Run {
       tiles += long(p.tiles_i) * p.tiles_j;
     }
     if (tiles == 0) return;      // no rows
-    const long slots = 256L * (512 / C::NT);
+    const long slots = 256L * (C::TI * C::TJ > 128 * 128 ? 1 : 2);
     for (int k = 0; k < all.n; ++k) {
       Problem& p = all.p[k];
       const int total = p.steps * p.segs;
@@ -625,7 +627,7 @@ void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Sid
     hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(d.width), steps_of(d.out), segs,
                        d.activation, h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
   };
-  if (use_large(d.rows, 2 * hp)) go(Large{});
+  if (use_large(d.rows, 2 * hp)) go(LargeBack{});
   else go(Small{});
 }
 
