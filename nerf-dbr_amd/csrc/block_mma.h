@@ -156,7 +156,6 @@ struct Reader {
 template <int WI_, int WJ_, int NI_, int NJ_>
 struct Tile {
   static constexpr int WI = WI_, WJ = WJ_, NI = NI_, NJ = NJ_;
-  static constexpr int kWaves = NI * NJ > 32 ? 1 : 2;   // waves a SIMD: 512 or 256 registers
   static constexpr int NT = WI * WJ * 64, TI = WI * NI * 16, TJ = WJ * NJ * 16;
 };
 
@@ -234,29 +233,36 @@ struct Product {
           __syncthreads();
         }
         const int ahead = q + L;
-        if (ahead < G) fi[ahead / C::NI][ahead % C::NI] = read_i(ahead % C::NI, now, ahead / C::NI);
-        if (q >= C::NI - L - 1 && q < C::NI - 1)
+        // what a group has to do besides: its I read, J reads, pieces; dealt over the NJ gaps between its
+        // matrix instructions, so that a wave alone on its SIMD keeps the matrix unit busy
+        const auto others = [&](int slot) {
 #pragma unroll
-          for (int j = (q - (C::NI - L - 1)) * kJ; j < (q - (C::NI - L - 1) + 1) * kJ; ++j)
-            if (j < C::NJ) fj[1][j] = read_j(j, now, 1);
-        if (ahead >= G) {
-          if constexpr (decltype(more)::value) {
-#pragma unroll
-            for (int j = (ahead - G) * kJ; j < (ahead - G + 1) * kJ; ++j)
-              if (j < C::NJ) fj[0][j] = read_j(j, next, 0);
-            fi[0][ahead - G] = read_i(ahead - G, next, 0);
-          }
-          if constexpr (kFetch != 0)
-#pragma unroll
-            for (int c = (ahead - G) * kP; c < (ahead - G + 1) * kP; ++c) {
+          for (int op = slot; op < 1 + kJ + kP; op += C::NJ) {
+            if (op == 0) {
+              if (ahead < G) fi[ahead / C::NI][ahead % C::NI] = read_i(ahead % C::NI, now, ahead / C::NI);
+              else if (decltype(more)::value) fi[0][ahead % C::NI] = read_i(ahead % C::NI, next, 0);
+            } else if (op <= kJ) {
+              if (q >= C::NI - L - 1 && q < C::NI - 1) {
+                const int j = (q - (C::NI - L - 1)) * kJ + op - 1;
+                if (j < C::NJ) fj[1][j] = read_j(j, now, 1);
+              } else if (ahead >= G && decltype(more)::value) {
+                const int j = (ahead - G) * kJ + op - 1;
+                if (j < C::NJ) fj[0][j] = read_j(j, next, 0);
+              }
+            } else if (ahead >= G && kFetch != 0) {
+              const int c = (ahead - G) * kP + op - 1 - kJ;
               if (c < SI::kChunks) a.template fetch<kFetch == 2>(c, pa, si, k0, now);
               else if (c < kPieces) b.template fetch<kFetch == 2>(c - SI::kChunks, pb, sj, k0, now + SI::kBytes);
             }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+          }
+        };
 #pragma unroll
-        for (int j = 0; j < C::NJ; ++j) acc[j][q % C::NI] = Frag<T>::mma(fj[q / C::NI][j], fi[q / C::NI][q % C::NI], acc[j][q % C::NI]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < C::NJ; ++j) {
+          acc[j][q % C::NI] = Frag<T>::mma(fj[q / C::NI][j], fi[q / C::NI][q % C::NI], acc[j][q % C::NI]);
+          __builtin_amdgcn_sched_barrier(0);
+          others(j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if constexpr (kFetch != 0) advance();
     };
@@ -284,6 +290,40 @@ __device__ __forceinline__ void accumulate(f32x4_t (&acc)[C::NJ][C::NI], const S
   p.run(acc, si, sj, i0, j0, steps_per, first, last, lds);
 }
 
+// A workgroup's results on their way to memory: a lane holds 4 neighbouring j of 16 rows' worth of lanes,
+// 32 bytes of a row, so a tile goes through LDS (rows 16 bytes longer than their values: the 16 rows a
+// write touches start in different banks) and leaves in 16-byte stores of whole lines.
+template <typename O, int COLS>
+struct Out {
+  typedef O V4 __attribute__((ext_vector_type(4)));
+  static constexpr int kRow = COLS * int(sizeof(O)) + 16, kV = 16 / int(sizeof(O));
+  typedef O V __attribute__((ext_vector_type(kV)));
+
+  static __device__ __forceinline__ void put(char* lds, int r, int c, f32x4_t v) {
+    V4 o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = O(v[k]);
+    *reinterpret_cast<V4*>(lds + r * kRow + c * sizeof(O)) = o;
+  }
+  // rows [0, ROWS) of the tile at (row0, col0) of an m x n matrix; wide: its rows allow 16-byte stores
+  template <int ROWS, int NT>
+  static __device__ __forceinline__ void flush(const char* lds, O* out, long ld, long row0, long col0, long m, long n, bool wide) {
+    constexpr int kAcross = COLS / kV;
+#pragma unroll 4
+    for (int at = threadIdx.x; at < ROWS * kAcross; at += NT) {
+      const int r = at / kAcross, c = at % kAcross * kV;
+      const long row = row0 + r, col = col0 + c;
+      if (row >= m || col >= n) continue;
+      const V v = *reinterpret_cast<const V*>(lds + r * kRow + c * sizeof(O));
+      O* to = out + row * ld + col;
+      if (wide && col + kV <= n) *reinterpret_cast<V*>(to) = v;
+      else
+#pragma unroll
+        for (int k = 0; k < kV; ++k)
+          if (col + k < n) to[k] = v[k];
+    }
+  }
+};
 // Four neighbouring values of a row; `wide`: the row's address allows one store.
 template <typename O>
 struct alignas(sizeof(O) * 4) Out4 {

@@ -33,9 +33,14 @@ __device__ __forceinline__ void activate(int kind, float g, float& a, float& d) 
 // The 256 x 256 tile of 8 waves carries long products; the 128 x 128 tile of 4 waves (two workgroups a CU)
 // fills the machine where there are few tiles.
 typedef Tile<2, 4, 8, 4> Large;
-typedef Tile<4, 2, 4, 8> LargeBack;
+typedef Tile<2, 4, 8, 4> LargeBack;
 
 typedef Tile<2, 2, 4, 4> Small;
+
+// LDS of a tile kernel: two stages, later the results of kRows rows (and all columns) of C columns
+template <typename C>
+constexpr int stages() { return 2 * (C::TI + C::TJ) * 128; }
+constexpr int larger(int a, int b) { return a > b ? a : b; }
 
 // 32-bit operands run on the f16 matrix cores as two halves each, x 2^e = hi + lo with e from the largest
 // value of the operand's row (or column, where the sum runs over rows), so that hi lies in [2^-14, 2^15] and
@@ -51,29 +56,29 @@ __device__ __forceinline__ int exponent(unsigned top) { return 141 - max(int(top
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
 template <typename T, typename C, typename O>
-__global__ __launch_bounds__(C::NT, C::kWaves) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
+__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
+  typedef Out<O, C::TJ / 2> W;
+  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
   unsigned ti, tj;
   tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * (C::TJ / 2);
   f32x4_t acc[C::NJ][C::NI] = {};
   accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long ib = i0 + (wave / C::WJ) * C::NI * 16 + (l & 15), jb = j0 + (wave % C::WJ) * (C::NJ / 2) * 16 + (l >> 4) * 4;
+  const int ib = (wave / C::WJ) * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * (C::NJ / 2) * 16 + (l >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
 #pragma unroll
     for (int j = 0; j < C::NJ / 2; ++j) {
-      const long row = ib + i * 16, col = jb + j * 16;
-      if (row >= rows || col >= ld_h) continue;
+      const long row = i0 + ib + i * 16, col = j0 + jb + j * 16;
       f32x4_t o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float a, d, g = acc[j][i][r], u = acc[j + C::NJ / 2][i][r];
         const bool in = col + r < hidden;
-        if (kScaled && in) {
+        if (kScaled && in && row < rows) {
           const int e = exponent(sc.x[row]);
           g = ldexpf(g, -e - exponent(sc.wg[col + r]));
           u = ldexpf(u, -e - exponent(sc.wu[col + r]));
@@ -81,19 +86,22 @@ __global__ __launch_bounds__(C::NT, C::kWaves) void gate_mma_kernel(Side x, Side
         activate(kind, g, a, d);
         o[r] = in ? a * u : 0.0f;
       }
-      store_row4(h + row * ld_h, col, ld_h, true, o);
+      W::put(lds, ib + i * 16, jb + j * 16, o);
     }
+  __syncthreads();
+  W::template flush<C::TI, C::NT>(lds, h, ld_h, i0, j0, rows, ld_h, true);
 }
 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
 // and h, dg and du of the tile from the three.
 template <typename T, typename C, typename O>
-__global__ __launch_bounds__(C::NT, C::kWaves) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
+__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
                                                                  int kind, O* h, O* dg, O* du, long ld_h, long rows, long hidden,
                                                                  unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
   typedef Tile<C::WI, C::WJ, C::NI, C::NJ / 2> Half;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
+  typedef Out<O, Half::TJ> W;
+  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
   unsigned ti, tj;
   tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * Half::TJ;
@@ -101,19 +109,18 @@ __global__ __launch_bounds__(C::NT, C::kWaves) void gate_back_mma_kernel(Side x,
   accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
   accumulate<T, Half, true, false, 1>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy * segs, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long ib = i0 + (wave / C::WJ) * C::NI * 16 + (l & 15), jb = j0 + (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
+  const int ib = (wave / C::WJ) * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
 #pragma unroll
     for (int j = 0; j < Half::NJ; ++j) {
-      const long row = ib + i * 16, col = jb + j * 16;
-      if (row >= rows || col >= ld_h) continue;
-      f32x4_t oh, og, ou;
+      const long row = i0 + ib + i * 16, col = j0 + jb + j * 16;
+      f32x4_t oh;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float a, s, g = acc[j][i][r], u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
         const bool in = col + r < hidden;
-        if (kScaled && in) {
+        if (kScaled && in && row < rows) {
           const int e = exponent(sc.x[row]);
           g = ldexpf(g, -e - exponent(sc.wg[col + r]));
           u = ldexpf(u, -e - exponent(sc.wu[col + r]));
@@ -121,13 +128,23 @@ __global__ __launch_bounds__(C::NT, C::kWaves) void gate_back_mma_kernel(Side x,
         }
         activate(kind, g, a, s);
         oh[r] = in ? a * u : 0.0f;
-        og[r] = in ? d * u * s : 0.0f;
-        ou[r] = in ? d * a : 0.0f;
+        acc[j][i][r] = in ? d * u * s : 0.0f;               // dg and du take g's and u's place
+        acc[j + Half::NJ][i][r] = in ? d * a : 0.0f;
       }
-      store_row4(h + row * ld_h, col, ld_h, true, oh);
-      store_row4(dg + row * ld_h, col, ld_h, true, og);
-      store_row4(du + row * ld_h, col, ld_h, true, ou);
+      W::put(lds, ib + i * 16, jb + j * 16, oh);
     }
+  __syncthreads();
+  W::template flush<C::TI, C::NT>(lds, h, ld_h, i0, j0, rows, ld_h, true);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int j = 0; j < Half::NJ; ++j) W::put(lds, ib + i * 16, jb + j * 16, acc[j + k * Half::NJ][i]);
+    __syncthreads();
+    W::template flush<C::TI, C::NT>(lds, k ? du : dg, ld_h, i0, j0, rows, ld_h, true);
+  }
 }
 
 // C(i, j) of up to three problems in one launch, the sum over k cut into `splits` where tiles are few: then
@@ -151,23 +168,24 @@ struct Problems {
   int n;
   float* part;
 };
-template <typename C, typename O>
-__device__ __forceinline__ void store_tile(const Problem& p, unsigned ti, unsigned tj, int i, int j, f32x4_t v) {
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long row = long(ti) * C::TI + ((wave / C::WJ) * C::NI + i) * 16 + (l & 15);
-  const long col = long(tj) * C::TJ + ((wave % C::WJ) * C::NJ + j) * 16 + (l >> 4) * 4;
-  if (row >= p.m || col >= p.n) return;
-  if (sizeof(O) == 4) {
+// 32-bit results: the operands' scales taken out
+template <typename O>
+__device__ __forceinline__ f32x4_t scaled(const Problem& p, long row, long col, f32x4_t v) {
+  if (sizeof(O) == 4 && row < p.m) {
     const int e = exponent(p.top_i[row]);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (col + r < p.n) v[r] = ldexpf(v[r], -e - exponent(p.top_j[col + r]));
   }
-  store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, v);
+  return v;
 }
 template <typename T, typename C, bool IK, bool JK, typename O>
-__global__ __launch_bounds__(C::NT, C::kWaves) void product_mma_kernel(Problems all) {
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (C::TI + C::TJ) * 128];
+__global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
+  // the results of 4-byte types leave in two passes of half the rows
+  typedef Out<O, C::TJ> W;
+  constexpr int kPasses = sizeof(O) == 4 ? 2 : 1, kRows = C::TI / kPasses;
+  static_assert(kPasses == 1 || C::WI % kPasses == 0, "a pass is whole waves");
+  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), kRows * W::kRow)];
   int k = 0;
   while (k + 1 < all.n && blockIdx.x >= all.p[k + 1].first) ++k;
   const Problem& p = all.p[k];
@@ -179,10 +197,22 @@ __global__ __launch_bounds__(C::NT, C::kWaves) void product_mma_kernel(Problems 
   const int total = p.steps * p.segs, first = int(split) * p.per, last = first + p.per < total ? first + p.per : total;
   accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, long(ti) * C::TI, long(tj) * C::TJ, p.steps, first, last, lds_addr(lds));
   if (p.splits == 1) {
+    const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
+    const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * C::NJ * 16 + (l >> 4) * 4;
+    const long i0 = long(ti) * C::TI, j0 = long(tj) * C::TJ;
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i)
+    for (int pass = 0; pass < kPasses; ++pass) {
+      if (wi / (C::WI / kPasses) == pass) {
 #pragma unroll
-      for (int j = 0; j < C::NJ; ++j) store_tile<C, O>(p, ti, tj, i, j, acc[j][i]);
+        for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+          for (int j = 0; j < C::NJ; ++j)
+            W::put(lds, ib + i * 16 - pass * kRows, jb + j * 16, scaled<O>(p, i0 + ib + i * 16, j0 + jb + j * 16, acc[j][i]));
+      }
+      __syncthreads();
+      W::template flush<kRows, C::NT>(lds, static_cast<O*>(p.out), p.ld, i0 + pass * kRows, j0, p.m, p.n, p.wide);
+      if (pass + 1 < kPasses) __syncthreads();
+    }
   } else {
     f32x4_t* part = reinterpret_cast<f32x4_t*>(all.part) + (p.part + long(split) * tiles + long(ti) * p.tiles_j + tj) * (C::NI * C::NJ * C::NT);
 #pragma unroll
@@ -201,7 +231,10 @@ __global__ __launch_bounds__(C::NT) void join_kernel(Problem p, const float* par
   f32x4_t v = part[0];
 #pragma unroll 4
   for (unsigned s = 1; s < p.splits; ++s) v += part[s * step];
-  store_tile<C, O>(p, tile / p.tiles_j, tile % p.tiles_j, f / C::NJ, f % C::NJ, v);
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const long row = long(tile / p.tiles_j) * C::TI + ((wave / C::WJ) * C::NI + f / C::NJ) * 16 + (l & 15);
+  const long col = long(tile % p.tiles_j) * C::TJ + ((wave % C::WJ) * C::NJ + f % C::NJ) * 16 + (l >> 4) * 4;
+  if (row < p.m && col < p.n) store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, scaled<O>(p, row, col, v));
 }
 
 // Rows of `n` values copied to rows of a multiple of 8, zeros behind: operands whose rows are not whole
@@ -575,7 +608,7 @@ template <typename O>
 Problem problem(const Side& i, const Side& j, long m, long n, long k, int segs, void* out, long ld) {
   Problem p{};
   p.i = i, p.j = j, p.m = m, p.n = n, p.out = out, p.ld = ld, p.steps = int((k + 63) / 64), p.segs = segs;
-  p.wide = !(uintptr_t(out) & (4 * sizeof(O) - 1)) && ld % 4 == 0;
+  p.wide = !(uintptr_t(out) & 15) && ld % (16 / long(sizeof(O))) == 0;
   return p;
 }
 
