@@ -343,12 +343,15 @@ __device__ __forceinline__ void store_row4(O* row, long j, long n, bool wide, f3
   }
 }
 
-// Workgroup b of n as a tile number: workgroups go round the 8 XCDs, so every XCD gets a contiguous run of
-// tiles and its L2 holds the operand rows they share; runs go down `group` rows of tiles before the next
-// column.
-__device__ __forceinline__ void tile_of(unsigned b, unsigned n, unsigned tiles_i, unsigned tiles_j, unsigned& ti, unsigned& tj) {
-  const unsigned q = n / 8, r = n % 8, x = b % 8, y = b / 8;
-  const unsigned at = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + y;
+// Workgroup b of n, renumbered within each wave of `slots` that run at a time, so that the workgroups of one XCD
+// (they go round all 8) are neighbours there: its L2 holds the operand rows that neighbouring tiles share, and all
+// XCDs meet in the same rows in memory's cache.
+__device__ __forceinline__ unsigned near(unsigned b, unsigned n, unsigned slots) {
+  const unsigned w = b / slots * slots, m = n - w < slots ? n - w : slots, q = m / 8, r = m % 8, x = b % 8, y = (b - w) / 8;
+  return w + (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + y;
+}
+// Tile number `at`: down 8 rows of tiles, then the next column.
+__device__ __forceinline__ void tile_of(unsigned at, unsigned tiles_i, unsigned tiles_j, unsigned& ti, unsigned& tj) {
   constexpr unsigned kGroup = 8;
   const unsigned full = kGroup * tiles_j, gi = at / full, left = at - gi * full;
   const unsigned rows = tiles_i - gi * kGroup < kGroup ? tiles_i - gi * kGroup : kGroup;

@@ -13,29 +13,63 @@
 namespace nerf {
 namespace {
 
-// act(g) and act'(g)
-__device__ __forceinline__ void activate(int kind, float g, float& a, float& d) {
-  if (kind == NERF_RELU) {
+// exp(x) to 2^-22 or better: the part of x log2 e that its rounding loses is put back; the clamp keeps
+// infinities out of the difference (exp(200) is an infinity and exp(-200) zero in fp32).
+__device__ __forceinline__ float exp_fast(float x) {
+  x = __builtin_amdgcn_fmed3f(x, -200.0f, 200.0f);
+  const float y = x * 1.44269504f;
+  const float r = fmaf(x, 1.44269504f, -y) + x * 1.92596299e-8f;
+  return __builtin_amdgcn_exp2f(y) * fmaf(r, 0.693147181f, 1.0f);
+}
+// act(g) and act'(g), without branches: they run on every accumulator of a tile, where a kind chosen at run
+// time and the library's erfcf were hundreds of branches (the forward's at 131072 x 256 x 512: 148 -> 108 us)
+template <int KIND>
+__device__ __forceinline__ void activate(float g, float& a, float& d) {
+  if constexpr (KIND == NERF_RELU) {
     a = g > 0.0f ? g : (g != g ? g : 0.0f);
     d = g > 0.0f ? 1.0f : 0.0f;
-  } else if (kind == NERF_SILU) {
-    const float e = 1.0f / (1.0f + expf(-g));
+  } else if constexpr (KIND == NERF_SILU) {
+    const float e = __builtin_amdgcn_rcpf(1.0f + exp_fast(-g));
     a = g * e;
     d = e * (1.0f + g * (1.0f - e));
   } else {
-    const float c = 0.5f * erfcf(-g * 0.70710678118654752440f);
+    // Phi(g) = 1 - erfc(z) / 2 for g >= 0 and erfc(z) / 2 below, z = |g| / sqrt 2, with erfc(z) = e^(-z^2) t P(t),
+    // t = 1 / (1 + 0.3 z): P fitted to e^(z^2) erfc(z) / t on [0, 14] in fp64, relative error 4e-8
+    const float z = fabsf(g) * 0.707106781f, t = __builtin_amdgcn_rcpf(fmaf(0.3f, z, 1.0f));
+    float q = -0.1266212098340432f;
+    q = fmaf(q, t, 0.4718487095901134f);
+    q = fmaf(q, t, -0.4847378408362197f);
+    q = fmaf(q, t, 0.5171006909279582f);
+    q = fmaf(q, t, -0.07408421230047764f);
+    q = fmaf(q, t, 0.20639971292244577f);
+    q = fmaf(q, t, 0.15046525403500766f);
+    q = fmaf(q, t, 0.17042420882459997f);
+    q = fmaf(q, t, 0.16920472558993327f);
+    const float h = g * g, low = fmaf(g, g, -h);                          // g^2 = h + low
+    const float e = exp_fast(-0.5f * h) * fmaf(-0.5f, h < 1e30f ? low : 0.0f, 1.0f);
+    const float tail = 0.5f * e * t * q;
+    const float c = g >= 0.0f ? 1.0f - tail : (g < 0.0f ? tail : g);      // NaN stays
     a = g * c;
-    d = c + g * expf(-0.5f * g * g) * 0.39894228040143267794f;
+    d = c + g * e * 0.39894228040143267794f;
   }
+}
+template <typename F>
+__host__ __device__ inline void with_kind(int kind, F f) {
+  if (kind == NERF_RELU) f(std::integral_constant<int, NERF_RELU>{});
+  else if (kind == NERF_SILU) f(std::integral_constant<int, NERF_SILU>{});
+  else f(std::integral_constant<int, NERF_GELU>{});
 }
 
 // ------------------------------------------------------------------ 16-bit types on the matrix cores --
 // The 256 x 256 tile of 8 waves carries long products; the 128 x 128 tile of 4 waves (two workgroups a CU)
 // fills the machine where there are few tiles.
 typedef Tile<2, 4, 8, 4> Large;
-typedef Tile<2, 4, 8, 4> LargeBack;
-
 typedef Tile<2, 2, 4, 4> Small;
+
+template <typename C>
+__host__ __device__ constexpr bool is_large() { return C::TI * C::TJ > 128 * 128; }
+template <typename C>
+__host__ __device__ constexpr long slots() { return is_large<C>() ? 256 : 512; }
 
 // LDS of a tile kernel: two stages, later the results of kRows rows (and all columns) of C columns
 template <typename C>
@@ -55,14 +89,14 @@ __device__ __forceinline__ int exponent(unsigned top) { return 141 - max(int(top
 // h = act(x Wg^T) (x Wu^T): the J tile holds TJ / 2 rows of Wg and the same rows of Wu, so a lane owns the
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
-template <typename T, typename C, typename O>
-__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, int kind, O* h, long ld_h, long rows,
+template <typename T, typename C, typename O, int KIND>
+__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
   typedef Out<O, C::TJ / 2> W;
   __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
   unsigned ti, tj;
-  tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
+  tile_of(near(blockIdx.x, gridDim.x, slots<C>()), tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * (C::TJ / 2);
   f32x4_t acc[C::NJ][C::NI] = {};
   accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
@@ -83,7 +117,7 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
           g = ldexpf(g, -e - exponent(sc.wg[col + r]));
           u = ldexpf(u, -e - exponent(sc.wu[col + r]));
         }
-        activate(kind, g, a, d);
+        activate<KIND>(g, a, d);
         o[r] = in ? a * u : 0.0f;
       }
       W::put(lds, ib + i * 16, jb + j * 16, o);
@@ -94,80 +128,124 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
 // and h, dg and du of the tile from the three.
-template <typename T, typename C, typename O>
+template <typename T, typename C, typename O, int KIND>
 __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
-                                                                 int kind, O* h, O* dg, O* du, long ld_h, long rows, long hidden,
+                                                                 O* h, O* dg, O* du, long ld_h, long rows, long hidden,
                                                                  unsigned tiles_i, unsigned tiles_j, Scales sc) {
   constexpr bool kScaled = sizeof(O) == 4;
   typedef Tile<C::WI, C::WJ, C::NI, C::NJ / 2> Half;
   typedef Out<O, Half::TJ> W;
-  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
+  // results of 4-byte types leave in two passes of half the rows; h and dg leave together, then du
+  constexpr int kPasses = sizeof(O) == 4 ? 2 : 1, kRows = C::TI / kPasses, kImage = kRows * W::kRow;
+  static_assert(C::WI % kPasses == 0, "a pass is whole waves");
+  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), 2 * kImage)];
   unsigned ti, tj;
-  tile_of(blockIdx.x, gridDim.x, tiles_i, tiles_j, ti, tj);
+  tile_of(near(blockIdx.x, gridDim.x, slots<C>()), tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * Half::TJ;
   f32x4_t acc[C::NJ][C::NI] = {}, dh[Half::NJ][C::NI] = {};
   accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
   accumulate<T, Half, true, false, 1>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy * segs, lds_addr(lds));
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const int ib = (wave / C::WJ) * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
+  const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
 #pragma unroll
-  for (int i = 0; i < C::NI; ++i)
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const bool mine = wi / (C::WI / kPasses) == pass;
+    const int row0 = ib - pass * kRows;
+    if (pass) __syncthreads();
+    if (mine) {
 #pragma unroll
-    for (int j = 0; j < Half::NJ; ++j) {
-      const long row = i0 + ib + i * 16, col = j0 + jb + j * 16;
-      f32x4_t oh;
+      for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float a, s, g = acc[j][i][r], u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
-        const bool in = col + r < hidden;
-        if (kScaled && in && row < rows) {
-          const int e = exponent(sc.x[row]);
-          g = ldexpf(g, -e - exponent(sc.wg[col + r]));
-          u = ldexpf(u, -e - exponent(sc.wu[col + r]));
-          d = ldexpf(d, -exponent(sc.dy[row]) - exponent(sc.wd[col + r]));
+        for (int j = 0; j < Half::NJ; ++j) {
+          const int left = int(hidden - j0 < Half::TJ ? hidden - j0 : Half::TJ) - jb - j * 16;    // columns of this lane's four
+          f32x4_t oh, og, ou;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float a, s, g = acc[j][i][r], u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
+            if (kScaled && r < left && i0 + ib + i * 16 < rows) {
+              const long row = i0 + ib + i * 16, col = j0 + jb + j * 16 + r;
+              const int e = exponent(sc.x[row]);
+              g = ldexpf(g, -e - exponent(sc.wg[col]));
+              u = ldexpf(u, -e - exponent(sc.wu[col]));
+              d = ldexpf(d, -exponent(sc.dy[row]) - exponent(sc.wd[col]));
+            }
+            activate<KIND>(g, a, s);
+            oh[r] = r < left ? a * u : 0.0f;
+            og[r] = r < left ? d * u * s : 0.0f;
+            ou[r] = r < left ? d * a : 0.0f;
+          }
+          W::put(lds, row0 + i * 16, jb + j * 16, oh);
+          W::put(lds + kImage, row0 + i * 16, jb + j * 16, og);
+          dh[j][i] = ou;                         // waits in dh's place
+          // one fragment's temporaries at a time: g, u and dh fill the registers (keeping dg there too: 154 spilled)
+          __builtin_amdgcn_sched_barrier(0);
         }
-        activate(kind, g, a, s);
-        oh[r] = in ? a * u : 0.0f;
-        acc[j][i][r] = in ? d * u * s : 0.0f;               // dg and du take g's and u's place
-        acc[j + Half::NJ][i][r] = in ? d * a : 0.0f;
-      }
-      W::put(lds, ib + i * 16, jb + j * 16, oh);
     }
-  __syncthreads();
-  W::template flush<C::TI, C::NT>(lds, h, ld_h, i0, j0, rows, ld_h, true);
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-      for (int j = 0; j < Half::NJ; ++j) W::put(lds, ib + i * 16, jb + j * 16, acc[j + k * Half::NJ][i]);
+    W::template flush<kRows, C::NT>(lds, h, ld_h, i0 + pass * kRows, j0, rows, ld_h, true);
+    W::template flush<kRows, C::NT>(lds + kImage, dg, ld_h, i0 + pass * kRows, j0, rows, ld_h, true);
     __syncthreads();
-    W::template flush<C::TI, C::NT>(lds, k ? du : dg, ld_h, i0, j0, rows, ld_h, true);
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < Half::NJ; ++j) W::put(lds, row0 + i * 16, jb + j * 16, dh[j][i]);
+    }
+    __syncthreads();
+    W::template flush<kRows, C::NT>(lds, du, ld_h, i0 + pass * kRows, j0, rows, ld_h, true);
   }
 }
 
-// C(i, j) of up to three problems in one launch, the sum over k cut into `splits` where tiles are few: then
-// each piece leaves fp32 partials (fragment order: neighbouring threads, neighbouring 16 bytes) that
-// join_kernel adds in order.
+// C(i, j) of up to three problems at once.  Their tiles (numbered through) are shared out
+//   whole, as many full waves of workgroups as there are (product_mma_kernel), and the remaining tiles' steps
+//   evenly over `streams` workgroups, each a run of steps that may end one tile and begin the next; or
+//   where tiles are few, all of them cut into the same `cuts` pieces of k: the workgroups of one piece read
+//   the same rows and lie on one XCD.
+// parts_mma_kernel's fp32 partials (neighbouring threads, neighbouring 16 bytes) are added by join_kernel in
+// order.  One kernel for both kinds of tile had 49 spilled registers and lost 7% at whole tiles.
 struct Problem {
   Side i, j;
   void* out;
   long ld;           // elements
   long m, n;         // C is m x n; a side whose rows were padded to 8 has a larger extent
-  int steps;         // steps of 64 k of one segment
-  int segs;
-  int per;           // steps of a piece
-  unsigned splits, tiles_i, tiles_j, first;   // first workgroup
-  long part;         // first partial tile of this problem
+  unsigned tiles_i, tiles_j, first;   // first tile
   int wide;
   const unsigned *top_i, *top_j;   // 32-bit operands' scales
 };
 struct Problems {
   Problem p[3];
   int n;
+  int steps;         // steps of 64 k of one segment
+  int total;         // steps of all segments
+  unsigned tiles, whole, streams;     // tiles, workgroups of whole ones, of parts
+  int cuts, per;     // steps of a stream or of a piece
   float* part;
 };
+// Part `n` of the stream (which lies on one tile or two) or piece b: false if there is none.
+struct Part {
+  unsigned tile;
+  int first, last;
+  unsigned slot;      // its partials
+};
+__device__ __forceinline__ bool part_of(const Problems& all, unsigned b, int n, Part& out) {
+  const unsigned rest = all.tiles - all.whole;
+  if (all.cuts) {
+    const unsigned cut = b / rest;
+    out.tile = all.whole + b % rest;
+    out.first = int(cut) * all.per;
+    out.last = min(out.first + all.per, all.total);
+    out.slot = b;
+    return n == 0;
+  }
+  const long lo = long(b) * all.per, end = long(rest) * all.total, hi = lo + all.per < end ? lo + all.per : end;
+  const long tile = lo / all.total + n, start = tile * all.total;
+  if (start >= hi) return false;
+  out.tile = all.whole + unsigned(tile);
+  out.first = int(n ? 0 : lo - start);
+  out.last = int(hi - start < all.total ? hi - start : all.total);
+  out.slot = 2 * b + n;
+  return true;
+}
 // 32-bit results: the operands' scales taken out
 template <typename O>
 __device__ __forceinline__ f32x4_t scaled(const Problem& p, long row, long col, f32x4_t v) {
@@ -179,29 +257,24 @@ __device__ __forceinline__ f32x4_t scaled(const Problem& p, long row, long col, 
   }
   return v;
 }
-template <typename T, typename C, bool IK, bool JK, typename O>
-__global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
-  // the results of 4-byte types leave in two passes of half the rows
-  typedef Out<O, C::TJ> W;
-  constexpr int kPasses = sizeof(O) == 4 ? 2 : 1, kRows = C::TI / kPasses;
-  static_assert(kPasses == 1 || C::WI % kPasses == 0, "a pass is whole waves");
-  __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), kRows * W::kRow)];
+__device__ __forceinline__ const Problem& problem_of(const Problems& all, unsigned tile) {
   int k = 0;
-  while (k + 1 < all.n && blockIdx.x >= all.p[k + 1].first) ++k;
-  const Problem& p = all.p[k];
-  const unsigned tiles = p.tiles_i * p.tiles_j, b = blockIdx.x - p.first;
-  const unsigned split = b / tiles;
-  unsigned ti, tj;
-  tile_of(b - split * tiles, tiles, p.tiles_i, p.tiles_j, ti, tj);
-  f32x4_t acc[C::NJ][C::NI] = {};
-  const int total = p.steps * p.segs, first = int(split) * p.per, last = first + p.per < total ? first + p.per : total;
-  accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, long(ti) * C::TI, long(tj) * C::TJ, p.steps, first, last, lds_addr(lds));
-  if (p.splits == 1) {
+  while (k + 1 < all.n && tile >= all.p[k + 1].first) ++k;
+  return all.p[k];
+}
+// The accumulators of a whole tile to its place; the results of 4-byte types leave in two passes of half the rows.
+template <typename C, typename O>
+struct Leave {
+  typedef Out<O, C::TJ> W;
+  static constexpr int kPasses = sizeof(O) == 4 ? 2 : 1, kRows = C::TI / kPasses;
+  static_assert(C::WI % kPasses == 0, "a pass is whole waves");
+  static constexpr int kLds = larger(stages<C>(), kRows * W::kRow);
+  static __device__ __forceinline__ void run(char* lds, const Problem& p, long i0, long j0, const f32x4_t (&acc)[C::NJ][C::NI]) {
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
     const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * C::NJ * 16 + (l >> 4) * 4;
-    const long i0 = long(ti) * C::TI, j0 = long(tj) * C::TJ;
 #pragma unroll
     for (int pass = 0; pass < kPasses; ++pass) {
+      if (pass) __syncthreads();
       if (wi / (C::WI / kPasses) == pass) {
 #pragma unroll
         for (int i = 0; i < C::NI; ++i)
@@ -211,29 +284,61 @@ __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
       }
       __syncthreads();
       W::template flush<kRows, C::NT>(lds, static_cast<O*>(p.out), p.ld, i0 + pass * kRows, j0, p.m, p.n, p.wide);
-      if (pass + 1 < kPasses) __syncthreads();
     }
-  } else {
-    f32x4_t* part = reinterpret_cast<f32x4_t*>(all.part) + (p.part + long(split) * tiles + long(ti) * p.tiles_j + tj) * (C::NI * C::NJ * C::NT);
+  }
+};
+template <typename T, typename C, bool IK, bool JK, typename O>
+__global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
+  __shared__ __attribute__((aligned(1024))) char lds[Leave<C, O>::kLds];
+  const unsigned tile = near(blockIdx.x, gridDim.x, slots<C>());
+  const Problem& p = problem_of(all, tile);
+  unsigned ti, tj;
+  tile_of(tile - p.first, p.tiles_i, p.tiles_j, ti, tj);
+  const long i0 = long(ti) * C::TI, j0 = long(tj) * C::TJ;
+  f32x4_t acc[C::NJ][C::NI] = {};
+  accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, i0, j0, all.steps, 0, all.total, lds_addr(lds));
+  Leave<C, O>::run(lds, p, i0, j0, acc);
+}
+template <typename T, typename C, bool IK, bool JK>
+__global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
+  __shared__ __attribute__((aligned(1024))) char lds[stages<C>()];
+  const unsigned b = near(blockIdx.x, gridDim.x, slots<C>());
+  Part part;
+  for (int n = 0; n < 2 && part_of(all, b, n, part); ++n) {
+    const Problem& p = problem_of(all, part.tile);
+    unsigned ti, tj;
+    tile_of(part.tile - p.first, p.tiles_i, p.tiles_j, ti, tj);
+    f32x4_t acc[C::NJ][C::NI] = {};
+    accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, long(ti) * C::TI, long(tj) * C::TJ, all.steps, part.first, part.last, lds_addr(lds));
+    f32x4_t* to = reinterpret_cast<f32x4_t*>(all.part) + long(part.slot) * (C::NI * C::NJ * C::NT);
 #pragma unroll
     for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-      for (int j = 0; j < C::NJ; ++j) part[(i * C::NJ + j) * C::NT + threadIdx.x] = acc[j][i];
+      for (int j = 0; j < C::NJ; ++j) to[(i * C::NJ + j) * C::NT + threadIdx.x] = acc[j][i];
   }
 }
-// workgroup: one fragment of every wave of one tile
+// workgroup: one fragment of every wave of one of the remaining tiles
 template <typename C, typename O>
-__global__ __launch_bounds__(C::NT) void join_kernel(Problem p, const float* parts) {
-  const unsigned tile = blockIdx.x / (C::NI * C::NJ);
-  const int f = int(blockIdx.x % (C::NI * C::NJ));
-  const long tiles = long(p.tiles_i) * p.tiles_j, step = tiles * (C::NI * C::NJ * C::NT);
-  const f32x4_t* part = reinterpret_cast<const f32x4_t*>(parts) + (p.part + tile) * (C::NI * C::NJ * C::NT) + f * C::NT + threadIdx.x;
-  f32x4_t v = part[0];
+__global__ __launch_bounds__(C::NT) void join_kernel(Problems all) {
+  constexpr int kFrags = C::NI * C::NJ;
+  const unsigned rest = all.tiles - all.whole, r = blockIdx.x / kFrags;
+  const int f = int(blockIdx.x % kFrags);
+  const f32x4_t* part = reinterpret_cast<const f32x4_t*>(all.part) + f * C::NT + threadIdx.x;
+  const long size = kFrags * C::NT;
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (all.cuts) {
 #pragma unroll 4
-  for (unsigned s = 1; s < p.splits; ++s) v += part[s * step];
+    for (int s = 0; s < all.cuts; ++s) v += part[(long(s) * rest + r) * size];
+  } else {
+    const long lo = long(r) * all.total, hi = lo + all.total, b0 = lo / all.per, b1 = (hi - 1) / all.per;
+    for (long b = b0; b <= b1; ++b) v += part[(2 * b + (b * all.per < lo ? 1 : 0)) * size];
+  }
+  const Problem& p = problem_of(all, all.whole + r);
+  unsigned ti, tj;
+  tile_of(all.whole + r - p.first, p.tiles_i, p.tiles_j, ti, tj);
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  const long row = long(tile / p.tiles_j) * C::TI + ((wave / C::WJ) * C::NI + f / C::NJ) * 16 + (l & 15);
-  const long col = long(tile % p.tiles_j) * C::TJ + ((wave % C::WJ) * C::NJ + f % C::NJ) * 16 + (l >> 4) * 4;
+  const long row = long(ti) * C::TI + ((wave / C::WJ) * C::NI + f / C::NJ) * 16 + (l & 15);
+  const long col = long(tj) * C::TJ + ((wave % C::WJ) * C::NJ + f % C::NJ) * 16 + (l >> 4) * 4;
   if (row < p.m && col < p.n) store_row4(static_cast<O*>(p.out) + row * p.ld, col, p.n, p.wide, scaled<O>(p, row, col, v));
 }
 
@@ -364,15 +469,18 @@ __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
   const int row = i * 16 + e, col = j0 + g * 4;
   if (row >= p.rows) return;
   T* out = static_cast<T*>(p.out) + row * p.ld_out;
+  if (MODE == kGate)
+    with_kind(p.kind, [&](auto k) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v, d;
+        activate<decltype(k)::value>(a[r], v, d);
+        a[r] = v * b[r];
+      }
+    });
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float v = a[r], d;
-    if (MODE == kGate) {
-      activate(p.kind, a[r], v, d);
-      v *= b[r];
-    } else if (MODE == kHalves) {
-      v += b[r];
-    }
+    const float v = MODE == kHalves ? a[r] + b[r] : a[r];
     if (col + r < p.n_out) out[col + r] = T(col + r < p.n ? v : 0.0f);
   }
 }
@@ -507,12 +615,14 @@ constexpr long align_up(long n, long a) { return (n + a - 1) / a * a; }
 // Takes memory from the workspace; with no base it only counts.
 struct Arena {
   char* base;
-  size_t used = 0;
+  size_t used = 0, most = 0;
   void* take(size_t bytes) {
     void* p = base ? base + used : nullptr;
     used += size_t(align_up(long(bytes), 256));
+    reserve(0);
     return p;
   }
+  void reserve(size_t bytes) { most = used + bytes > most ? used + bytes : most; }   // behind what is taken
 };
 
 // A 16-bit matrix [rows][n] as a product reads it: where it lies, or a padded copy.
@@ -534,12 +644,26 @@ Side columns_side(const Matrix& m) {   // i = column, k = row
   return s;
 }
 
-// Large tiles where they fill the machine nearly as well as small ones do: a small tile runs its products
-// at about 3/4 of the large one's rate.
-bool use_large(long m, long n) {
-  const long l = ((m + 255) / 256) * ((n + 255) / 256), s = ((m + 127) / 128) * ((n + 127) / 128);
-  const double fl = double(l) / (256.0 * ((l + 255) / 256)), fs = double(s) / (512.0 * ((s + 511) / 512));
-  return fl >= 0.75 * fs;
+// What a launch is expected to take, in microseconds, from whole launches of either tile: a step where every
+// workgroup slot is taken and where a CU runs one workgroup alone (it then waits for its operands), what a tile
+// costs besides, a join, and a MiB of partials written or read.
+constexpr double kFullLarge = 1.4, kFullSmall = 1.1, kAlone = 0.9, kTileLarge = 7.0, kTileSmall = 5.0, kJoin = 5.0, kMiB = 0.2;
+long tiles_of(long m, long n, long ti, long tj) { return ((m + ti - 1) / ti) * ((n + tj - 1) / tj); }
+// `n` workgroups of `steps` steps at a time
+template <typename C>
+double wave_time(long n, double steps) {
+  const double full = is_large<C>() ? kFullLarge : kFullSmall, part = full * double(n) / double(slots<C>());
+  return steps * (part > kAlone ? part : kAlone) + (is_large<C>() ? kTileLarge : kTileSmall);
+}
+template <typename C>
+double whole_time(long tiles, double steps) {
+  const long full = tiles / slots<C>(), rest = tiles % slots<C>();
+  return double(full) * wave_time<C>(slots<C>(), steps) + (rest ? wave_time<C>(rest, steps) : 0.0);
+}
+// The gate kernels: whole tiles only, `steps` of both phases.
+bool gate_large(long rows, long cols, long steps) {
+  return whole_time<Large>(tiles_of(rows, cols, Large::TI, Large::TJ), double(steps)) <=
+         whole_time<Small>(tiles_of(rows, cols, Small::TI, Small::TJ), double(steps));
 }
 
 struct Run {
@@ -561,53 +685,78 @@ struct Run {
     return Matrix{q, n8, rows, n, n8};
   }
 
-  // C = the segments' products for up to three problems of one kind; partials come from the arena.
-  template <typename T, bool IK, bool JK, typename O, typename C>
-  void products_of(Problems& all) {
-    unsigned grid = 0;
-    long tiles = 0, parts = 0;
+  // How a launch's tiles are shared out, and what that is expected to take.
+  template <typename C>
+  static double share(Problems& all) {
+    all.tiles = 0;
     for (int k = 0; k < all.n; ++k) {
       Problem& p = all.p[k];
       p.tiles_i = unsigned((p.m + C::TI - 1) / C::TI), p.tiles_j = unsigned((p.n + C::TJ - 1) / C::TJ);
-      tiles += long(p.tiles_i) * p.tiles_j;
+      p.first = all.tiles;
+      all.tiles += p.tiles_i * p.tiles_j;
     }
-    if (tiles == 0) return;      // no rows
-    const long slots = 256L * (C::TI * C::TJ > 128 * 128 ? 1 : 2);
-    for (int k = 0; k < all.n; ++k) {
-      Problem& p = all.p[k];
-      const int total = p.steps * p.segs;
-      // pieces of at least 8 steps, as many as make one full wave of workgroups
-      long splits = tiles < slots ? slots / tiles : 1;
-      splits = splits > total / 8 ? total / 8 : splits;
-      splits = splits < 1 ? 1 : splits;
-      p.per = int((total + splits - 1) / splits);
-      p.splits = total ? unsigned((total + p.per - 1) / p.per) : 1;
-      p.first = grid;
-      p.part = parts;
-      grid += p.tiles_i * p.tiles_j * p.splits;
-      if (p.splits > 1) parts += long(p.tiles_i) * p.tiles_j * p.splits;
+    const long n = slots<C>(), total = all.total, tiles = all.tiles, full = tiles / n, rest = tiles % n;
+    const double mib = C::TI * C::TJ * 4.0 / (1 << 20);
+    all.whole = unsigned(tiles), all.streams = 0, all.cuts = 0, all.per = 0;
+    if (total == 0 || tiles == 0) return 0.0;
+    double best = whole_time<C>(tiles, double(total));
+    if (rest * 2 <= n && full == 0 && total >= 16) {        // few tiles: equal pieces of at least 8 steps
+      long cuts = n / rest < total / 8 ? n / rest : total / 8;
+      const long per = (total + cuts - 1) / cuts;
+      cuts = (total + per - 1) / per;
+      const double t = wave_time<C>(cuts * rest, double(per)) + kJoin + 2 * double(cuts * rest) * mib * kMiB;
+      if (t < best) best = t, all.whole = 0, all.streams = unsigned(cuts * rest), all.cuts = int(cuts), all.per = int(per);
     }
-    all.part = static_cast<float*>(a.take(size_t(parts) * C::TI * C::TJ * 4));
-    if (!go || !grid) return;
-    hipLaunchKernelGGL((product_mma_kernel<T, C, IK, JK, O>), dim3(grid), dim3(C::NT), 0, s, all);
-    for (int k = 0; k < all.n; ++k)
-      if (all.p[k].splits > 1)
-        hipLaunchKernelGGL((join_kernel<C, O>), dim3(all.p[k].tiles_i * all.p[k].tiles_j * C::NI * C::NJ), dim3(C::NT), 0, s, all.p[k],
-                           (const float*)all.part);
+    if (rest && rest * total >= 8 * n) {
+      const long per = (rest * total + n - 1) / n;
+      const double t = whole_time<C>(full * n, double(total)) + wave_time<C>(n, double(per)) + (is_large<C>() ? kTileLarge : kTileSmall) +
+                       kJoin + 2 * double(n + rest) * mib * kMiB;
+      if (t < best) best = t, all.whole = unsigned(full * n), all.streams = unsigned((rest * total + per - 1) / per), all.cuts = 0, all.per = int(per);
+    }
+    return best;
+  }
+  // C = the segments' products for up to three problems of one kind.  Partials lie behind what the arena has
+  // given out so far and are done with when the launches are.
+  template <typename C>
+  static size_t share_bytes(Problems& all) {
+    (void)share<C>(all);
+    return (all.cuts ? size_t(all.streams) : 2 * size_t(all.streams)) * C::TI * C::TJ * 4;
+  }
+  template <typename T, bool IK, bool JK, typename O, typename C>
+  size_t products_of(Problems& all) {
+    const size_t bytes = share_bytes<C>(all);
+    if (!go || !all.tiles) return bytes;
+    all.part = reinterpret_cast<float*>(a.base + a.used);
+    if (all.whole) hipLaunchKernelGGL((product_mma_kernel<T, C, IK, JK, O>), dim3(all.whole), dim3(C::NT), 0, s, all);
+    if (all.streams) {
+      hipLaunchKernelGGL((parts_mma_kernel<T, C, IK, JK>), dim3(all.streams), dim3(C::NT), 0, s, all);
+      hipLaunchKernelGGL((join_kernel<C, O>), dim3((all.tiles - all.whole) * C::NI * C::NJ), dim3(C::NT), 0, s, all);
+    }
+    return bytes;
   }
   template <typename T, bool IK, bool JK, typename O>
-  void products(Problems& all) {
-    bool large = false;
-    for (int k = 0; k < all.n; ++k) large = large || use_large(all.p[k].m, all.p[k].n);
-    if (large) products_of<T, IK, JK, O, Large>(all);
-    else products_of<T, IK, JK, O, Small>(all);
+  size_t products_one(Problems& all, long k, int segs) {
+    all.steps = int((k + 63) / 64), all.total = all.steps * segs;
+    const double large = share<Large>(all), small = share<Small>(all);
+    return large <= small ? products_of<T, IK, JK, O, Large>(all) : products_of<T, IK, JK, O, Small>(all);
+  }
+  template <typename T, bool IK, bool JK, typename O>
+  void products(const Problems& all, long k, int segs) {
+    // the workspace is asked for before it is known which results are wanted, and fewer may need more partials
+    for (int wanted = go ? (1 << all.n) - 1 : 1; wanted < 1 << all.n; ++wanted) {
+      Problems some = all;
+      some.n = 0;
+      for (int q = 0; q < all.n; ++q)
+        if (wanted >> q & 1) some.p[some.n++] = all.p[q];
+      a.reserve(products_one<T, IK, JK, O>(some, k, segs));
+    }
   }
 };
 
 template <typename O>
-Problem problem(const Side& i, const Side& j, long m, long n, long k, int segs, void* out, long ld) {
+Problem problem(const Side& i, const Side& j, long m, long n, void* out, long ld) {
   Problem p{};
-  p.i = i, p.j = j, p.m = m, p.n = n, p.out = out, p.ld = ld, p.steps = int((k + 63) / 64), p.segs = segs;
+  p.i = i, p.j = j, p.m = m, p.n = n, p.out = out, p.ld = ld;
   p.wide = !(uintptr_t(out) & 15) && ld % (16 / long(sizeof(O))) == 0;
   return p;
 }
@@ -643,10 +792,12 @@ void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w,
   const auto go = [&](auto tile) {
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
-    hipLaunchKernelGGL((gate_mma_kernel<T, C, O>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(d.width), segs, d.activation, h, hp,
-                       long(d.rows), long(d.hidden), ti, tj, sc);
+    with_kind(d.activation, [&](auto k) {
+      hipLaunchKernelGGL((gate_mma_kernel<T, C, O, decltype(k)::value>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(d.width), segs, h, hp,
+                         long(d.rows), long(d.hidden), ti, tj, sc);
+    });
   };
-  if (use_large(d.rows, 2 * hp)) go(Large{});
+  if (gate_large(d.rows, 2 * hp, long(steps_of(d.width)) * segs)) go(Large{});
   else go(Small{});
 }
 template <typename T, typename O>
@@ -657,10 +808,12 @@ void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Sid
   const auto go = [&](auto tile) {
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
-    hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(d.width), steps_of(d.out), segs,
-                       d.activation, h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
+    with_kind(d.activation, [&](auto k) {
+      hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O, decltype(k)::value>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(d.width),
+                         steps_of(d.out), segs, h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
+    });
   };
-  if (use_large(d.rows, 2 * hp)) go(LargeBack{});
+  if (gate_large(d.rows, 2 * hp, long(steps_of(d.width) + steps_of(d.out)) * segs)) go(Large{});
   else go(Small{});
 }
 
@@ -696,8 +849,8 @@ hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   launch_gate<T, T>(r, d, rows_side(x), halves(w), 1, h, hp, Scales{});
   Problems all{};
   all.n = 1;
-  all.p[0] = problem<T>(rows_side(Matrix{h, hp, rows, hidden, hp}), rows_side(wd), rows, d.out, hidden, 1, y, ld_y);
-  r.products<T, true, true, T>(all);
+  all.p[0] = problem<T>(rows_side(Matrix{h, hp, rows, hidden, hp}), rows_side(wd), rows, d.out, y, ld_y);
+  r.products<T, true, true, T>(all, hidden, 1);
   return hipGetLastError();
 }
 
@@ -720,14 +873,14 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
     j.p[1] = static_cast<const char*>(w.u.p);
     Problems all{};
     all.n = 1;
-    all.p[0] = problem<T>(i, j, rows, width, hidden, 2, dx, ld_dx);
-    r.products<T, true, false, T>(all);
+    all.p[0] = problem<T>(i, j, rows, width, dx, ld_dx);
+    r.products<T, true, false, T>(all, hidden, 2);
   }
   Problems all{};
-  if (dwg || !r.go) all.p[all.n++] = problem<T>(columns_side(mg), columns_side(x), hidden, width, rows, 1, dwg, width);
-  if (dwu || !r.go) all.p[all.n++] = problem<T>(columns_side(mu), columns_side(x), hidden, width, rows, 1, dwu, width);
-  if (dwd || !r.go) all.p[all.n++] = problem<T>(columns_side(dy), columns_side(mh), out, hidden, rows, 1, dwd, hidden);
-  if (all.n) r.products<T, false, false, T>(all);
+  if (dwg || !r.go) all.p[all.n++] = problem<T>(columns_side(mg), columns_side(x), hidden, width, dwg, width);
+  if (dwu || !r.go) all.p[all.n++] = problem<T>(columns_side(mu), columns_side(x), hidden, width, dwu, width);
+  if (dwd || !r.go) all.p[all.n++] = problem<T>(columns_side(dy), columns_side(mh), out, hidden, dwd, hidden);
+  if (all.n) r.products<T, false, false, T>(all, rows, 1);
   return hipGetLastError();
 }
 
@@ -784,9 +937,9 @@ void set_segments(Side& i, Side& j, int at, const Halves& a, const Halves& b) {
   i.p[at + 1] = p(a.lo), j.p[at + 1] = p(b.hi);
   i.p[at + 2] = p(a.hi), j.p[at + 2] = p(b.hi);
 }
-Problem problem32(Side i, Side j, const Halves& a, const Halves& b, long m, long n, long k, float* out, long ld) {
+Problem problem32(Side i, Side j, const Halves& a, const Halves& b, long m, long n, float* out, long ld) {
   set_segments(i, j, 0, a, b);
-  Problem p = problem<float>(i, j, m, n, k, 3, out, ld);
+  Problem p = problem<float>(i, j, m, n, out, ld);
   p.top_i = a.top, p.top_j = b.top;
   return p;
 }
@@ -815,8 +968,8 @@ hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r)
   two.run();
   Problems all{};
   all.n = 1;
-  all.p[0] = problem32(rows_side(hh.hi), rows_side(wd.hi), hh, wd, rows, out, hidden, y, ld_y);
-  r.products<_Float16, true, true, float>(all);
+  all.p[0] = problem32(rows_side(hh.hi), rows_side(wd.hi), hh, wd, rows, out, y, ld_y);
+  r.products<_Float16, true, true, float>(all, hidden, 3);
   return hipGetLastError();
 }
 
@@ -860,16 +1013,16 @@ hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_
     set_segments(a, b, 3, u, cu);
     Problems all{};
     all.n = 1;
-    all.p[0] = problem<float>(a, b, rows, width, hidden, 6, dx, ld_dx);
+    all.p[0] = problem<float>(a, b, rows, width, dx, ld_dx);
     all.p[0].top_i = tr, all.p[0].top_j = wc;
-    r.products<_Float16, true, false, float>(all);
+    r.products<_Float16, true, false, float>(all, hidden, 6);
   }
   const Halves cx = by_columns(jx), cg = by_columns(kg), cu = by_columns(ku), cy = by_columns(jy), ch = by_columns(kh);
   Problems all{};
-  if (dwg || !r.go) all.p[all.n++] = problem32(columns_side(cg.hi), columns_side(cx.hi), cg, cx, hidden, width, rows, dwg, width);
-  if (dwu || !r.go) all.p[all.n++] = problem32(columns_side(cu.hi), columns_side(cx.hi), cu, cx, hidden, width, rows, dwu, width);
-  if (dwd || !r.go) all.p[all.n++] = problem32(columns_side(cy.hi), columns_side(ch.hi), cy, ch, out, hidden, rows, dwd, hidden);
-  if (all.n) r.products<_Float16, false, false, float>(all);
+  if (dwg || !r.go) all.p[all.n++] = problem32(columns_side(cg.hi), columns_side(cx.hi), cg, cx, hidden, width, dwg, width);
+  if (dwu || !r.go) all.p[all.n++] = problem32(columns_side(cu.hi), columns_side(cx.hi), cu, cx, hidden, width, dwu, width);
+  if (dwd || !r.go) all.p[all.n++] = problem32(columns_side(cy.hi), columns_side(ch.hi), cy, ch, out, hidden, dwd, hidden);
+  if (all.n) r.products<_Float16, false, false, float>(all, rows, 3);
   return hipGetLastError();
 }
 
@@ -916,7 +1069,7 @@ size_t nerf_gated_block_workspace(const nerf_block_desc* d, int backward) {
     else (void)forward_halves(*d, nullptr, 0, r);
   } else if (backward) (void)backward_mma<__bf16>(*d, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, r);
   else (void)forward_mma<__bf16>(*d, nullptr, 0, r);
-  return r.a.used;
+  return r.a.most;
 }
 
 int nerf_gated_block_forward(const nerf_block_desc* d, void* y, int64_t ld_y, void* workspace, size_t workspace_bytes,
