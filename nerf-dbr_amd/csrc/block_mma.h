@@ -56,7 +56,7 @@ __device__ __forceinline__ void lds_dma_16(const void* p, unsigned lds_base) {
 
 __device__ __attribute__((aligned(16))) const unsigned kZeros[4] = {0, 0, 0, 0};   // what stands behind the end of k
 
-constexpr int kMaxSegs = 6;
+constexpr int kMaxSegs = 2;
 // One operand: `segs` matrices of the same shape whose products are added up (the launch's segs).
 // k contiguous: element (i, k) at p + i * ld + 2 k; own contiguous: at p + k * ld + 2 i.  Every p and ld is
 // a multiple of 16 bytes; the contiguous extent (k_n, or n) is a multiple of 8.  split > 0: rows of a tile
@@ -162,23 +162,30 @@ struct Tile {
 // acc[j][i] += the products of steps [first, last) of the segments' steps (steps_per = ceil(k / 64) each).
 // J fragments are the MFMA's first operand: a lane holds 4 neighbouring j of one i.
 //
-// A step is 2 NI groups of NJ matrix instructions: group q multiplies the I fragment q % NI of the half
+// A step is 2 NI groups of NJ matrix instructions: group q multiplies the I fragment q % NI of the half of k
 // q / NI by the half's J fragments.  I fragments are read L = NI / 2 groups ahead and J fragments over the
 // L groups before their half, so the last L groups of a step read from the next stage: the step's one
 // barrier stands before them.  By then a wave has read all of its own stage, which the step after next
 // may overwrite (its pieces are fetched over the same L groups), and its pieces of the next one have been
 // in flight for a step.  The compiler would place each read before its use and wait for it there, so the
 // order of the groups is pinned.
-template <typename T, typename C, bool IK, bool JK, int PARTS>
+//
+// HALVES: the operands are 32-bit values as two 16-bit halves, and a stage holds 32 values of k as 32 hi and
+// 32 lo: one fetch and four halves' reads carry three products, hi lo, lo hi and hi hi, in 3 NI groups (as
+// three sums over k of their own they fetched and read half as much again).
+template <typename T, typename C, bool IK, bool JK, int PARTS, bool HALVES>
 struct Product {
   typedef Stage<C::TI, C::NT, IK, 1> SI;
   typedef Stage<C::TJ, C::NT, JK, PARTS> SJ;
   typedef typename Frag<T>::type F;
   static constexpr unsigned kStage = SI::kBytes + SJ::kBytes;
   static constexpr int kPieces = SI::kChunks + SJ::kChunks;
-  static constexpr int L = C::NI / 2, G = 2 * C::NI;
+  static constexpr int kTurns = HALVES ? 3 : 2;      // through the tile a step
+  static constexpr int L = C::NI / 2, G = kTurns * C::NI;
+  static constexpr int half_i(int turn) { return HALVES ? turn == 1 : turn; }
+  static constexpr int half_j(int turn) { return HALVES ? turn == 0 : turn; }
   static constexpr int kJ = (C::NJ + L - 1) / L, kP = (kPieces + L - 1) / L;   // J reads and pieces a group
-  F fi[2][C::NI], fj[2][C::NJ];
+  F fi[kTurns][C::NI], fj[2][C::NJ];                 // J: the first turn's, the later turns'
   Reader<T, C::TI, IK> ri;
   Reader<T, C::TJ, JK> rj;
 
@@ -216,9 +223,9 @@ struct Product {
     __syncthreads();
     if (n > 1) fetch_all(lds + kStage);
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) fj[0][j] = read_j(j, lds, 0);
+    for (int j = 0; j < C::NJ; ++j) fj[0][j] = read_j(j, lds, half_j(0));
 #pragma unroll
-    for (int i = 0; i < L; ++i) fi[0][i] = read_i(i, lds, 0);
+    for (int i = 0; i < L; ++i) fi[0][i] = read_i(i, lds, half_i(0));
     // fetching: 0 nothing, 1 a whole step, 2 checked
     const auto one_step = [&](int t, auto more, auto fetching) {
       constexpr int kFetch = decltype(fetching)::value;
@@ -239,15 +246,15 @@ struct Product {
 #pragma unroll
           for (int op = slot; op < 1 + kJ + kP; op += C::NJ) {
             if (op == 0) {
-              if (ahead < G) fi[ahead / C::NI][ahead % C::NI] = read_i(ahead % C::NI, now, ahead / C::NI);
-              else if (decltype(more)::value) fi[0][ahead % C::NI] = read_i(ahead % C::NI, next, 0);
+              if (ahead < G) fi[ahead / C::NI][ahead % C::NI] = read_i(ahead % C::NI, now, half_i(ahead / C::NI));
+              else if (decltype(more)::value) fi[0][ahead % C::NI] = read_i(ahead % C::NI, next, half_i(0));
             } else if (op <= kJ) {
               if (q >= C::NI - L - 1 && q < C::NI - 1) {
                 const int j = (q - (C::NI - L - 1)) * kJ + op - 1;
-                if (j < C::NJ) fj[1][j] = read_j(j, now, 1);
+                if (j < C::NJ) fj[1][j] = read_j(j, now, half_j(1));
               } else if (ahead >= G && decltype(more)::value) {
                 const int j = (ahead - G) * kJ + op - 1;
-                if (j < C::NJ) fj[0][j] = read_j(j, next, 0);
+                if (j < C::NJ) fj[0][j] = read_j(j, next, half_j(0));
               }
             } else if (ahead >= G && kFetch != 0) {
               const int c = (ahead - G) * kP + op - 1 - kJ;
@@ -258,7 +265,7 @@ struct Product {
         };
 #pragma unroll
         for (int j = 0; j < C::NJ; ++j) {
-          acc[j][q % C::NI] = Frag<T>::mma(fj[q / C::NI][j], fi[q / C::NI][q % C::NI], acc[j][q % C::NI]);
+          acc[j][q % C::NI] = Frag<T>::mma(fj[q < C::NI ? 0 : 1][j], fi[q / C::NI][q % C::NI], acc[j][q % C::NI]);
           __builtin_amdgcn_sched_barrier(0);
           others(j);
           __builtin_amdgcn_sched_barrier(0);
@@ -283,10 +290,10 @@ struct Product {
     __syncthreads();      // the stages may be used again
   }
 };
-template <typename T, typename C, bool IK, bool JK, int PARTS>
+template <typename T, typename C, bool IK, bool JK, int PARTS, bool HALVES>
 __device__ __forceinline__ void accumulate(f32x4_t (&acc)[C::NJ][C::NI], const Side& si, const Side& sj, long i0, long j0,
                                            int steps_per, int first, int last, unsigned lds) {
-  Product<T, C, IK, JK, PARTS> p;
+  Product<T, C, IK, JK, PARTS, HALVES> p;
   p.run(acc, si, sj, i0, j0, steps_per, first, last, lds);
 }
 

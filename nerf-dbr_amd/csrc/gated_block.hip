@@ -85,40 +85,49 @@ struct Scales {
   const unsigned *x, *wg, *wu, *dy, *wd;
 };
 __device__ __forceinline__ int exponent(unsigned top) { return 141 - max(int(top >> 23), 1); }
+// what a lane's results are scaled back by: `n` of them, `step` apart (behind the end: the last one's)
+template <int N>
+__device__ __forceinline__ void exponents(int (&e)[N], const unsigned* top, long first, int step, long end) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const long at = first + i * step;
+    e[i] = -exponent(top[at < end ? at : end - 1]);
+  }
+}
 
 // h = act(x Wg^T) (x Wu^T): the J tile holds TJ / 2 rows of Wg and the same rows of Wu, so a lane owns the
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
 template <typename T, typename C, typename O, int KIND>
-__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, int segs, O* h, long ld_h, long rows,
+__global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
-  constexpr bool kScaled = sizeof(O) == 4;
+  constexpr bool kHalved = sizeof(O) == 4;
   typedef Out<O, C::TJ / 2> W;
   __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
   unsigned ti, tj;
   tile_of(near(blockIdx.x, gridDim.x, slots<C>()), tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * (C::TJ / 2);
   f32x4_t acc[C::NJ][C::NI] = {};
-  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
+  accumulate<T, C, true, true, 2, kHalved>(acc, x, w, i0, j0, steps, 0, steps, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   const int ib = (wave / C::WJ) * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * (C::NJ / 2) * 16 + (l >> 4) * 4;
+  int er[C::NI], eg[C::NJ / 2][4], eu[C::NJ / 2][4];
+  if constexpr (kHalved) {
+    exponents(er, sc.x, i0 + ib, 16, rows);
+#pragma unroll
+    for (int j = 0; j < C::NJ / 2; ++j) exponents(eg[j], sc.wg, j0 + jb + j * 16, 1, hidden), exponents(eu[j], sc.wu, j0 + jb + j * 16, 1, hidden);
+  }
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
 #pragma unroll
     for (int j = 0; j < C::NJ / 2; ++j) {
-      const long row = i0 + ib + i * 16, col = j0 + jb + j * 16;
       f32x4_t o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float a, d, g = acc[j][i][r], u = acc[j + C::NJ / 2][i][r];
-        const bool in = col + r < hidden;
-        if (kScaled && in && row < rows) {
-          const int e = exponent(sc.x[row]);
-          g = ldexpf(g, -e - exponent(sc.wg[col + r]));
-          u = ldexpf(u, -e - exponent(sc.wu[col + r]));
-        }
+        if constexpr (kHalved) g = ldexpf(g, er[i] + eg[j][r]), u = ldexpf(u, er[i] + eu[j][r]);
         activate<KIND>(g, a, d);
-        o[r] = in ? a * u : 0.0f;
+        o[r] = j0 + jb + j * 16 + r < hidden ? a * u : 0.0f;
       }
       W::put(lds, ib + i * 16, jb + j * 16, o);
     }
@@ -129,10 +138,10 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
 // and h, dg and du of the tile from the three.
 template <typename T, typename C, typename O, int KIND>
-__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy, int segs,
+__global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy,
                                                                  O* h, O* dg, O* du, long ld_h, long rows, long hidden,
                                                                  unsigned tiles_i, unsigned tiles_j, Scales sc) {
-  constexpr bool kScaled = sizeof(O) == 4;
+  constexpr bool kHalved = sizeof(O) == 4;
   typedef Tile<C::WI, C::WJ, C::NI, C::NJ / 2> Half;
   typedef Out<O, Half::TJ> W;
   // results of 4-byte types leave in two passes of half the rows; h and dg leave together, then du
@@ -143,10 +152,17 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
   tile_of(near(blockIdx.x, gridDim.x, slots<C>()), tiles_i, tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * Half::TJ;
   f32x4_t acc[C::NJ][C::NI] = {}, dh[Half::NJ][C::NI] = {};
-  accumulate<T, C, true, true, 2>(acc, x, w, i0, j0, steps, 0, steps * segs, lds_addr(lds));
-  accumulate<T, Half, true, false, 1>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy * segs, lds_addr(lds));
+  accumulate<T, C, true, true, 2, kHalved>(acc, x, w, i0, j0, steps, 0, steps, lds_addr(lds));
+  accumulate<T, Half, true, false, 1, kHalved>(dh, dy, wd, i0, j0, steps_dy, 0, steps_dy, lds_addr(lds));
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
   const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * Half::NJ * 16 + (l >> 4) * 4;
+  int eg[Half::NJ][4], eu[Half::NJ][4], ed[Half::NJ][4];
+  if constexpr (kHalved)
+#pragma unroll
+    for (int j = 0; j < Half::NJ; ++j) {
+      const long col = j0 + jb + j * 16;
+      exponents(eg[j], sc.wg, col, 1, hidden), exponents(eu[j], sc.wu, col, 1, hidden), exponents(ed[j], sc.wd, col, 1, hidden);
+    }
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
     const bool mine = wi / (C::WI / kPasses) == pass;
@@ -154,7 +170,12 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
     if (pass) __syncthreads();
     if (mine) {
 #pragma unroll
-      for (int i = 0; i < C::NI; ++i)
+      for (int i = 0; i < C::NI; ++i) {
+        int er = 0, ey = 0;
+        if constexpr (kHalved) {
+          const long row = i0 + ib + i * 16 < rows ? i0 + ib + i * 16 : rows - 1;
+          er = -exponent(sc.x[row]), ey = -exponent(sc.dy[row]);
+        }
 #pragma unroll
         for (int j = 0; j < Half::NJ; ++j) {
           const int left = int(hidden - j0 < Half::TJ ? hidden - j0 : Half::TJ) - jb - j * 16;    // columns of this lane's four
@@ -162,13 +183,7 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float a, s, g = acc[j][i][r], u = acc[j + Half::NJ][i][r], d = dh[j][i][r];
-            if (kScaled && r < left && i0 + ib + i * 16 < rows) {
-              const long row = i0 + ib + i * 16, col = j0 + jb + j * 16 + r;
-              const int e = exponent(sc.x[row]);
-              g = ldexpf(g, -e - exponent(sc.wg[col]));
-              u = ldexpf(u, -e - exponent(sc.wu[col]));
-              d = ldexpf(d, -exponent(sc.dy[row]) - exponent(sc.wd[col]));
-            }
+            if constexpr (kHalved) g = ldexpf(g, er + eg[j][r]), u = ldexpf(u, er + eu[j][r]), d = ldexpf(d, ey + ed[j][r]);
             activate<KIND>(g, a, s);
             oh[r] = r < left ? a * u : 0.0f;
             og[r] = r < left ? d * u * s : 0.0f;
@@ -180,6 +195,7 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
           // one fragment's temporaries at a time: g, u and dh fill the registers (keeping dg there too: 154 spilled)
           __builtin_amdgcn_sched_barrier(0);
         }
+      }
     }
     __syncthreads();
     W::template flush<kRows, C::NT>(lds, h, ld_h, i0 + pass * kRows, j0, rows, ld_h, true);
@@ -196,13 +212,14 @@ __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w,
   }
 }
 
-// C(i, j) of up to three problems at once.  Their tiles (numbered through) are shared out
-//   whole, as many full waves of workgroups as there are (product_mma_kernel), and the remaining tiles' steps
-//   evenly over `streams` workgroups, each a run of steps that may end one tile and begin the next; or
-//   where tiles are few, all of them cut into the same `cuts` pieces of k: the workgroups of one piece read
-//   the same rows and lie on one XCD.
-// parts_mma_kernel's fp32 partials (neighbouring threads, neighbouring 16 bytes) are added by join_kernel in
-// order.  One kernel for both kinds of tile had 49 spilled registers and lost 7% at whole tiles.
+// C(i, j) of up to three problems at once.  Their tiles (numbered through) run whole, as many full waves of
+// workgroups as there are (product_mma_kernel); the remaining ones do too where they fill most of a wave, or are
+// cut into equal pieces of k (parts_mma_kernel): `even` tiles into `cuts` pieces, which fill the wave, and what is
+// left over into `odd_cuts` pieces that come second in the same workgroups.  The workgroups of one piece read the
+// same rows and lie on one XCD: equal runs of steps over all tiles, each with a place of its own in k, filled the
+// machine as well and read everything from memory (1024 x 2816 x 4096 three times, fp32: 230 against 180 us).
+// The pieces' fp32 partials (neighbouring threads, neighbouring 16 bytes) are added by join_kernel in order.  One
+// kernel for whole tiles and pieces had 49 spilled registers and lost 7% at whole ones.
 struct Problem {
   Side i, j;
   void* out;
@@ -217,33 +234,26 @@ struct Problems {
   int n;
   int steps;         // steps of 64 k of one segment
   int total;         // steps of all segments
-  unsigned tiles, whole, streams;     // tiles, workgroups of whole ones, of parts
-  int cuts, per;     // steps of a stream or of a piece
+  unsigned tiles, whole;              // tiles, whole ones
+  unsigned even, cuts, odd_cuts;
+  int per, odd_per;                   // steps of a piece
   float* part;
 };
-// Part `n` of the stream (which lies on one tile or two) or piece b: false if there is none.
 struct Part {
   unsigned tile;
   int first, last;
   unsigned slot;      // its partials
 };
+// workgroup b's part `n`
 __device__ __forceinline__ bool part_of(const Problems& all, unsigned b, int n, Part& out) {
-  const unsigned rest = all.tiles - all.whole;
-  if (all.cuts) {
-    const unsigned cut = b / rest;
-    out.tile = all.whole + b % rest;
-    out.first = int(cut) * all.per;
-    out.last = min(out.first + all.per, all.total);
-    out.slot = b;
-    return n == 0;
-  }
-  const long lo = long(b) * all.per, end = long(rest) * all.total, hi = lo + all.per < end ? lo + all.per : end;
-  const long tile = lo / all.total + n, start = tile * all.total;
-  if (start >= hi) return false;
-  out.tile = all.whole + unsigned(tile);
-  out.first = int(n ? 0 : lo - start);
-  out.last = int(hi - start < all.total ? hi - start : all.total);
-  out.slot = 2 * b + n;
+  const unsigned odd = all.tiles - all.whole - all.even, tiles = n ? odd : all.even;
+  if (b >= tiles * (n ? all.odd_cuts : all.cuts)) return false;
+  const unsigned cut = b / tiles;
+  const int per = n ? all.odd_per : all.per;
+  out.tile = all.whole + (n ? all.even : 0) + b % tiles;
+  out.first = int(cut) * per;
+  out.last = min(out.first + per, all.total);
+  out.slot = (n ? all.even * all.cuts : 0) + b;
   return true;
 }
 // 32-bit results: the operands' scales taken out
@@ -272,6 +282,12 @@ struct Leave {
   static __device__ __forceinline__ void run(char* lds, const Problem& p, long i0, long j0, const f32x4_t (&acc)[C::NJ][C::NI]) {
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
     const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * C::NJ * 16 + (l >> 4) * 4;
+    int er[C::NI], ec[C::NJ][4];
+    if constexpr (sizeof(O) == 4) {
+      exponents(er, p.top_i, i0 + ib, 16, p.m);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) exponents(ec[j], p.top_j, j0 + jb + j * 16, 1, p.n);
+    }
 #pragma unroll
     for (int pass = 0; pass < kPasses; ++pass) {
       if (pass) __syncthreads();
@@ -279,8 +295,13 @@ struct Leave {
 #pragma unroll
         for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-          for (int j = 0; j < C::NJ; ++j)
-            W::put(lds, ib + i * 16 - pass * kRows, jb + j * 16, scaled<O>(p, i0 + ib + i * 16, j0 + jb + j * 16, acc[j][i]));
+          for (int j = 0; j < C::NJ; ++j) {
+            f32x4_t v = acc[j][i];
+            if constexpr (sizeof(O) == 4)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], er[i] + ec[j][r]);
+            W::put(lds, ib + i * 16 - pass * kRows, jb + j * 16, v);
+          }
       }
       __syncthreads();
       W::template flush<kRows, C::NT>(lds, static_cast<O*>(p.out), p.ld, i0 + pass * kRows, j0, p.m, p.n, p.wide);
@@ -289,6 +310,7 @@ struct Leave {
 };
 template <typename T, typename C, bool IK, bool JK, typename O>
 __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
+  constexpr bool HALVES = sizeof(O) == 4;
   __shared__ __attribute__((aligned(1024))) char lds[Leave<C, O>::kLds];
   const unsigned tile = near(blockIdx.x, gridDim.x, slots<C>());
   const Problem& p = problem_of(all, tile);
@@ -296,10 +318,10 @@ __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
   tile_of(tile - p.first, p.tiles_i, p.tiles_j, ti, tj);
   const long i0 = long(ti) * C::TI, j0 = long(tj) * C::TJ;
   f32x4_t acc[C::NJ][C::NI] = {};
-  accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, i0, j0, all.steps, 0, all.total, lds_addr(lds));
+  accumulate<T, C, IK, JK, 1, HALVES>(acc, p.i, p.j, i0, j0, all.steps, 0, all.total, lds_addr(lds));
   Leave<C, O>::run(lds, p, i0, j0, acc);
 }
-template <typename T, typename C, bool IK, bool JK>
+template <typename T, typename C, bool IK, bool JK, bool HALVES>
 __global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
   __shared__ __attribute__((aligned(1024))) char lds[stages<C>()];
   const unsigned b = near(blockIdx.x, gridDim.x, slots<C>());
@@ -309,7 +331,7 @@ __global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
     unsigned ti, tj;
     tile_of(part.tile - p.first, p.tiles_i, p.tiles_j, ti, tj);
     f32x4_t acc[C::NJ][C::NI] = {};
-    accumulate<T, C, IK, JK, 1>(acc, p.i, p.j, long(ti) * C::TI, long(tj) * C::TJ, all.steps, part.first, part.last, lds_addr(lds));
+    accumulate<T, C, IK, JK, 1, HALVES>(acc, p.i, p.j, long(ti) * C::TI, long(tj) * C::TJ, all.steps, part.first, part.last, lds_addr(lds));
     f32x4_t* to = reinterpret_cast<f32x4_t*>(all.part) + long(part.slot) * (C::NI * C::NJ * C::NT);
 #pragma unroll
     for (int i = 0; i < C::NI; ++i)
@@ -321,18 +343,16 @@ __global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
 template <typename C, typename O>
 __global__ __launch_bounds__(C::NT) void join_kernel(Problems all) {
   constexpr int kFrags = C::NI * C::NJ;
-  const unsigned rest = all.tiles - all.whole, r = blockIdx.x / kFrags;
+  const unsigned r = blockIdx.x / kFrags, odd = all.tiles - all.whole - all.even;
   const int f = int(blockIdx.x % kFrags);
-  const f32x4_t* part = reinterpret_cast<const f32x4_t*>(all.part) + f * C::NT + threadIdx.x;
-  const long size = kFrags * C::NT;
+  const bool even = r < all.even;
+  const unsigned cuts = even ? all.cuts : all.odd_cuts;
+  const long size = kFrags * C::NT, next = long(even ? all.even : odd) * size;
+  const f32x4_t* part = reinterpret_cast<const f32x4_t*>(all.part) + f * C::NT + threadIdx.x +
+                        long(even ? r : all.even * all.cuts + r - all.even) * size;
   f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (all.cuts) {
 #pragma unroll 4
-    for (int s = 0; s < all.cuts; ++s) v += part[(long(s) * rest + r) * size];
-  } else {
-    const long lo = long(r) * all.total, hi = lo + all.total, b0 = lo / all.per, b1 = (hi - 1) / all.per;
-    for (long b = b0; b <= b1; ++b) v += part[(2 * b + (b * all.per < lo ? 1 : 0)) * size];
-  }
+  for (unsigned s = 0; s < cuts; ++s) v += part[s * next];
   const Problem& p = problem_of(all, all.whole + r);
   unsigned ti, tj;
   tile_of(all.whole + r - p.first, p.tiles_i, p.tiles_j, ti, tj);
@@ -506,9 +526,10 @@ constexpr int kFewRows = 64;
 // zeroed tables; a maximum does not depend on the order of the atomics), then the halves by either.
 struct SplitJob {
   const float* src;
-  long ld, rows, n, n8;
+  long ld, rows, n;
   unsigned *row_top, *col_top;     // null: not wanted
-  _Float16 *row_hi, *col_hi;       // [rows][n8]; the lo half follows at + rows * n8
+  _Float16 *row_hi, *col_hi;       // [rows][n32 x 2], [rows32 x 2][n8]: 32 hi, then their 32 lo, zeros behind the ends
+  long n8, n32, rows32;
   unsigned first;                  // first workgroup
   unsigned across;                 // workgroups along a row
   int wide;
@@ -590,7 +611,6 @@ __global__ __launch_bounds__(256) void split_kernel(SplitJobs all) {
   const unsigned b = blockIdx.x - p.first;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long row0 = long(b / p.across) * kSplitRows + wave * 16, col = long(b % p.across) * kSplitCols + lane * 4;
-  if (col >= p.n8) return;
   int ec[4] = {0, 0, 0, 0};
   if (p.col_hi)
 #pragma unroll
@@ -599,13 +619,13 @@ __global__ __launch_bounds__(256) void split_kernel(SplitJobs all) {
 #pragma unroll 4
   for (int i = 0; i < 16; ++i) {
     const long row = row0 + i;
-    if (row >= p.rows) return;
-    const f32x4_t v = split_load(p, row, col);
-    if (p.row_hi) {
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < p.rows) v = split_load(p, row, col);
+    if (p.row_hi && row < p.rows && col < p.n32) {
       const int x = exponent(p.row_top[row]), e[4] = {x, x, x, x};
-      split_store(p.row_hi + row * p.n8 + col, p.rows * p.n8, v, e);
+      split_store(p.row_hi + row * p.n32 * 2 + (col & ~31L) * 2 + (col & 31), 32, v, e);
     }
-    if (p.col_hi) split_store(p.col_hi + row * p.n8 + col, p.rows * p.n8, v, ec);
+    if (p.col_hi && row < p.rows32 && col < p.n8) split_store(p.col_hi + ((row & ~31L) * 2 + (row & 31)) * p.n8 + col, 32 * p.n8, v, ec);
   }
 }
 
@@ -645,15 +665,18 @@ Side columns_side(const Matrix& m) {   // i = column, k = row
 }
 
 // What a launch is expected to take, in microseconds, from whole launches of either tile: a step where every
-// workgroup slot is taken and where a CU runs one workgroup alone (it then waits for its operands), what a tile
-// costs besides, a join, and a MiB of partials written or read.
-constexpr double kFullLarge = 1.4, kFullSmall = 1.1, kAlone = 0.9, kTileLarge = 7.0, kTileSmall = 5.0, kJoin = 5.0, kMiB = 0.2;
+// workgroup slot is taken (8192 x 4096 x 10240: 1.7) and where a CU runs one workgroup alone and waits for its
+// operands, what a tile costs besides, a join, and a MiB of partials written or read.
+constexpr double kFullLarge = 1.7, kFullSmall = 1.1, kAloneLarge = 1.45, kAloneSmall = 0.8, kTileLarge = 7.0, kTileSmall = 5.0;
+constexpr double kJoin = 5.0, kMiB = 0.2;
+constexpr long kPiece = 8;   // steps: less is mostly a tile's costs
 long tiles_of(long m, long n, long ti, long tj) { return ((m + ti - 1) / ti) * ((n + tj - 1) / tj); }
 // `n` workgroups of `steps` steps at a time
 template <typename C>
 double wave_time(long n, double steps) {
-  const double full = is_large<C>() ? kFullLarge : kFullSmall, part = full * double(n) / double(slots<C>());
-  return steps * (part > kAlone ? part : kAlone) + (is_large<C>() ? kTileLarge : kTileSmall);
+  const double full = is_large<C>() ? kFullLarge : kFullSmall, alone = is_large<C>() ? kAloneLarge : kAloneSmall;
+  const double part = full * double(n) / double(slots<C>());
+  return steps * (part > alone ? part : alone) + (is_large<C>() ? kTileLarge : kTileSmall);
 }
 template <typename C>
 double whole_time(long tiles, double steps) {
@@ -661,10 +684,13 @@ double whole_time(long tiles, double steps) {
   return double(full) * wave_time<C>(slots<C>(), steps) + (rest ? wave_time<C>(rest, steps) : 0.0);
 }
 // The gate kernels: whole tiles only, `steps` of both phases.
-bool gate_large(long rows, long cols, long steps) {
-  return whole_time<Large>(tiles_of(rows, cols, Large::TI, Large::TJ), double(steps)) <=
-         whole_time<Small>(tiles_of(rows, cols, Small::TI, Small::TJ), double(steps));
+bool gate_large(long rows, long cols, long steps, double turns) {
+  return whole_time<Large>(tiles_of(rows, cols, Large::TI, Large::TJ), steps * turns) <=
+         whole_time<Small>(tiles_of(rows, cols, Small::TI, Small::TJ), steps * turns);
 }
+// 32-bit results: a step of halves carries three products instead of two
+template <typename O>
+constexpr double turns() { return sizeof(O) == 4 ? 1.5 : 1.0; }
 
 struct Run {
   hipStream_t s;
@@ -687,7 +713,7 @@ struct Run {
 
   // How a launch's tiles are shared out, and what that is expected to take.
   template <typename C>
-  static double share(Problems& all) {
+  static double share(Problems& all, double turns) {
     all.tiles = 0;
     for (int k = 0; k < all.n; ++k) {
       Problem& p = all.p[k];
@@ -697,39 +723,43 @@ struct Run {
     }
     const long n = slots<C>(), total = all.total, tiles = all.tiles, full = tiles / n, rest = tiles % n;
     const double mib = C::TI * C::TJ * 4.0 / (1 << 20);
-    all.whole = unsigned(tiles), all.streams = 0, all.cuts = 0, all.per = 0;
+    all.whole = all.tiles, all.even = all.cuts = all.odd_cuts = 0, all.per = all.odd_per = 0;
     if (total == 0 || tiles == 0) return 0.0;
-    double best = whole_time<C>(tiles, double(total));
-    if (rest * 2 <= n && full == 0 && total >= 16) {        // few tiles: equal pieces of at least 8 steps
-      long cuts = n / rest < total / 8 ? n / rest : total / 8;
-      const long per = (total + cuts - 1) / cuts;
-      cuts = (total + per - 1) / per;
-      const double t = wave_time<C>(cuts * rest, double(per)) + kJoin + 2 * double(cuts * rest) * mib * kMiB;
-      if (t < best) best = t, all.whole = 0, all.streams = unsigned(cuts * rest), all.cuts = int(cuts), all.per = int(per);
-    }
-    if (rest && rest * total >= 8 * n) {
-      const long per = (rest * total + n - 1) / n;
-      const double t = whole_time<C>(full * n, double(total)) + wave_time<C>(n, double(per)) + (is_large<C>() ? kTileLarge : kTileSmall) +
-                       kJoin + 2 * double(n + rest) * mib * kMiB;
-      if (t < best) best = t, all.whole = unsigned(full * n), all.streams = unsigned((rest * total + per - 1) / per), all.cuts = 0, all.per = int(per);
+    double best = whole_time<C>(tiles, total * turns);
+    for (long cuts = rest ? n / rest : 0; rest && cuts <= n / rest + 1; ++cuts) {
+      if (cuts < 2) continue;
+      const long c = cuts * kPiece < total ? cuts : total / kPiece;
+      if (c < 2) break;
+      const long per = (total + c - 1) / c, pieces = (total + per - 1) / per, fit = n / pieces, even = rest < fit ? rest : fit, odd = rest - even;
+      long odd_cuts = odd ? even * pieces / odd : 0;         // no more than there are workgroups
+      if (odd && odd_cuts < 1) continue;
+      if (odd_cuts > total / kPiece) odd_cuts = total / kPiece;
+      const long odd_per = odd ? (total + odd_cuts - 1) / odd_cuts : 0;
+      if (odd) odd_cuts = (total + odd_per - 1) / odd_per;
+      const long parts = even * pieces + odd * odd_cuts;
+      const double t = whole_time<C>(full * n, total * turns) + wave_time<C>(even * pieces, per * turns) +
+                       (odd ? wave_time<C>(odd * odd_cuts, odd_per * turns) : 0.0) + kJoin + 2 * double(parts) * mib * kMiB;
+      if (t >= best) continue;
+      best = t, all.whole = unsigned(full * n), all.even = unsigned(even), all.cuts = unsigned(pieces), all.per = int(per);
+      all.odd_cuts = unsigned(odd_cuts), all.odd_per = int(odd_per);
     }
     return best;
   }
   // C = the segments' products for up to three problems of one kind.  Partials lie behind what the arena has
   // given out so far and are done with when the launches are.
   template <typename C>
-  static size_t share_bytes(Problems& all) {
-    (void)share<C>(all);
-    return (all.cuts ? size_t(all.streams) : 2 * size_t(all.streams)) * C::TI * C::TJ * 4;
+  static size_t share_bytes(Problems& all, double turns) {
+    (void)share<C>(all, turns);
+    return (size_t(all.even) * all.cuts + size_t(all.tiles - all.whole - all.even) * all.odd_cuts) * C::TI * C::TJ * 4;
   }
   template <typename T, bool IK, bool JK, typename O, typename C>
   size_t products_of(Problems& all) {
-    const size_t bytes = share_bytes<C>(all);
+    const size_t bytes = share_bytes<C>(all, turns<O>());
     if (!go || !all.tiles) return bytes;
     all.part = reinterpret_cast<float*>(a.base + a.used);
     if (all.whole) hipLaunchKernelGGL((product_mma_kernel<T, C, IK, JK, O>), dim3(all.whole), dim3(C::NT), 0, s, all);
-    if (all.streams) {
-      hipLaunchKernelGGL((parts_mma_kernel<T, C, IK, JK>), dim3(all.streams), dim3(C::NT), 0, s, all);
+    if (all.even) {
+      hipLaunchKernelGGL((parts_mma_kernel<T, C, IK, JK, sizeof(O) == 4>), dim3(all.even * all.cuts), dim3(C::NT), 0, s, all);
       hipLaunchKernelGGL((join_kernel<C, O>), dim3((all.tiles - all.whole) * C::NI * C::NJ), dim3(C::NT), 0, s, all);
     }
     return bytes;
@@ -737,7 +767,7 @@ struct Run {
   template <typename T, bool IK, bool JK, typename O>
   size_t products_one(Problems& all, long k, int segs) {
     all.steps = int((k + 63) / 64), all.total = all.steps * segs;
-    const double large = share<Large>(all), small = share<Small>(all);
+    const double large = share<Large>(all, turns<O>()), small = share<Small>(all, turns<O>());
     return large <= small ? products_of<T, IK, JK, O, Large>(all) : products_of<T, IK, JK, O, Small>(all);
   }
   template <typename T, bool IK, bool JK, typename O>
@@ -786,34 +816,34 @@ dim3 gate_grid(long rows, long hidden, unsigned& ti, unsigned& tj) {
 int steps_of(long k) { return int((k + 63) / 64); }
 
 template <typename T, typename O>
-void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, int segs, O* h, long hp, const Scales& sc) {
+void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, long k, O* h, long hp, const Scales& sc) {
   if (!r.go || !d.rows) return;
   unsigned ti, tj;
   const auto go = [&](auto tile) {
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
-    with_kind(d.activation, [&](auto k) {
-      hipLaunchKernelGGL((gate_mma_kernel<T, C, O, decltype(k)::value>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(d.width), segs, h, hp,
+    with_kind(d.activation, [&](auto kind) {
+      hipLaunchKernelGGL((gate_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(k), h, hp,
                          long(d.rows), long(d.hidden), ti, tj, sc);
     });
   };
-  if (gate_large(d.rows, 2 * hp, long(steps_of(d.width)) * segs)) go(Large{});
+  if (gate_large(d.rows, 2 * hp, steps_of(k), turns<O>())) go(Large{});
   else go(Small{});
 }
 template <typename T, typename O>
-void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, const Side& dy, const Side& wd, int segs, O* h, O* dg,
-                      O* du, long hp, const Scales& sc) {
+void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, const Side& dy, const Side& wd, long k, long k_dy, O* h,
+                      O* dg, O* du, long hp, const Scales& sc) {
   if (!r.go || !d.rows) return;
   unsigned ti, tj;
   const auto go = [&](auto tile) {
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
-    with_kind(d.activation, [&](auto k) {
-      hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O, decltype(k)::value>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(d.width),
-                         steps_of(d.out), segs, h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
+    with_kind(d.activation, [&](auto kind) {
+      hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(k),
+                         steps_of(k_dy), h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
     });
   };
-  if (gate_large(d.rows, 2 * hp, long(steps_of(d.width) + steps_of(d.out)) * segs)) go(Large{});
+  if (gate_large(d.rows, 2 * hp, steps_of(k) + steps_of(k_dy), turns<O>())) go(Large{});
   else go(Small{});
 }
 
@@ -846,7 +876,7 @@ hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const Pair w = weights<T>(r, d);
   const Matrix wd = r.matrix<T>(d.w_down, d.ld_down, d.out, hidden);
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  launch_gate<T, T>(r, d, rows_side(x), halves(w), 1, h, hp, Scales{});
+  launch_gate<T, T>(r, d, rows_side(x), halves(w), d.width, h, hp, Scales{});
   Problems all{};
   all.n = 1;
   all.p[0] = problem<T>(rows_side(Matrix{h, hp, rows, hidden, hp}), rows_side(wd), rows, d.out, y, ld_y);
@@ -865,7 +895,7 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* dg = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* du = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  launch_gate_back<T, T>(r, d, rows_side(x), halves(w), rows_side(dy), columns_side(wd), 1, h, dg, du, hp, Scales{});
+  launch_gate_back<T, T>(r, d, rows_side(x), halves(w), rows_side(dy), columns_side(wd), width, out, h, dg, du, hp, Scales{});
   const Matrix mh{h, hp, rows, hidden, hp}, mg{dg, hp, rows, hidden, hp}, mu{du, hp, rows, hidden, hp};
   if ((dx || !r.go) && rows) {
     Side i = rows_side(mg), j = columns_side(w.g);
@@ -885,9 +915,9 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
 }
 
 // ------------------------------------------------------------------------------ 32-bit, in two halves --
-// A matrix's halves and its scales' table.
+// A matrix's halves as one side, and its scales' table.
 struct Halves {
-  Matrix hi, lo;
+  Side side;
   const unsigned* top;
 };
 // Takes tables and halves for the jobs of one pass, and runs scan and split over them.
@@ -906,10 +936,11 @@ struct Splitter {
   // by: 1 rows, 2 columns, 3 both; the tables' addresses are given (joint scales share one)
   SplitJob& add(const float* src, long ld, long rows, long n, unsigned* row_top, unsigned* col_top, int by) {
     SplitJob& j = all.j[all.n++];
-    j.src = src, j.ld = ld, j.rows = rows, j.n = n, j.n8 = align_up(n, 8);
+    j.src = src, j.ld = ld, j.rows = rows, j.n = n;
+    j.n8 = align_up(n, 8), j.n32 = align_up(n, 32), j.rows32 = align_up(rows, 32);
     j.row_top = row_top, j.col_top = col_top;
-    if (by & 1) j.row_hi = static_cast<_Float16*>(r.a.take(size_t(rows) * j.n8 * 4));
-    if (by & 2) j.col_hi = static_cast<_Float16*>(r.a.take(size_t(rows) * j.n8 * 4));
+    if (by & 1) j.row_hi = static_cast<_Float16*>(r.a.take(size_t(rows) * j.n32 * 4));
+    if (by & 2) j.col_hi = static_cast<_Float16*>(r.a.take(size_t(j.rows32) * j.n8 * 4));
     j.wide = !(uintptr_t(src) & 15) && ld % 4 == 0;
     return j;
   }
@@ -918,7 +949,7 @@ struct Splitter {
     for (int k = 0; k < all.n; ++k) {
       SplitJob& j = all.j[k];
       j.first = grid;
-      j.across = unsigned((j.n8 + kSplitCols - 1) / kSplitCols);
+      j.across = unsigned((j.n32 + kSplitCols - 1) / kSplitCols);
       grid += j.across * unsigned((j.rows + kSplitRows - 1) / kSplitRows);
     }
     if (!r.go) return;
@@ -928,18 +959,24 @@ struct Splitter {
     hipLaunchKernelGGL(split_kernel, dim3(grid), dim3(256), 0, r.s, all);
   }
 };
-Halves by_rows(const SplitJob& j) { return {{j.row_hi, j.n8, j.rows, j.n, j.n8}, {j.row_hi + j.rows * j.n8, j.n8, j.rows, j.n, j.n8}, j.row_top}; }
-Halves by_columns(const SplitJob& j) { return {{j.col_hi, j.n8, j.rows, j.n, j.n8}, {j.col_hi + j.rows * j.n8, j.n8, j.rows, j.n, j.n8}, j.col_top}; }
-// hi hi + hi lo + lo hi, the small products first
-void set_segments(Side& i, Side& j, int at, const Halves& a, const Halves& b) {
-  const auto p = [](const Matrix& m) { return static_cast<const char*>(m.p); };
-  i.p[at] = p(a.hi), j.p[at] = p(b.lo);
-  i.p[at + 1] = p(a.lo), j.p[at + 1] = p(b.hi);
-  i.p[at + 2] = p(a.hi), j.p[at + 2] = p(b.hi);
+Halves by_rows(const SplitJob& j) {
+  Side s{};
+  s.p[0] = reinterpret_cast<const char*>(j.row_hi), s.ld = j.n32 * 4, s.n = j.rows, s.k_n = j.n32 * 2;
+  return {s, j.row_top};
 }
-Problem problem32(Side i, Side j, const Halves& a, const Halves& b, long m, long n, float* out, long ld) {
-  set_segments(i, j, 0, a, b);
-  Problem p = problem<float>(i, j, m, n, out, ld);
+Halves by_columns(const SplitJob& j) {
+  Side s{};
+  s.p[0] = reinterpret_cast<const char*>(j.col_hi), s.ld = j.n8 * 2, s.n = j.n8, s.k_n = j.rows32 * 2;
+  return {s, j.col_top};
+}
+long halved(long k) { return align_up(k, 32) * 2; }
+Side pair(const Halves& g, const Halves& u) {
+  Side s = g.side;
+  s.split = u.side.p[0] - s.p[0];
+  return s;
+}
+Problem problem32(const Halves& a, const Halves& b, long m, long n, float* out, long ld) {
+  Problem p = problem<float>(a.side, b.side, m, n, out, ld);
   p.top_i = a.top, p.top_j = b.top;
   return p;
 }
@@ -958,9 +995,7 @@ hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r)
   const Halves wd = by_rows(one.add((const float*)d.w_down, d.ld_down, out, hidden, td, nullptr, 1));
   one.run();
   float* h = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
-  Side i = rows_side(x.hi), j = halves(Pair{wg.hi, wu.hi});
-  set_segments(i, j, 0, x, wg);
-  launch_gate<_Float16, float>(r, d, i, j, 3, h, hp, Scales{tx, tg, tu, nullptr, nullptr});
+  launch_gate<_Float16, float>(r, d, x.side, pair(wg, wu), halved(width), h, hp, Scales{tx, tg, tu, nullptr, nullptr});
   Splitter two(r);
   two.tops = th;       // zeroed twice: its table lies in the first pass's memory
   two.n_tops = align_up(rows, 64);
@@ -968,8 +1003,8 @@ hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r)
   two.run();
   Problems all{};
   all.n = 1;
-  all.p[0] = problem32(rows_side(hh.hi), rows_side(wd.hi), hh, wd, rows, out, y, ld_y);
-  r.products<_Float16, true, true, float>(all, hidden, 3);
+  all.p[0] = problem32(hh, wd, rows, out, y, ld_y);
+  r.products<_Float16, true, true, float>(all, halved(hidden), 1);
   return hipGetLastError();
 }
 
@@ -994,10 +1029,8 @@ hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_
   float* dg = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
   float* du = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
   const Halves x = by_rows(jx), wg = by_rows(jg), wu = by_rows(ju), dy = by_rows(jy), wd = by_columns(jd);
-  Side i = rows_side(x.hi), j = halves(Pair{wg.hi, wu.hi}), iy = rows_side(dy.hi), jw = columns_side(wd.hi);
-  set_segments(i, j, 0, x, wg);
-  set_segments(iy, jw, 0, dy, wd);
-  launch_gate_back<_Float16, float>(r, d, i, j, iy, jw, 3, h, dg, du, hp, Scales{xr, gr, ur, yr, dc});
+  launch_gate_back<_Float16, float>(r, d, x.side, pair(wg, wu), dy.side, wd.side, halved(width), halved(out), h, dg, du, hp,
+                                    Scales{xr, gr, ur, yr, dc});
   Splitter two(r);
   two.tops = base ? base + n1 : nullptr;
   unsigned *tr = two.table(two.tops, rows), *hc = two.table(two.tops, hidden), *gc = two.table(two.tops, hidden),
@@ -1008,21 +1041,18 @@ hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_
   two.run();
   if ((dx || !r.go) && rows) {
     const Halves g = by_rows(kg), u = by_rows(ku), cg = by_columns(jg), cu = by_columns(ju);
-    Side a = rows_side(g.hi), b = columns_side(cg.hi);
-    set_segments(a, b, 0, g, cg);
-    set_segments(a, b, 3, u, cu);
     Problems all{};
     all.n = 1;
-    all.p[0] = problem<float>(a, b, rows, width, dx, ld_dx);
-    all.p[0].top_i = tr, all.p[0].top_j = wc;
-    r.products<_Float16, true, false, float>(all, hidden, 6);
+    all.p[0] = problem32(g, cg, rows, width, dx, ld_dx);
+    all.p[0].i.p[1] = u.side.p[0], all.p[0].j.p[1] = cu.side.p[0];
+    r.products<_Float16, true, false, float>(all, halved(hidden), 2);
   }
   const Halves cx = by_columns(jx), cg = by_columns(kg), cu = by_columns(ku), cy = by_columns(jy), ch = by_columns(kh);
   Problems all{};
-  if (dwg || !r.go) all.p[all.n++] = problem32(columns_side(cg.hi), columns_side(cx.hi), cg, cx, hidden, width, dwg, width);
-  if (dwu || !r.go) all.p[all.n++] = problem32(columns_side(cu.hi), columns_side(cx.hi), cu, cx, hidden, width, dwu, width);
-  if (dwd || !r.go) all.p[all.n++] = problem32(columns_side(cy.hi), columns_side(ch.hi), cy, ch, out, hidden, dwd, hidden);
-  if (all.n) r.products<_Float16, false, false, float>(all, rows, 3);
+  if (dwg || !r.go) all.p[all.n++] = problem32(cg, cx, hidden, width, dwg, width);
+  if (dwu || !r.go) all.p[all.n++] = problem32(cu, cx, hidden, width, dwu, width);
+  if (dwd || !r.go) all.p[all.n++] = problem32(cy, ch, out, hidden, dwd, hidden);
+  if (all.n) r.products<_Float16, false, false, float>(all, halved(rows), 1);
   return hipGetLastError();
 }
 
