@@ -406,18 +406,16 @@ struct FewStep<float> {
     return c;
   }
 };
-// the lane's values of k from k0 (a multiple of kLane) of one row, zeros behind the end
-template <typename T, bool WHOLE>
+// the lane's values of k from k0 of one row, zeros behind the end; rows start where they like, the load is one
+// instruction all the same (value by value, rows of odd lengths took 1.5 times as long)
+template <typename T, bool CHECKED>
 __device__ __forceinline__ typename FewStep<T>::Data few_load(const T* row, long k0, long k) {
-  typename FewStep<T>::Data v;
-  if (WHOLE) {
-    if (k0 < k) v = *reinterpret_cast<const typename FewStep<T>::Data*>(row + k0);
-    else
-      for (int r = 0; r < FewStep<T>::kLane; ++r) v[r] = T(0.0f);
-  } else {
+  typedef typename FewStep<T>::Data Data;
+  typedef Data Loose __attribute__((aligned(sizeof(T))));
+  if (!CHECKED || k0 + FewStep<T>::kLane <= k) return *reinterpret_cast<const Loose*>(row + k0);
+  Data v;
 #pragma unroll
-    for (int r = 0; r < FewStep<T>::kLane; ++r) v[r] = k0 + r < k ? row[k0 + r] : T(0.0f);
-  }
+  for (int r = 0; r < FewStep<T>::kLane; ++r) v[r] = k0 + r < k ? row[k0 + r] : T(0.0f);
   return v;
 }
 struct Few {
@@ -427,7 +425,7 @@ struct Few {
   long k;
   void* out;
 };
-template <typename T, int NI, int WAVES, bool WHOLE, int MODE>
+template <typename T, int NI, int WAVES, int MODE>
 __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
   typedef FewStep<T> S;
   constexpr int kU = NI == 1 ? 8 : 4, kCols = MODE == kRows ? 16 : 8;
@@ -456,9 +454,9 @@ __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long at = k0 + u * WAVES * S::kK;
-      fw[u] = few_load<T, WHOLE>(w, at, k);
+      fw[u] = few_load<T, decltype(checked)::value>(w, at, k);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fx[u][i] = few_load<T, WHOLE>(x[i], at, k);
+      for (int i = 0; i < NI; ++i) fx[u][i] = few_load<T, decltype(checked)::value>(x[i], at, k);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -466,12 +464,10 @@ __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
       for (int i = 0; i < NI; ++i) acc[i] = S::mma(fw[u], fx[u][i], acc[i]);
   };
   long k0 = long(wave) * S::kK;
-  if (WHOLE) {
-    for (; k0 + ((kU - 1) * WAVES + 1) * S::kK <= k_all; k0 += kU * WAVES * S::kK)
-      steps(k0, std::integral_constant<int, kU>{}, std::false_type{});
-    for (; k0 + (WAVES + 1) * S::kK <= k_all; k0 += 2 * WAVES * S::kK)
-      steps(k0, std::integral_constant<int, 2>{}, std::false_type{});
-  }
+  for (; k0 + ((kU - 1) * WAVES + 1) * S::kK <= k_all; k0 += kU * WAVES * S::kK)
+    steps(k0, std::integral_constant<int, kU>{}, std::false_type{});
+  for (; k0 + (WAVES + 1) * S::kK <= k_all; k0 += 2 * WAVES * S::kK)
+    steps(k0, std::integral_constant<int, 2>{}, std::false_type{});
   for (; k0 < half; k0 += WAVES * S::kK) steps(k0, std::integral_constant<int, 1>{}, std::true_type{});
 #pragma unroll
   for (int i = 0; i < NI; ++i) red[wave][i][l] = acc[i];
@@ -505,19 +501,15 @@ __global__ __launch_bounds__(WAVES * 64) void few_kernel(Few p) {
   }
 }
 template <typename T, int MODE>
-void launch_few(const Few& p, bool all_whole, hipStream_t s) {
+void launch_few(const Few& p, hipStream_t s) {
   const dim3 grid(unsigned((p.n_out + (MODE == kRows ? 15 : 7)) / (MODE == kRows ? 16 : 8)));
-  const auto go = [&](auto ni, auto whole) {
+  const auto go = [&](auto ni) {
     constexpr int NI = decltype(ni)::value, WAVES = MODE == kGate ? 8 : NI == 1 ? 16 : 8;
-    hipLaunchKernelGGL((few_kernel<T, NI, WAVES, decltype(whole)::value, MODE>), grid, dim3(WAVES * 64), 0, s, p);
+    hipLaunchKernelGGL((few_kernel<T, NI, WAVES, MODE>), grid, dim3(WAVES * 64), 0, s, p);
   };
-  const auto rows = [&](auto whole) {
-    if (MODE == kHalves || p.rows <= 16) go(std::integral_constant<int, 1>{}, whole);
-    else if (p.rows <= 32) go(std::integral_constant<int, MODE == kHalves ? 1 : 2>{}, whole);
-    else go(std::integral_constant<int, MODE == kHalves ? 1 : 4>{}, whole);
-  };
-  if (all_whole) rows(std::true_type{});
-  else rows(std::false_type{});
+  if (MODE == kHalves || p.rows <= 16) go(std::integral_constant<int, 1>{});
+  else if (p.rows <= 32) go(std::integral_constant<int, MODE == kHalves ? 1 : 2>{});
+  else go(std::integral_constant<int, MODE == kHalves ? 1 : 4>{});
 }
 // h's row stride for few rows: whole 16-byte pieces
 constexpr int kFewRows = 64;
@@ -852,20 +844,17 @@ hipError_t forward_few(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const long hp = align_up(d.hidden, 8);
   T* h = static_cast<T*>(r.a.take(size_t(d.rows) * hp * sizeof(T)));
   if (!r.go) return hipSuccess;
-  constexpr long kV = 16 / sizeof(T);
-  const auto whole16 = [](const void* p, long ld, long n) { return !(uintptr_t(p) & 15) && ld % kV == 0 && n % kV == 0; };
   Few a{};
   a.x = d.x, a.w = d.w_gate, a.w2 = d.w_up, a.out = h;
   a.ld_x = d.ld_x, a.ld_w = d.ld_gate, a.ld_w2 = d.ld_up, a.ld_out = hp;
   a.rows = int(d.rows), a.n = d.hidden, a.n_out = int(hp), a.kind = d.activation, a.k = d.width;
-  launch_few<T, kGate>(a, whole16(d.x, d.ld_x, d.width) && whole16(d.w_gate, d.ld_gate, d.width) && whole16(d.w_up, d.ld_up, d.width), r.s);
+  launch_few<T, kGate>(a, r.s);
   Few b{};
   b.x = h, b.w = d.w_down, b.out = y;
   b.ld_x = hp, b.ld_w = d.ld_down, b.ld_out = ld_y;
   b.rows = int(d.rows), b.n = b.n_out = d.out, b.k = d.hidden;
-  const bool w = whole16(d.w_down, d.ld_down, d.hidden);
-  if (d.rows <= 8) launch_few<T, kHalves>(b, w, r.s);
-  else launch_few<T, kRows>(b, w, r.s);
+  if (d.rows <= 8) launch_few<T, kHalves>(b, r.s);
+  else launch_few<T, kRows>(b, r.s);
   return hipGetLastError();
 }
 
