@@ -532,6 +532,11 @@ struct SplitJobs {
 };
 constexpr int kSplitRows = 64, kSplitCols = 256;   // a workgroup's piece: 4 waves of 16 rows, 4 columns a lane
 
+__device__ __forceinline__ unsigned finite_bits(float v) {
+  const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;        // infinities and NaN set no scale
+}
+__device__ __forceinline__ void raise(unsigned* at, unsigned bits) { __hip_atomic_fetch_max(at, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ f32x4_t split_load(const SplitJob& p, long row, long col) {
   f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* at = p.src + row * p.ld + col;
@@ -565,8 +570,7 @@ __global__ __launch_bounds__(256) void split_scan_kernel(SplitJobs all) {
       const f32x4_t v = split_load(p, row, col);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const unsigned bits = __float_as_uint(v[r]) & 0x7fffffffu;
-        const unsigned f = bits < 0x7f800000u ? bits : 0u;    // infinities and NaN set no scale
+        const unsigned f = finite_bits(v[r]);
         top[r] = max(top[r], f);
         mine = max(mine, f);
       }
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(256) void split_scan_kernel(SplitJobs all) {
     if (p.row_top) {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) mine = max(mine, unsigned(__shfl_xor(int(mine), o, 64)));
-      if (lane == 0 && row < p.rows && mine) __hip_atomic_fetch_max(p.row_top + row, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (lane == 0 && row < p.rows && mine) raise(p.row_top + row, mine);
     }
   }
   if (!p.col_top) return;
@@ -584,7 +588,7 @@ __global__ __launch_bounds__(256) void split_scan_kernel(SplitJobs all) {
   const int c = threadIdx.x;
   const unsigned m = max(max(cols[0][c], cols[1][c]), max(cols[2][c], cols[3][c]));
   const long at = long(b % p.across) * kSplitCols + c;
-  if (at < p.n && m) __hip_atomic_fetch_max(p.col_top + at, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (at < p.n && m) raise(p.col_top + at, m);
 }
 __device__ __forceinline__ void split_store(_Float16* hi, long lo, f32x4_t v, const int e[4]) {
   Out4<_Float16> h, l;
@@ -618,6 +622,32 @@ __global__ __launch_bounds__(256) void split_kernel(SplitJobs all) {
       split_store(p.row_hi + row * p.n32 * 2 + (col & ~31L) * 2 + (col & 31), 32, v, e);
     }
     if (p.col_hi && row < p.rows32 && col < p.n8) split_store(p.col_hi + ((row & ~31L) * 2 + (row & 31)) * p.n8 + col, 32 * p.n8, v, ec);
+  }
+}
+
+// Halves by rows alone: a wave finds a row's largest value and reads the row again, from the caches (a scan of its
+// own, with tables to zero, took 40 us more in the forward of 4096 x 1024 x 2816).
+__global__ __launch_bounds__(256) void split_rows_kernel(SplitJobs all) {
+  const SplitJob& p = split_job(all);
+  const int lane = threadIdx.x & 63;
+  const long row = long(blockIdx.x - p.first) * 4 + (threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  unsigned mine = 0;
+#pragma unroll 4
+  for (long col = lane * 4; col < p.n; col += 256) {
+    const f32x4_t v = split_load(p, row, col);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mine = max(mine, finite_bits(v[r]));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mine = max(mine, unsigned(__shfl_xor(int(mine), o, 64)));
+  if (lane == 0) p.row_top[row] = mine;
+  const int x = exponent(mine), e[4] = {x, x, x, x};
+#pragma unroll 4
+  for (long col = lane * 4; col < p.n32; col += 256) {
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < p.n) v = split_load(p, row, col);
+    split_store(p.row_hi + row * p.n32 * 2 + (col & ~31L) * 2 + (col & 31), 32, v, e);
   }
 }
 
@@ -909,19 +939,13 @@ struct Halves {
   Side side;
   const unsigned* top;
 };
-// Takes tables and halves for the jobs of one pass, and runs scan and split over them.
+// Takes halves for the jobs of one pass, and runs them.  (The backward's first kernel finding the largest values of
+// its own results cost it 61 us where the scan takes 33, at 4096 x 1024 x 2816.)
 struct Splitter {
   Run& r;
   SplitJobs all{};
-  unsigned* tops = nullptr;     // tables of this pass, zeroed together
-  long n_tops = 0;
   explicit Splitter(Run& run) : r(run) {}
 
-  unsigned* table(unsigned* base, long n) {
-    unsigned* p = base ? base + n_tops : nullptr;
-    n_tops += align_up(n, 64);
-    return p;
-  }
   // by: 1 rows, 2 columns, 3 both; the tables' addresses are given (joint scales share one)
   SplitJob& add(const float* src, long ld, long rows, long n, unsigned* row_top, unsigned* col_top, int by) {
     SplitJob& j = all.j[all.n++];
@@ -933,19 +957,35 @@ struct Splitter {
     j.wide = !(uintptr_t(src) & 15) && ld % 4 == 0;
     return j;
   }
-  void run() {
-    unsigned grid = 0;
+  unsigned grid(bool by_rows) {
+    unsigned n = 0;
     for (int k = 0; k < all.n; ++k) {
       SplitJob& j = all.j[k];
-      j.first = grid;
-      j.across = unsigned((j.n32 + kSplitCols - 1) / kSplitCols);
-      grid += j.across * unsigned((j.rows + kSplitRows - 1) / kSplitRows);
+      j.first = n;
+      j.across = by_rows ? 1 : unsigned((j.n32 + kSplitCols - 1) / kSplitCols);
+      n += j.across * unsigned((j.rows + (by_rows ? 4 : kSplitRows) - 1) / (by_rows ? 4 : kSplitRows));
     }
-    if (!r.go) return;
-    hipLaunchKernelGGL(fill_kernel, dim3(unsigned((n_tops + 255) / 256)), dim3(256), 0, r.s, tops, n_tops);
-    if (!grid) return;
-    hipLaunchKernelGGL(split_scan_kernel, dim3(grid), dim3(256), 0, r.s, all);
-    hipLaunchKernelGGL(split_kernel, dim3(grid), dim3(256), 0, r.s, all);
+    return n;
+  }
+  // every job by rows alone
+  void run_rows() {
+    const unsigned n = grid(true);
+    if (r.go && n) hipLaunchKernelGGL(split_rows_kernel, dim3(n), dim3(256), 0, r.s, all);
+  }
+  void run() {
+    const unsigned n = grid(false);
+    if (!r.go || !n) return;
+    hipLaunchKernelGGL(split_scan_kernel, dim3(n), dim3(256), 0, r.s, all);
+    hipLaunchKernelGGL(split_kernel, dim3(n), dim3(256), 0, r.s, all);
+  }
+};
+// Tables of `n` values each, zeroed together.
+struct Tables {
+  unsigned *base, *end;
+  unsigned* take(long n) {
+    unsigned* p = end;
+    if (base) end += align_up(n, 64);
+    return p;
   }
 };
 Halves by_rows(const SplitJob& j) {
@@ -972,24 +1012,20 @@ Problem problem32(const Halves& a, const Halves& b, long m, long n, float* out, 
 
 hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r) {
   const long rows = d.rows, width = d.width, hidden = d.hidden, out = d.out, hp = align_up(hidden, 8);
-  const long n_tops = 2 * align_up(rows, 64) + 2 * align_up(hidden, 64) + align_up(out, 64);
-  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(n_tops) * 4));
+  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(2 * align_up(rows, 64) + 2 * align_up(hidden, 64) + align_up(out, 64)) * 4));
+  Tables t{base, base};
+  unsigned *tx = t.take(rows), *tg = t.take(hidden), *tu = t.take(hidden), *td = t.take(out), *th = t.take(rows);
   Splitter one(r);
-  one.tops = base;
-  unsigned *tx = one.table(base, rows), *tg = one.table(base, hidden), *tu = one.table(base, hidden), *td = one.table(base, out),
-           *th = one.table(base, rows);
   const Halves x = by_rows(one.add((const float*)d.x, d.ld_x, rows, width, tx, nullptr, 1));
   const Halves wg = by_rows(one.add((const float*)d.w_gate, d.ld_gate, hidden, width, tg, nullptr, 1));
   const Halves wu = by_rows(one.add((const float*)d.w_up, d.ld_up, hidden, width, tu, nullptr, 1));
   const Halves wd = by_rows(one.add((const float*)d.w_down, d.ld_down, out, hidden, td, nullptr, 1));
-  one.run();
+  one.run_rows();
   float* h = static_cast<float*>(r.a.take(size_t(rows) * hp * 4));
-  launch_gate<_Float16, float>(r, d, x.side, pair(wg, wu), halved(width), h, hp, Scales{tx, tg, tu, nullptr, nullptr});
+  launch_gate<_Float16, float>(r, d, x.side, pair(wg, wu), halved(width), h, hp, Scales{tx, tg, tu});
   Splitter two(r);
-  two.tops = th;       // zeroed twice: its table lies in the first pass's memory
-  two.n_tops = align_up(rows, 64);
   const Halves hh = by_rows(two.add(h, hp, rows, hidden, th, nullptr, 1));
-  two.run();
+  two.run_rows();
   Problems all{};
   all.n = 1;
   all.p[0] = problem32(hh, wd, rows, out, y, ld_y);
@@ -1000,13 +1036,13 @@ hipError_t forward_halves(const nerf_block_desc& d, float* y, long ld_y, Run& r)
 hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_dy, float* dx, long ld_dx, float* dwg, float* dwu,
                            float* dwd, Run& r) {
   const long rows = d.rows, width = d.width, hidden = d.hidden, out = d.out, hp = align_up(hidden, 8);
-  const long n1 = 2 * align_up(rows, 64) + 3 * align_up(hidden, 64) + 2 * align_up(width, 64) + align_up(out, 64);
-  const long n2 = align_up(rows, 64) + 3 * align_up(hidden, 64);
-  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(n1 + n2) * 4));
+  const long n_tops = 3 * align_up(rows, 64) + 6 * align_up(hidden, 64) + 2 * align_up(width, 64) + align_up(out, 64);
+  unsigned* base = static_cast<unsigned*>(r.a.take(size_t(n_tops) * 4));
+  Tables t{base, base};
+  unsigned *xr = t.take(rows), *xc = t.take(width), *gr = t.take(hidden), *ur = t.take(hidden), *wc = t.take(width), *dc = t.take(hidden),
+           *yr = t.take(rows), *yc = t.take(out), *tr = t.take(rows), *hc = t.take(hidden), *gc = t.take(hidden), *uc = t.take(hidden);
+  if (r.go) hipLaunchKernelGGL(fill_kernel, dim3(unsigned((n_tops + 255) / 256)), dim3(256), 0, r.s, base, n_tops);
   Splitter one(r);
-  one.tops = base;
-  unsigned *xr = one.table(base, rows), *xc = one.table(base, width), *gr = one.table(base, hidden), *ur = one.table(base, hidden),
-           *wc = one.table(base, width), *dc = one.table(base, hidden), *yr = one.table(base, rows), *yc = one.table(base, out);
   const SplitJob jx = one.add((const float*)d.x, d.ld_x, rows, width, xr, xc, 3);
   // dx adds the products of both weights: one table of their columns
   const SplitJob jg = one.add((const float*)d.w_gate, d.ld_gate, hidden, width, gr, wc, 3);
@@ -1021,9 +1057,6 @@ hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_
   launch_gate_back<_Float16, float>(r, d, x.side, pair(wg, wu), dy.side, wd.side, halved(width), halved(out), h, dg, du, hp,
                                     Scales{xr, gr, ur, yr, dc});
   Splitter two(r);
-  two.tops = base ? base + n1 : nullptr;
-  unsigned *tr = two.table(two.tops, rows), *hc = two.table(two.tops, hidden), *gc = two.table(two.tops, hidden),
-           *uc = two.table(two.tops, hidden);
   const SplitJob kh = two.add(h, hp, rows, hidden, nullptr, hc, 2);
   const SplitJob kg = two.add(dg, hp, rows, hidden, tr, gc, 3);      // one table of both gradients' rows
   const SplitJob ku = two.add(du, hp, rows, hidden, tr, uc, 3);
