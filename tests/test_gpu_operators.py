@@ -158,6 +158,50 @@ def test_block_long_sum_over_rows(dtype):
     _check_block(_block_case(dtype, 9001, 40, 56, 24), "silu")
 
 
+# tall products whose last tiles are cut along k: one of 513 or 514 tiles, and the 129th or 257th of which 128 or 256
+# are cut in two, on the larger tile (136 columns) and the smaller
+@pytest.mark.parametrize("dtype, rows, width, hidden", [(BF16, 65768, 136, 520), (F16, 65768, 40, 520), (F32, 65768, 136, 520),
+                                                        (F32, 32872, 40, 2056), (F32, 32872, 136, 2056)], ids=str)
+def test_block_tiles_in_parts(dtype, rows, width, hidden):
+    from nerf_amd.operators import gated_block, gated_block_backward
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _block_case(dtype, rows, width, hidden, width))
+    want = truth.block(x, wg, wu, wd, "silu", dy)
+    truth.within(gated_block(x, wg, wu, wd), *want["y"], "y")
+    got = gated_block_backward(dy, x, wg, wu, wd)
+    for name, g in zip(("dx", "dw_gate", "dw_up", "dw_down"), got):
+        truth.within(g, *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows, width, hidden, out", [(3001, 100, 300, 60), (9001, 40, 56, 24), (2100, 520, 1300, 520)])
+def test_block_any_choice_of_gradients(dtype, rows, width, hidden, out):
+    # fewer weight gradients share the machine otherwise, and may need more of the workspace
+    from nerf_amd.operators import gated_block_backward
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _block_case(dtype, rows, width, hidden, out))
+    want = truth.block(x, wg, wu, wd, "gelu", dy)
+    names = ("dx", "dw_gate", "dw_up", "dw_down")
+    for mask in range(1, 16):
+        needs = tuple(bool(mask >> i & 1) for i in range(4))
+        got = gated_block_backward(dy, x, wg, wu, wd, activation="gelu", needs=needs)
+        for name, wanted, g in zip(names, needs, got):
+            assert (g is not None) == wanted
+            if wanted:
+                truth.within(g, *want[name], f"{name} of {needs}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 31, 33, 64])
+@pytest.mark.parametrize("width, hidden, out", [(2049, 131, 17), (37, 1031, 300), (1000, 4099, 5)])
+def test_block_few_rows_of_odd_lengths(dtype, rows, width, hidden, out):
+    from nerf_amd.operators import gated_block
+
+    x, wg, wu, wd, _ = _block_case(dtype, rows, width, hidden, out)
+    want = truth.block(x, wg, wu, wd, "silu")
+    truth.within(gated_block(x.cuda(), wg.cuda(), wu.cuda(), wd.cuda()), *want["y"], "y")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows, pad", [(5, 3), (150, 3), (150, 8)])
 def test_block_strided_operands(dtype, rows, pad):
