@@ -3,7 +3,12 @@
 //   dh = dy Wd, du = dh act(g), dg = dh u act'(g)
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // g and u never reach memory: the forward's first kernel holds both accumulators of a tile and writes
-// h; the backward's first kernel recomputes them beside dh and writes h, dg and du.
+// h; the backward's first kernel recomputes them beside dh and writes h, dg and du (h, dg and du are what the
+// products after it sum over: each is read whole, so keeping g and u instead would move more bytes).
+// h, dg and du are rounded to the operands' type once, as operands of the next product; every sum is fp32.
+// Measured at 8192 x 4096 x 10240 bf16, both passes: 5.9 ms, 1270 TF/s, at the power limit (matrix units 57 to 71%
+// busy at 1.8 GHz); at 131072 x 256 x 512: 0.58 ms, where h, dg and du (1.3 GB in all) and the few steps of a
+// tile's sum bound it.
 #include <cmath>
 #include <type_traits>
 
@@ -61,8 +66,8 @@ __host__ __device__ inline void with_kind(int kind, F f) {
 }
 
 // ------------------------------------------------------------------ 16-bit types on the matrix cores --
-// The 256 x 256 tile of 8 waves carries long products; the 128 x 128 tile of 4 waves (two workgroups a CU)
-// fills the machine where there are few tiles.
+// The 256 x 256 tile of 8 waves reads each operand byte from LDS for twice the products, one workgroup a CU; the
+// 128 x 128 tile of 4 waves, two a CU, leaves less of the machine idle where tiles are few.
 typedef Tile<2, 4, 8, 4> Large;
 typedef Tile<2, 2, 4, 4> Small;
 
@@ -98,6 +103,8 @@ __device__ __forceinline__ void exponents(int (&e)[N], const unsigned* top, long
 // h = act(x Wg^T) (x Wu^T): the J tile holds TJ / 2 rows of Wg and the same rows of Wu, so a lane owns the
 // same (row, column) of both and the activation runs on accumulators.  h's columns behind `hidden` up to
 // its row stride are zeros: they are summed over by the next product.
+// 8192 x 4096 x 10240 bf16: 1054 us, 1304 TF/s, the matrix units' power; 131072 x 256 x 512: 104 us, four steps
+// a tile between its first operands' latency and its results.
 template <typename T, typename C, typename O, int KIND>
 __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
@@ -136,7 +143,9 @@ __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int 
 }
 
 // The backward's first kernel: g and u as above, then dh = dy Wd of the same tile in a third accumulator,
-// and h, dg and du of the tile from the three.
+// and h, dg and du of the tile from the three.  8192 x 4096 x 10240 bf16: 1.85 ms, 1110 TF/s: dh's half as wide
+// steps read LDS as long as they multiply (waves of 64 x 64 instead of 128 x 32 read less and spilled more: 1.95).
+// 131072 x 256 x 512: 211 us, 2.4 TB/s.
 template <typename T, typename C, typename O, int KIND>
 __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy,
                                                                  O* h, O* dg, O* du, long ld_h, long rows, long hidden,
@@ -308,6 +317,8 @@ struct Leave {
     }
   }
 };
+// 8192 x 4096 x 10240 bf16: y 540 us (1273 TF/s), dx 1056 (1301), the weights' gradients 1.73 ms (1194); torch's
+// product of 8192^3 reaches 1309, 1170 and 1022 with the operands as they lie there.
 template <typename T, typename C, bool IK, bool JK, typename O>
 __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
   constexpr bool HALVES = sizeof(O) == 4;
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
       for (int j = 0; j < C::NJ; ++j) to[(i * C::NJ + j) * C::NT + threadIdx.x] = acc[j][i];
   }
 }
-// workgroup: one fragment of every wave of one of the remaining tiles
+// workgroup: one fragment of every wave of one of the remaining tiles.  Bound by the partials' bytes (30 MiB: 9.4 us).
 template <typename C, typename O>
 __global__ __launch_bounds__(C::NT) void join_kernel(Problems all) {
   constexpr int kFrags = C::NI * C::NJ;
@@ -363,7 +374,7 @@ __global__ __launch_bounds__(C::NT) void join_kernel(Problems all) {
 }
 
 // Rows of `n` values copied to rows of a multiple of 8, zeros behind: operands whose rows are not whole
-// aligned 16-byte pieces.
+// aligned 16-byte pieces (1001 x 2730 fp16: 5.4 us, a launch's length).
 template <typename T>
 __global__ __launch_bounds__(256) void pad_kernel(const T* src, long ld, long rows, long n, T* dst, long ld_dst) {
   const long per = ld_dst / 8, e = long(blockIdx.x) * 256 + threadIdx.x;
@@ -389,6 +400,8 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long ld, long ro
 //            the rows of x, repeated in columns 8.. with their second half; up to 8 rows of x.
 // fp32 runs on the f32 matrix instruction at full precision: at a few rows it still outruns memory
 // (4 x 32 cycles a KiB of weights a SIMD).
+// One row of 2048 x 5120 bf16: 10.8 us (42 MB) and 6.0 us (21 MB), 3.7 TB/s: each wave has its loads in flight
+// for a latency or two, and the host's two launches take as long.
 enum { kRows, kGate, kHalves };
 template <typename T>
 struct FewStep {   // 16 bytes of k a lane: 32 values of k a step
@@ -511,11 +524,21 @@ void launch_few(const Few& p, hipStream_t s) {
   else if (p.rows <= 32) go(std::integral_constant<int, MODE == kHalves ? 1 : 2>{});
   else go(std::integral_constant<int, MODE == kHalves ? 1 : 4>{});
 }
-// h's row stride for few rows: whole 16-byte pieces
+// Whether the forward takes the path of few rows: up to 64 of them, four accumulators.  Every workgroup reads all of
+// x from L2, so its time grows with the rows and the tiles' does not; they meet where rows^2 x the weights' bytes
+// is near 1.1e11.  In us, few rows and tiles, bf16: 2048 x 5120 x 2048 at 32 rows 43 : 50, at 64 65 : 50; 4096 x
+// 10240 x 4096 at 16 rows 85 : 96, at 32 109 : 96; 512 x 1408 x 512 at 64 rows 14 : 22.  The tiles' halves of 32-bit
+// operands never win: 2048 x 5120 x 2048 at 64 rows 124 : 150, 4096 x 10240 x 4096 319 : 479.
 constexpr int kFewRows = 64;
+bool few_rows(const nerf_block_desc& d) {
+  const double bytes = (2.0 * d.width + d.out) * d.hidden * 2.0;
+  return d.rows <= kFewRows && (d.dtype == NERF_F32 || double(d.rows) * double(d.rows) * bytes <= 1.1e11);
+}
 
 // 32-bit matrices on their way to halves: the largest finite |value| of each row and / or column (bits in
-// zeroed tables; a maximum does not depend on the order of the atomics), then the halves by either.
+// zeroed tables; a maximum does not depend on the order of the atomics), then the halves by either.  Bound by
+// bytes: dg and du by rows and columns and h by columns, 3 x 4096 x 2816: 32 us for the scan (4.3 TB/s), 86 us for
+// the halves (4.3 TB/s).
 struct SplitJob {
   const float* src;
   long ld, rows, n;
@@ -705,7 +728,9 @@ double whole_time(long tiles, double steps) {
   const long full = tiles / slots<C>(), rest = tiles % slots<C>();
   return double(full) * wave_time<C>(slots<C>(), steps) + (rest ? wave_time<C>(rest, steps) : 0.0);
 }
-// The gate kernels: whole tiles only, `steps` of both phases.
+// The gate kernels: whole tiles only, `steps` of both phases.  Large and Small measured, in us, forward and
+// backward: 131072 x 256 x 512 bf16 105 : 114, 213 : 234; 1531 x 1000 x 2730 fp16 39 : 42, 61 : 70; 8192 x 4096 x
+// 10240 bf16 1029 : 1237, 1850 : 2643; 4096 x 1024 x 2816 fp32, 352 large tiles on 256 CUs, 152 : 133, 270 : 234.
 bool gate_large(long rows, long cols, long steps, double turns) {
   return whole_time<Large>(tiles_of(rows, cols, Large::TI, Large::TJ), steps * turns) <=
          whole_time<Small>(tiles_of(rows, cols, Small::TI, Small::TJ), steps * turns);
@@ -1113,7 +1138,7 @@ extern "C" {
 size_t nerf_gated_block_workspace(const nerf_block_desc* d, int backward) {
   if (check(d, "nerf_gated_block_workspace") != NERF_OK) return 0;
   Run r{nullptr, Arena{nullptr}, false};
-  if (!backward && d->rows <= kFewRows) {
+  if (!backward && few_rows(*d)) {
     if (d->dtype == NERF_F32) (void)forward_few<float>(*d, nullptr, 0, r);
     else (void)forward_few<__bf16>(*d, nullptr, 0, r);
   } else if (d->dtype == NERF_F32) {
@@ -1134,7 +1159,7 @@ int nerf_gated_block_forward(const nerf_block_desc* d, void* y, int64_t ld_y, vo
   if ((rc = check_workspace(d, 0, workspace, workspace_bytes, who)) != NERF_OK) return rc;
   const hipStream_t s = (hipStream_t)stream;
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
-  const bool few = d->rows <= kFewRows;
+  const bool few = few_rows(*d);
   const hipError_t e =
       d->dtype == NERF_F32        ? (few ? forward_few<float>(*d, (float*)y, ld_y, r) : forward_halves(*d, (float*)y, ld_y, r))
       : d->dtype == NERF_BFLOAT16 ? (few ? forward_few<__bf16>(*d, (__bf16*)y, ld_y, r) : forward_mma<__bf16>(*d, (__bf16*)y, ld_y, r))

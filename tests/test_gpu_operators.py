@@ -202,6 +202,16 @@ def test_block_few_rows_of_odd_lengths(dtype, rows, width, hidden, out):
     truth.within(gated_block(x.cuda(), wg.cuda(), wu.cuda(), wd.cuda()), *want["y"], "y")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("rows", [60, 64])
+def test_block_few_rows_and_wide_weights(dtype, rows):
+    # 16-bit weights of 30 MB: the path of few rows ends between these
+    from nerf_amd.operators import gated_block
+
+    x, wg, wu, wd, _ = (t.cuda() for t in _block_case(dtype, rows, 1600, 3150, 1560))
+    truth.within(gated_block(x, wg, wu, wd), *truth.block(x, wg, wu, wd, "silu")["y"], "y")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows, pad", [(5, 3), (150, 3), (150, 8)])
 def test_block_strided_operands(dtype, rows, pad):
