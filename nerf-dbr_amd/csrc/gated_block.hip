@@ -696,7 +696,8 @@ struct Matrix {
   long ld;      // elements
   long rows, n, n8;
 };
-bool whole(const void* p, long ld, long n) { return !(uintptr_t(p) & 15) && ld % 8 == 0 && n % 8 == 0; }
+// (a tile's 256 rows lie within the 32-bit offsets of its fetches)
+bool whole(const void* p, long ld, long n) { return !(uintptr_t(p) & 15) && ld % 8 == 0 && n % 8 == 0 && ld <= 1L << 22; }
 
 Side rows_side(const Matrix& m) {      // i = row, k = column
   Side s{};

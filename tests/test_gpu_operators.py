@@ -239,6 +239,24 @@ def test_block_strided_operands(dtype, rows, pad):
     assert (dx[:, :1] == 5).all() and (dx[:, 73:] == 5).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("rows", [3, 140])
+def test_block_rows_far_apart(dtype, rows):
+    # a tile's rows are 4.7 GB (bf16) and 9.4 GB apart: offsets that pass 32 bits
+    from nerf_amd.operators import gated_block, gated_block_backward
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _block_case(dtype, rows, 64, 96, 48))
+    step = (1 << 24) + 8
+    far = torch.empty(rows * step, dtype=dtype, device="cuda").as_strided((rows, 64), (step, 1))
+    far.copy_(x)
+    want = truth.block(x, wg, wu, wd, "silu", dy)
+    truth.within(gated_block(far, wg, wu, wd), *want["y"], "y")
+    for name, g in zip(("dx", "dw_gate", "dw_up", "dw_down"), gated_block_backward(dy, far, wg, wu, wd)):
+        truth.within(g, *want[name], name)
+    y = torch.empty(rows * step, dtype=dtype, device="cuda").as_strided((rows, 48), (step, 1))
+    truth.within(gated_block(x, wg, wu, wd, out=y), *want["y"], "y far apart")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_block_leading_dimensions_and_no_rows(dtype):
     from nerf_amd.operators import gated_block, gated_block_backward
