@@ -464,7 +464,7 @@ int nerf_gated_block_backward(const nerf_block_desc* desc, const void* dy, int64
  * advances on the device so that a captured call counts its replays; the gradient norm (max_norm
  * > 0 or NERF_ADAMW_SKIP_NONFINITE) and the steps skipped.  flags: NERF_ADAMW_SKIP_NONFINITE leaves
  * everything as it is when the norm is not finite (counted in control); NERF_ADAMW_WRITE_GRADS
- * stores the clipped gradients.  lr_device (device fp32, or NULL) replaces lr.
+ * stores the clipped gradients (no two may share memory then).  lr_device (device fp32, or NULL) replaces lr.
  * workspace: nerf_adamw_workspace(plan) bytes of device memory, 8-byte aligned. */
 #define NERF_ADAMW_BLOCK 256
 #define NERF_ADAMW_SKIP_NONFINITE 1

@@ -20,6 +20,12 @@ _NONE = type(None)
 _dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
 
 
+def _shared(tensors) -> bool:
+    """Whether two of the contiguous tensors share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 def blocks(numel: int) -> int:
     """Scales of an 8-bit moment of numel values."""
     return -(-int(numel) // BLOCK)
@@ -61,8 +67,7 @@ class AdamW:
                 raise ValueError(f"parameter {i} is on {p.device}, not on {device}")
         if not sum(p.numel() for p in self.params):
             raise ValueError("no values in the parameters")
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        if _shared(self.params):
             raise ValueError("parameters share memory (one is given twice?)")
         decay = [float(weight_decay)] * len(self.params) if np.ndim(weight_decay) == 0 else [float(w) for w in weight_decay]
         if len(decay) != len(self.params):
@@ -117,6 +122,9 @@ class AdamW:
         steps = int(state.pop("steps", 0))
         if state:
             raise ValueError(f"unknown state {sorted(state)}")
+        if _shared([*self.params, *self.exp_avg, *self.exp_avg_sq, *(self.exp_avg_scale or ()), *(self.exp_avg_sq_scale or ()),
+                    *(m for m in self.masters if m is not None)]):
+            raise ValueError("parameters and state share memory")
         self._control = torch.zeros(ctypes.sizeof(rt.AdamWControl) // 4, dtype=torch.int32, device=device)
         self._control[0] = steps
         self.grad_norm = self._control.view(torch.float32)[3]
@@ -186,6 +194,8 @@ class AdamW:
                                       or g.get_device() != index):
                     raise ValueError(f"gradient {i} {tuple(g.shape)} {g.dtype} on {g.device} must be contiguous, "
                                      f"{tuple(self._shapes[i])} and on {self.device}")
+        if self._config.flags & rt.NERF_ADAMW_WRITE_GRADS and _shared(given):
+            raise ValueError("gradients that are written share memory (one is given twice?)")
         addresses = np.fromiter(map(torch.Tensor.data_ptr, given), np.uint64, len(given))
         if len(set(kinds)) == 1:
             codes = np.full(len(given), self._grad[kinds[0]], np.int32)

@@ -467,6 +467,22 @@ def test_adamw_clipped_gradients_and_learning_rates():
     assert torch.allclose(p2.detach(), torch.full((4,), -1.0, device="cuda"), atol=1e-6)
 
 
+def test_adamw_refuses_what_shares_memory():
+    from nerf_amd.optim import AdamW
+
+    p = [torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")]
+    store = torch.zeros(900, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW(p, state=dict(exp_avg=[store[:300], store[299:599]]))
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW(p, state=dict(exp_avg=[store[:300], store[300:600]], exp_avg_sq=[store[600:], p[0]]))
+    g = torch.ones(300, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW(p, max_norm=1.0, write_grads=True).step([g, g])
+    AdamW(p, max_norm=1.0).step([g, g])       # read only: one gradient of two parameters
+    assert torch.equal(p[0], p[1]) and (p[0] != 0).all() and (g == 1).all()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_state_round_trip(bits):
     from nerf_amd.optim import AdamW
