@@ -38,6 +38,20 @@ struct Frag<_Float16> {
   static __device__ __forceinline__ f32x4_t mma(type a, type b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
+// fp32 without halves: a lane's 4 values of k go to 4 instructions of one k each, in the same order on both sides
+template <>
+struct Frag<float> {
+  typedef f32x4_t type;
+  static __device__ __forceinline__ f32x4_t mma(type a, type b, f32x4_t c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+    return c;
+  }
+};
+// values of k a step: 128 bytes of a row
+template <typename T>
+constexpr int step_k() { return 128 / int(sizeof(T)); }
+
 // 16 bytes per lane from its own address to LDS byte lds_base + lane * 16 (wave-uniform base in M0);
 // completion counts in vmcnt.  nerf_asm.h says why this is asm and who checks M0.
 __device__ __forceinline__ void lds_dma_16(const void* p, unsigned lds_base) {
@@ -69,14 +83,16 @@ struct Side {
   long k_n;   // extent of k: zeros behind it
 };
 
-// E: the tile's extent of the side; NT: threads; KC: k contiguous; PARTS: 2 = halves from two matrices
-template <int E, int NT, bool KC, int PARTS>
+// E: the tile's extent of the side; NT: threads; KC: k contiguous; PARTS: 2 = halves from two matrices; SZ: bytes of
+// a value (4: 32 values of k, and own contiguous 16-byte piece p of row k at piece p ^ turn(k >> 2))
+template <int E, int NT, bool KC, int PARTS, int SZ>
 struct Stage {
-  static constexpr int kBytes = E * 64 * 2;
+  static constexpr int kBytes = E * 128, kV = 16 / SZ;
   static constexpr int kChunks = E * 8 / NT;   // 16-byte pieces a thread fetches per step
   static_assert(PARTS == 1 || (KC && kChunks % 2 == 0), "a piece lies in one half");
   unsigned off[kChunks];                       // from the tile's first row (KC) or column
 
+  static __device__ __forceinline__ int turn(int g) { return ((g & 3) << 2) & (E / 4 - 1); }
   static __device__ __forceinline__ int gran(int k) { return ((k & 3) | (((k >> 3) & 3) << 2)) & (E / 16 - 1); }
   static __device__ __forceinline__ long half(int c) { return PARTS == 2 && c >= kChunks / 2; }
 
@@ -90,15 +106,16 @@ struct Stage {
         const long most = s.n - 1 - i0;       // behind the edge: the last row, its results are not stored
         off[c] = unsigned((rr < most ? rr : most) * s.ld) + chunk * 16;
       } else {
-        const int k = q / (E / 8), slot = q & (E / 8 - 1);
-        const long col = ((slot >> 1) ^ gran(k)) * 16 + (slot & 1) * 8, most = s.n - 8 - i0;
-        off[c] = unsigned(k * s.ld) + unsigned(col < most ? col : most) * 2;
+        const int k = q / (E / kV), slot = q & (E / kV - 1);
+        const long col = SZ == 2 ? ((slot >> 1) ^ gran(k)) * 16 + (slot & 1) * 8 : (slot ^ turn(k >> 2)) * 4;
+        const long most = s.n - kV - i0;
+        off[c] = unsigned(k * s.ld) + unsigned(col < most ? col : most) * SZ;
       }
     }
   }
   // where a segment's 64 values of k from k0 begin (uniform)
   __device__ __forceinline__ const char* base(const char* p, const Side& s, long i0, long k0) const {
-    return p + (KC ? i0 * s.ld + k0 * 2 : k0 * s.ld + i0 * 2);
+    return p + (KC ? i0 * s.ld + k0 * SZ : k0 * s.ld + i0 * SZ);
   }
   // fetch piece c of them into the stage at LDS byte `lds`; CHECKED: k may end inside
   template <bool CHECKED>
@@ -107,7 +124,7 @@ struct Stage {
     const char* at = from + (half(c) ? s.split : 0);
     if constexpr (CHECKED) {
       const int q = c * NT + threadIdx.x;
-      const long k = k0 + (KC ? ((q & 7) ^ ((q >> 3) & 7)) * 8 : q / (E / 8));
+      const long k = k0 + (KC ? ((q & 7) ^ ((q >> 3) & 7)) * kV : q / (E / kV));
       lds_dma_16(k < s.k_n ? at + off[c] : reinterpret_cast<const char*>(kZeros), to);
     } else {
       lds_dma_16_s(at, off[c], to);
@@ -127,9 +144,11 @@ struct Reader {
     if constexpr (KC) {
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) lane[ks] = (first + e) * 128 + (((4 * ks + g) ^ (e & 7)) << 4);
+    } else if constexpr (sizeof(T) == 4) {
+      lane[0] = 4 * g * (E * 4) + ((((first + e) >> 2) ^ Stage<E, 64, false, 1, 4>::turn(g)) << 4) + ((e & 3) << 2);
     } else {
       const int k = 8 * g + (e >> 2);
-      lane[0] = k * (E * 2) + (((first >> 4) ^ Stage<E, 64, false, 1>::gran(k)) << 5) + ((e & 3) << 3);
+      lane[0] = k * (E * 2) + (((first >> 4) ^ Stage<E, 64, false, 1, 2>::gran(k)) << 5) + ((e & 3) << 3);
     }
   }
   // rows: the fragment's distance in rows, known at compile time
@@ -137,6 +156,12 @@ struct Reader {
     if constexpr (KC) {
       const auto* p = (const __attribute__((address_space(3))) char*)(uintptr_t)(stage + lane[ks]);
       return *(const __attribute__((address_space(3))) F*)(p + rows * 128);
+    } else if constexpr (sizeof(T) == 4) {
+      const auto* p = (const __attribute__((address_space(3))) char*)(uintptr_t)((stage + lane[0]) ^ (unsigned(rows) << 2));
+      F v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = *(const __attribute__((address_space(3))) float*)(p + (ks * 16 + r) * (E * 4));
+      return v;
     } else {
       typedef __attribute__((address_space(3))) short4_t lds_short4;
       // the granule is an exclusive or with the lane's swizzle, and the fragment's number is in bits of
@@ -175,8 +200,8 @@ struct Tile {
 // three sums over k of their own they fetched and read half as much again).
 template <typename T, typename C, bool IK, bool JK, int PARTS, bool HALVES>
 struct Product {
-  typedef Stage<C::TI, C::NT, IK, 1> SI;
-  typedef Stage<C::TJ, C::NT, JK, PARTS> SJ;
+  typedef Stage<C::TI, C::NT, IK, 1, sizeof(T)> SI;
+  typedef Stage<C::TJ, C::NT, JK, PARTS, sizeof(T)> SJ;
   typedef typename Frag<T>::type F;
   static constexpr unsigned kStage = SI::kBytes + SJ::kBytes;
   static constexpr int kPieces = SI::kChunks + SJ::kChunks;
@@ -210,7 +235,7 @@ struct Product {
       if (++step == steps_per) step = 0, ++seg;
     };
     const auto fetch_all = [&](unsigned at) {
-      const long k0 = long(step) * 64;
+      const long k0 = long(step) * step_k<T>();
       const char *pa = a.base(si.p[seg], si, i0, k0), *pb = b.base(sj.p[seg], sj, j0, k0);
 #pragma unroll
       for (int c = 0; c < SI::kChunks; ++c) a.template fetch<true>(c, pa, si, k0, at);
@@ -230,7 +255,7 @@ struct Product {
     const auto one_step = [&](int t, auto more, auto fetching) {
       constexpr int kFetch = decltype(fetching)::value;
       const unsigned now = lds + (t & 1) * kStage, next = lds + (~t & 1) * kStage;
-      const long k0 = long(step) * 64;
+      const long k0 = long(step) * step_k<T>();
       const char *pa = nullptr, *pb = nullptr;
       if constexpr (kFetch != 0) pa = a.base(si.p[seg], si, i0, k0), pb = b.base(sj.p[seg], sj, j0, k0);
 #pragma unroll
@@ -275,7 +300,7 @@ struct Product {
     };
     // steps whose fetch is whole: all of them, or up to the first end of k inside a step (two counted loops:
     // one with the choice, or an exit, inside took new registers for every accumulator and spilled 390)
-    const long most = long(steps_per) * 64;
+    const long most = long(steps_per) * step_k<T>();
     const bool tail = si.k_n < most || sj.k_n < most;
     int quick = tail && steps_per - 1 - step < n - 2 ? steps_per - 1 - step : n - 2;
     int t = 0;

@@ -70,11 +70,14 @@ __host__ __device__ inline void with_kind(int kind, F f) {
 // 128 x 128 tile of 4 waves, two a CU, leaves less of the machine idle where tiles are few.
 typedef Tile<2, 4, 8, 4> Large;
 typedef Tile<2, 2, 4, 4> Small;
+// fp32 as it is: a step's instructions take 16 times as long, and sums over k are short of workgroups sooner than of
+// operands (128 rows of 2048 x 5120 x 2048, both passes: 521 us with Small, 356 with Tiny).
+typedef Tile<2, 2, 2, 2> Tiny;
 
 template <typename C>
 __host__ __device__ constexpr bool is_large() { return C::TI * C::TJ > 128 * 128; }
 template <typename C>
-__host__ __device__ constexpr long slots() { return is_large<C>() ? 256 : 512; }
+__host__ __device__ constexpr long slots() { return is_large<C>() ? 256 : C::TI == 128 ? 512 : 1024; }
 
 // LDS of a tile kernel: two stages, later the results of kRows rows (and all columns) of C columns
 template <typename C>
@@ -84,8 +87,8 @@ constexpr int larger(int a, int b) { return a > b ? a : b; }
 // 32-bit operands run on the f16 matrix cores as two halves each, x 2^e = hi + lo with e from the largest
 // value of the operand's row (or column, where the sum runs over rows), so that hi lies in [2^-14, 2^15] and
 // lo's rounding is 2^-25 of 2^15: x b ~ hi bh + hi bl + lo bh, 22 bits of every operand at a third of the
-// 16-bit rate.  The f32 matrix instruction carries 24 bits at a sixteenth.  The tables hold the largest
-// values' bits, index by row or column.
+// 16-bit rate.  The f32 matrix instruction carries 24 bits at a sixteenth (few rows and small blocks take it:
+// few_rows, direct).  The tables hold the largest values' bits, index by row or column.
 struct Scales {
   const unsigned *x, *wg, *wu, *dy, *wd;
 };
@@ -108,7 +111,7 @@ __device__ __forceinline__ void exponents(int (&e)[N], const unsigned* top, long
 template <typename T, typename C, typename O, int KIND>
 __global__ __launch_bounds__(C::NT, 2) void gate_mma_kernel(Side x, Side w, int steps, O* h, long ld_h, long rows,
                                                             long hidden, unsigned tiles_i, unsigned tiles_j, Scales sc) {
-  constexpr bool kHalved = sizeof(O) == 4;
+  constexpr bool kHalved = sizeof(O) == 4 && sizeof(T) == 2;
   typedef Out<O, C::TJ / 2> W;
   __shared__ __attribute__((aligned(1024))) char lds[larger(stages<C>(), C::TI * W::kRow)];
   unsigned ti, tj;
@@ -150,7 +153,7 @@ template <typename T, typename C, typename O, int KIND>
 __global__ __launch_bounds__(C::NT, 2) void gate_back_mma_kernel(Side x, Side w, Side dy, Side wd, int steps, int steps_dy,
                                                                  O* h, O* dg, O* du, long ld_h, long rows, long hidden,
                                                                  unsigned tiles_i, unsigned tiles_j, Scales sc) {
-  constexpr bool kHalved = sizeof(O) == 4;
+  constexpr bool kHalved = sizeof(O) == 4 && sizeof(T) == 2;
   typedef Tile<C::WI, C::WJ, C::NI, C::NJ / 2> Half;
   typedef Out<O, Half::TJ> W;
   // results of 4-byte types leave in two passes of half the rows; h and dg leave together, then du
@@ -268,7 +271,7 @@ __device__ __forceinline__ bool part_of(const Problems& all, unsigned b, int n, 
 // 32-bit results: the operands' scales taken out
 template <typename O>
 __device__ __forceinline__ f32x4_t scaled(const Problem& p, long row, long col, f32x4_t v) {
-  if (sizeof(O) == 4 && row < p.m) {
+  if (sizeof(O) == 4 && p.top_i && row < p.m) {
     const int e = exponent(p.top_i[row]);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -282,7 +285,7 @@ __device__ __forceinline__ const Problem& problem_of(const Problems& all, unsign
   return all.p[k];
 }
 // The accumulators of a whole tile to its place; the results of 4-byte types leave in two passes of half the rows.
-template <typename C, typename O>
+template <typename C, typename O, bool HALVES>
 struct Leave {
   typedef Out<O, C::TJ> W;
   static constexpr int kPasses = sizeof(O) == 4 ? 2 : 1, kRows = C::TI / kPasses;
@@ -292,7 +295,7 @@ struct Leave {
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, wi = wave / C::WJ;
     const int ib = wi * C::NI * 16 + (l & 15), jb = (wave % C::WJ) * C::NJ * 16 + (l >> 4) * 4;
     int er[C::NI], ec[C::NJ][4];
-    if constexpr (sizeof(O) == 4) {
+    if constexpr (HALVES) {
       exponents(er, p.top_i, i0 + ib, 16, p.m);
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) exponents(ec[j], p.top_j, j0 + jb + j * 16, 1, p.n);
@@ -306,7 +309,7 @@ struct Leave {
 #pragma unroll
           for (int j = 0; j < C::NJ; ++j) {
             f32x4_t v = acc[j][i];
-            if constexpr (sizeof(O) == 4)
+            if constexpr (HALVES)
 #pragma unroll
               for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], er[i] + ec[j][r]);
             W::put(lds, ib + i * 16 - pass * kRows, jb + j * 16, v);
@@ -321,8 +324,8 @@ struct Leave {
 // product of 8192^3 reaches 1309, 1170 and 1022 with the operands as they lie there.
 template <typename T, typename C, bool IK, bool JK, typename O>
 __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
-  constexpr bool HALVES = sizeof(O) == 4;
-  __shared__ __attribute__((aligned(1024))) char lds[Leave<C, O>::kLds];
+  constexpr bool HALVES = sizeof(O) == 4 && sizeof(T) == 2;
+  __shared__ __attribute__((aligned(1024))) char lds[Leave<C, O, HALVES>::kLds];
   const unsigned tile = near(blockIdx.x, gridDim.x, slots<C>());
   const Problem& p = problem_of(all, tile);
   unsigned ti, tj;
@@ -330,7 +333,7 @@ __global__ __launch_bounds__(C::NT, 2) void product_mma_kernel(Problems all) {
   const long i0 = long(ti) * C::TI, j0 = long(tj) * C::TJ;
   f32x4_t acc[C::NJ][C::NI] = {};
   accumulate<T, C, IK, JK, 1, HALVES>(acc, p.i, p.j, i0, j0, all.steps, 0, all.total, lds_addr(lds));
-  Leave<C, O>::run(lds, p, i0, j0, acc);
+  Leave<C, O, HALVES>::run(lds, p, i0, j0, acc);
 }
 template <typename T, typename C, bool IK, bool JK, bool HALVES>
 __global__ __launch_bounds__(C::NT, 2) void parts_mma_kernel(Problems all) {
@@ -699,30 +702,35 @@ struct Matrix {
 // (a tile's 256 rows lie within the 32-bit offsets of its fetches)
 bool whole(const void* p, long ld, long n) { return !(uintptr_t(p) & 15) && ld % 8 == 0 && n % 8 == 0 && ld <= 1L << 22; }
 
+template <typename T>
 Side rows_side(const Matrix& m) {      // i = row, k = column
   Side s{};
-  s.p[0] = static_cast<const char*>(m.p), s.ld = m.ld * 2, s.n = m.rows, s.k_n = m.n8;
+  s.p[0] = static_cast<const char*>(m.p), s.ld = m.ld * long(sizeof(T)), s.n = m.rows, s.k_n = m.n8;
   return s;
 }
+template <typename T>
 Side columns_side(const Matrix& m) {   // i = column, k = row
   Side s{};
-  s.p[0] = static_cast<const char*>(m.p), s.ld = m.ld * 2, s.n = m.n8, s.k_n = m.rows;
+  s.p[0] = static_cast<const char*>(m.p), s.ld = m.ld * long(sizeof(T)), s.n = m.n8, s.k_n = m.rows;
   return s;
 }
 
-// What a launch is expected to take, in microseconds, from whole launches of either tile: a step where every
-// workgroup slot is taken (8192 x 4096 x 10240: 1.7) and where a CU runs one workgroup alone and waits for its
-// operands, what a tile costs besides, a join, and a MiB of partials written or read.
-constexpr double kFullLarge = 1.7, kFullSmall = 1.1, kAloneLarge = 1.45, kAloneSmall = 0.8, kTileLarge = 7.0, kTileSmall = 5.0;
+// What a launch is expected to take, in microseconds, from whole launches of each tile: a step where every
+// workgroup slot is taken (Large at 8192 x 4096 x 10240: 1.7) and where a CU runs one workgroup alone and waits for
+// its operands, what a tile costs besides, a join, and a MiB of partials written or read.
+struct Cost {
+  double full, alone, tile;
+};
+template <typename C>
+constexpr Cost cost() { return is_large<C>() ? Cost{1.7, 1.45, 7.0} : C::TI == 128 ? Cost{1.1, 0.8, 5.0} : Cost{1.9, 0.6, 4.0}; }
 constexpr double kJoin = 5.0, kMiB = 0.2;
 constexpr long kPiece = 8;   // steps: less is mostly a tile's costs
 long tiles_of(long m, long n, long ti, long tj) { return ((m + ti - 1) / ti) * ((n + tj - 1) / tj); }
 // `n` workgroups of `steps` steps at a time
 template <typename C>
 double wave_time(long n, double steps) {
-  const double full = is_large<C>() ? kFullLarge : kFullSmall, alone = is_large<C>() ? kAloneLarge : kAloneSmall;
-  const double part = full * double(n) / double(slots<C>());
-  return steps * (part > alone ? part : alone) + (is_large<C>() ? kTileLarge : kTileSmall);
+  const double part = cost<C>().full * double(n) / double(slots<C>());
+  return steps * (part > cost<C>().alone ? part : cost<C>().alone) + cost<C>().tile;
 }
 template <typename C>
 double whole_time(long tiles, double steps) {
@@ -736,9 +744,12 @@ bool gate_large(long rows, long cols, long steps, double turns) {
   return whole_time<Large>(tiles_of(rows, cols, Large::TI, Large::TJ), steps * turns) <=
          whole_time<Small>(tiles_of(rows, cols, Small::TI, Small::TJ), steps * turns);
 }
-// 32-bit results: a step of halves carries three products instead of two
-template <typename O>
-constexpr double turns() { return sizeof(O) == 4 ? 1.5 : 1.0; }
+// 32-bit results from halves: a step carries three products instead of two
+template <typename T, typename O>
+constexpr double turns() { return sizeof(O) == 4 && sizeof(T) == 2 ? 1.5 : 1.0; }
+
+template <typename T>
+int steps_of(long k) { return int((k + step_k<T>() - 1) / step_k<T>()); }
 
 struct Run {
   hipStream_t s;
@@ -802,21 +813,24 @@ struct Run {
   }
   template <typename T, bool IK, bool JK, typename O, typename C>
   size_t products_of(Problems& all) {
-    const size_t bytes = share_bytes<C>(all, turns<O>());
+    const size_t bytes = share_bytes<C>(all, turns<T, O>());
     if (!go || !all.tiles) return bytes;
     all.part = reinterpret_cast<float*>(a.base + a.used);
     if (all.whole) hipLaunchKernelGGL((product_mma_kernel<T, C, IK, JK, O>), dim3(all.whole), dim3(C::NT), 0, s, all);
     if (all.even) {
-      hipLaunchKernelGGL((parts_mma_kernel<T, C, IK, JK, sizeof(O) == 4>), dim3(all.even * all.cuts), dim3(C::NT), 0, s, all);
+      hipLaunchKernelGGL((parts_mma_kernel<T, C, IK, JK, sizeof(O) == 4 && sizeof(T) == 2>), dim3(all.even * all.cuts), dim3(C::NT), 0, s, all);
       hipLaunchKernelGGL((join_kernel<C, O>), dim3((all.tiles - all.whole) * C::NI * C::NJ), dim3(C::NT), 0, s, all);
     }
     return bytes;
   }
   template <typename T, bool IK, bool JK, typename O>
   size_t products_one(Problems& all, long k, int segs) {
-    all.steps = int((k + 63) / 64), all.total = all.steps * segs;
-    const double large = share<Large>(all, turns<O>()), small = share<Small>(all, turns<O>());
-    return large <= small ? products_of<T, IK, JK, O, Large>(all) : products_of<T, IK, JK, O, Small>(all);
+    all.steps = steps_of<T>(k), all.total = all.steps * segs;
+    if constexpr (sizeof(T) == 4) return products_of<T, IK, JK, O, Tiny>(all);
+    else {
+      const double large = share<Large>(all, turns<T, O>()), small = share<Small>(all, turns<T, O>());
+      return large <= small ? products_of<T, IK, JK, O, Large>(all) : products_of<T, IK, JK, O, Small>(all);
+    }
   }
   template <typename T, bool IK, bool JK, typename O>
   void products(const Problems& all, long k, int segs) {
@@ -850,8 +864,9 @@ Pair weights(Run& r, const nerf_block_desc& d) {
     return {{d.w_gate, d.ld_gate, d.hidden, d.width, n8}, {d.w_up, d.ld_up, d.hidden, d.width, n8}};
   return {r.padded<T>(d.w_gate, d.ld_gate, d.hidden, d.width), r.padded<T>(d.w_up, d.ld_up, d.hidden, d.width)};
 }
+template <typename T>
 Side halves(const Pair& w) {
-  Side s = rows_side(w.g);
+  Side s = rows_side<T>(w.g);
   s.split = static_cast<const char*>(w.u.p) - static_cast<const char*>(w.g.p);
   return s;
 }
@@ -861,7 +876,6 @@ dim3 gate_grid(long rows, long hidden, unsigned& ti, unsigned& tj) {
   ti = unsigned((rows + C::TI - 1) / C::TI), tj = unsigned((hidden + C::TJ / 2 - 1) / (C::TJ / 2));
   return dim3(ti * tj);
 }
-int steps_of(long k) { return int((k + 63) / 64); }
 
 template <typename T, typename O>
 void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w, long k, O* h, long hp, const Scales& sc) {
@@ -871,11 +885,12 @@ void launch_gate(Run& r, const nerf_block_desc& d, const Side& x, const Side& w,
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
     with_kind(d.activation, [&](auto kind) {
-      hipLaunchKernelGGL((gate_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, steps_of(k), h, hp,
+      hipLaunchKernelGGL((gate_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, steps_of<T>(k), h, hp,
                          long(d.rows), long(d.hidden), ti, tj, sc);
     });
   };
-  if (gate_large(d.rows, 2 * hp, steps_of(k), turns<O>())) go(Large{});
+  if constexpr (sizeof(T) == 4) go(Tiny{});
+  else if (gate_large(d.rows, 2 * hp, steps_of<T>(k), turns<T, O>())) go(Large{});
   else go(Small{});
 }
 template <typename T, typename O>
@@ -887,11 +902,12 @@ void launch_gate_back(Run& r, const nerf_block_desc& d, const Side& x, const Sid
     typedef decltype(tile) C;
     const dim3 grid = gate_grid<C>(d.rows, hp, ti, tj);
     with_kind(d.activation, [&](auto kind) {
-      hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of(k),
-                         steps_of(k_dy), h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
+      hipLaunchKernelGGL((gate_back_mma_kernel<T, C, O, decltype(kind)::value>), grid, dim3(C::NT), 0, r.s, x, w, dy, wd, steps_of<T>(k),
+                         steps_of<T>(k_dy), h, dg, du, hp, long(d.rows), long(d.hidden), ti, tj, sc);
     });
   };
-  if (gate_large(d.rows, 2 * hp, steps_of(k) + steps_of(k_dy), turns<O>())) go(Large{});
+  if constexpr (sizeof(T) == 4) go(Tiny{});
+  else if (gate_large(d.rows, 2 * hp, steps_of<T>(k) + steps_of<T>(k_dy), turns<T, O>())) go(Large{});
   else go(Small{});
 }
 
@@ -921,10 +937,10 @@ hipError_t forward_mma(const nerf_block_desc& d, T* y, long ld_y, Run& r) {
   const Pair w = weights<T>(r, d);
   const Matrix wd = r.matrix<T>(d.w_down, d.ld_down, d.out, hidden);
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  launch_gate<T, T>(r, d, rows_side(x), halves(w), d.width, h, hp, Scales{});
+  launch_gate<T, T>(r, d, rows_side<T>(x), halves<T>(w), d.width, h, hp, Scales{});
   Problems all{};
   all.n = 1;
-  all.p[0] = problem<T>(rows_side(Matrix{h, hp, rows, hidden, hp}), rows_side(wd), rows, d.out, y, ld_y);
+  all.p[0] = problem<T>(rows_side<T>(Matrix{h, hp, rows, hidden, hp}), rows_side<T>(wd), rows, d.out, y, ld_y);
   r.products<T, true, true, T>(all, hidden, 1);
   return hipGetLastError();
 }
@@ -940,10 +956,10 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
   T* h = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* dg = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
   T* du = static_cast<T*>(r.a.take(size_t(rows) * hp * sizeof(T)));
-  launch_gate_back<T, T>(r, d, rows_side(x), halves(w), rows_side(dy), columns_side(wd), width, out, h, dg, du, hp, Scales{});
+  launch_gate_back<T, T>(r, d, rows_side<T>(x), halves<T>(w), rows_side<T>(dy), columns_side<T>(wd), width, out, h, dg, du, hp, Scales{});
   const Matrix mh{h, hp, rows, hidden, hp}, mg{dg, hp, rows, hidden, hp}, mu{du, hp, rows, hidden, hp};
   if ((dx || !r.go) && rows) {
-    Side i = rows_side(mg), j = columns_side(w.g);
+    Side i = rows_side<T>(mg), j = columns_side<T>(w.g);
     i.p[1] = reinterpret_cast<const char*>(du);
     j.p[1] = static_cast<const char*>(w.u.p);
     Problems all{};
@@ -952,9 +968,9 @@ hipError_t backward_mma(const nerf_block_desc& d, const void* dy_p, long ld_dy, 
     r.products<T, true, false, T>(all, hidden, 2);
   }
   Problems all{};
-  if (dwg || !r.go) all.p[all.n++] = problem<T>(columns_side(mg), columns_side(x), hidden, width, dwg, width);
-  if (dwu || !r.go) all.p[all.n++] = problem<T>(columns_side(mu), columns_side(x), hidden, width, dwu, width);
-  if (dwd || !r.go) all.p[all.n++] = problem<T>(columns_side(dy), columns_side(mh), out, hidden, dwd, hidden);
+  if (dwg || !r.go) all.p[all.n++] = problem<T>(columns_side<T>(mg), columns_side<T>(x), hidden, width, dwg, width);
+  if (dwu || !r.go) all.p[all.n++] = problem<T>(columns_side<T>(mu), columns_side<T>(x), hidden, width, dwu, width);
+  if (dwd || !r.go) all.p[all.n++] = problem<T>(columns_side<T>(dy), columns_side<T>(mh), out, hidden, dwd, hidden);
   if (all.n) r.products<T, false, false, T>(all, rows, 1);
   return hipGetLastError();
 }
@@ -1104,6 +1120,14 @@ hipError_t backward_halves(const nerf_block_desc& d, const float* dy_p, long ld_
   return hipGetLastError();
 }
 
+// fp32 as it is, on the f32 matrix instruction, where the halves' passes over the weights and their launches cost
+// more than a third of the instructions' time saves.  As it is and in halves, in us, forward + backward: 2048 x 5120
+// x 2048 at 128 rows 105 + 251 : 152 + 364, at 256 152 + 393 : 163 + 391, at 400 257 + 655 : 195 + 452; 512 x 1408 x
+// 512 at 256 rows 27 + 62 : 46 + 122, at 800 52 + 122 : 47 + 147.
+bool direct(const nerf_block_desc& d) {
+  return d.rows <= 256 || double(d.rows) * (2.0 * d.width + d.out) * d.hidden <= 2e9;
+}
+
 int check(const nerf_block_desc* d, const char* who) {
   if (!d) return set_error(NERF_E_INVALID, "%s: null descriptor", who);
   if (d->dtype != NERF_F32 && d->dtype != NERF_BFLOAT16 && d->dtype != NERF_FLOAT16) return set_error(NERF_E_INVALID, "%s: dtype %d", who, d->dtype);
@@ -1142,6 +1166,9 @@ size_t nerf_gated_block_workspace(const nerf_block_desc* d, int backward) {
   if (!backward && few_rows(*d)) {
     if (d->dtype == NERF_F32) (void)forward_few<float>(*d, nullptr, 0, r);
     else (void)forward_few<__bf16>(*d, nullptr, 0, r);
+  } else if (d->dtype == NERF_F32 && direct(*d)) {
+    if (backward) (void)backward_mma<float>(*d, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, r);
+    else (void)forward_mma<float>(*d, nullptr, 0, r);
   } else if (d->dtype == NERF_F32) {
     if (backward) (void)backward_halves(*d, nullptr, d->out, nullptr, 0, nullptr, nullptr, nullptr, r);
     else (void)forward_halves(*d, nullptr, 0, r);
@@ -1162,7 +1189,9 @@ int nerf_gated_block_forward(const nerf_block_desc* d, void* y, int64_t ld_y, vo
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
   const bool few = few_rows(*d);
   const hipError_t e =
-      d->dtype == NERF_F32        ? (few ? forward_few<float>(*d, (float*)y, ld_y, r) : forward_halves(*d, (float*)y, ld_y, r))
+      d->dtype == NERF_F32        ? (few            ? forward_few<float>(*d, (float*)y, ld_y, r)
+                                     : direct(*d) ? forward_mma<float>(*d, (float*)y, ld_y, r)
+                                                  : forward_halves(*d, (float*)y, ld_y, r))
       : d->dtype == NERF_BFLOAT16 ? (few ? forward_few<__bf16>(*d, (__bf16*)y, ld_y, r) : forward_mma<__bf16>(*d, (__bf16*)y, ld_y, r))
                                   : (few ? forward_few<_Float16>(*d, (_Float16*)y, ld_y, r) : forward_mma<_Float16>(*d, (_Float16*)y, ld_y, r));
   if (e != hipSuccess) return set_error(NERF_E_HIP, "%s: %s", who, hipGetErrorString(e));
@@ -1184,7 +1213,9 @@ int nerf_gated_block_backward(const nerf_block_desc* d, const void* dy, int64_t 
   const hipStream_t s = (hipStream_t)stream;
   Run r{s, Arena{static_cast<char*>(workspace)}, true};
   const hipError_t e =
-      d->dtype == NERF_F32 ? backward_halves(*d, (const float*)dy, ld_dy, (float*)dx, ld_dx, (float*)dw_gate, (float*)dw_up, (float*)dw_down, r)
+      d->dtype == NERF_F32 && direct(*d)
+          ? backward_mma<float>(*d, dy, ld_dy, (float*)dx, ld_dx, (float*)dw_gate, (float*)dw_up, (float*)dw_down, r)
+      : d->dtype == NERF_F32 ? backward_halves(*d, (const float*)dy, ld_dy, (float*)dx, ld_dx, (float*)dw_gate, (float*)dw_up, (float*)dw_down, r)
       : d->dtype == NERF_BFLOAT16
           ? backward_mma<__bf16>(*d, dy, ld_dy, (__bf16*)dx, ld_dx, (__bf16*)dw_gate, (__bf16*)dw_up, (__bf16*)dw_down, r)
           : backward_mma<_Float16>(*d, dy, ld_dy, (_Float16*)dx, ld_dx, (_Float16*)dw_gate, (_Float16*)dw_up, (_Float16*)dw_down, r);

@@ -310,6 +310,57 @@ def test_block_scales_of_32_bits(scale):
         truth.within(g, *want[name], name)
 
 
+# fp32 large enough for its operands to be split in halves: odd sizes, values far from 1, columns and rows of their own size
+@pytest.mark.parametrize("rows, width, hidden, out, kind, scale", [
+    (300, 2301, 1999, 777, "gelu", 1.0), (5000, 333, 1301, 129, "silu", 1.0), (2600, 640, 648, 640, "relu", 1e-12),
+    (2600, 640, 648, 640, "relu", 1e9)])
+def test_block_halves_of_32_bits(rows, width, hidden, out, kind, scale):
+    from nerf_amd.operators import gated_block, gated_block_backward
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _block_case(F32, rows, width, hidden, out))
+    x, wd = x * scale, wd / scale
+    x[::7] *= 1e-3
+    dy[::5] *= 1e4
+    wu[3::11] *= 1e-5
+    want = truth.block(x, wg, wu, wd, kind, dy)
+    truth.within(gated_block(x, wg, wu, wd, activation=kind), *want["y"], "y")
+    first = gated_block_backward(dy, x, wg, wu, wd, activation=kind)
+    for name, g in zip(("dx", "dw_gate", "dw_up", "dw_down"), first):
+        truth.within(g, *want[name], name)
+    again = gated_block_backward(dy, x, wg, wu, wd, activation=kind)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_block_halves_nonfinite_rows_and_replays():
+    from nerf_amd.operators import gated_block, gated_block_backward
+
+    rows = 1700
+    x, wg, wu, wd, dy = (t.cuda() for t in _block_case(F32, rows, 640, 648, 640))
+    bad = x.clone()
+    bad[1, 5] = float("inf")
+    bad[2, 9] = float("nan")
+    y = gated_block(bad, wg, wu, wd)
+    clean = [r for r in range(rows) if r not in (1, 2)]
+    assert y[2].isnan().all() and not y[1].isfinite().any()
+    truth.within(y[clean], *truth.block(x[clean], wg, wu, wd, "silu")["y"], "clean rows")
+    xin = x.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        gated_block_backward(dy, xin, wg, wu, wd)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (gated_block(xin, wg, wu, wd), *gated_block_backward(dy, xin, wg, wu, wd))
+    for i in range(4):
+        now = x * (1 + 0.5 * i)
+        xin.copy_(now)
+        graph.replay()
+        want = (gated_block(now, wg, wu, wd), *gated_block_backward(dy, now, wg, wu, wd))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
 def test_block_is_deterministic_and_follows_its_stream():
     from nerf_amd.operators import gated_block, gated_block_backward
 
