@@ -1,5 +1,5 @@
-// The tiled 16-bit matrix product under the gated block: C(i, j) = sum over k of I(i, k) J(j, k), fp32
-// accumulators, on v_mfma_f32_16x16x32.
+// The tiled matrix product under the gated block: C(i, j) = sum over k of I(i, k) J(j, k), fp32
+// accumulators, on v_mfma_f32_16x16x32 (16-bit operands) or v_mfma_f32_16x16x4 (fp32).
 //
 // A side (I or J) is read as it lies: k contiguous (rows of x, of a weight) or its own index contiguous
 // (the same rows when the sum runs over them); no operand is transposed in memory.  64 values of k of
